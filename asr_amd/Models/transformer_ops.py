@@ -1,0 +1,140 @@
+"""Differentiable operators of Transformer-style encoder layers on the HIP kernels.
+
+    q, k = qk_norm_rope(q, k, q_weight, k_weight)      # per-head RMS norm and rotary positions
+
+Not in the reference, which has sinusoidal relative positions and a plain Swish block in these places
+(Models/Transformer_encoder.py:55-137,191-209); ``ConformerEncoderLayer`` takes them as options.  Tensors are float32,
+bfloat16 or float16 on the GPU, all of one type unless said otherwise; anything else raises.  Layouts are (batch, frame,
+head, width); a head must be contiguous, the other strides are free (views of one packed projection need no copy).
+Calls enqueue on the current stream of the tensors' device and return without synchronising; gradients are computed by
+kernels too, without atomics: the same call gives the same bits.
+"""
+import contextlib
+import ctypes as C
+
+import torch
+
+from .. import _lib
+from .._lib import check
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _on(device):
+    """The tensors' device as the current one for the launches inside."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _tensor(who, name, t, dim, like=None, dtype=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"asr_amd.{who}: {name} must be a tensor on the GPU; the HIP path has no CPU fallback")
+    want = dtype if dtype is not None else like.dtype if like is not None else None
+    if want is None and t.dtype not in _DTYPES:
+        raise RuntimeError(f"asr_amd.{who}: {name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if want is not None and t.dtype != want:
+        raise RuntimeError(f"asr_amd.{who}: {name} must be {want}, got {t.dtype}")
+    if t.dim() != dim:
+        raise RuntimeError(f"asr_amd.{who}: {name} must have {dim} dimensions, got {tuple(t.shape)}")
+    if like is not None and t.device != like.device:
+        raise RuntimeError(f"asr_amd.{who}: {name} is on {t.device}, expected {like.device}")
+
+
+def _heads(t):
+    """t with contiguous heads: itself, or a copy."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+# ----------------------------------------------------------------------------------------- norm and rotation --
+def _rope_args(q, k, wq, wk, pos, rot, base, eps):
+    B, T, H, D = q.shape
+    a = _lib.RopeArgs()
+    a.q, a.k, a.wq, a.wk = q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr()
+    a.q_sb, a.q_st, a.q_sh, _ = q.stride()
+    a.k_sb, a.k_st, a.k_sh, _ = k.stride()
+    if pos is not None:
+        a.pos, a.pos_sb = pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0
+    a.B, a.T, a.H, a.Hk, a.D, a.rot, a.dtype = B, T, H, k.shape[2], D, rot, _DTYPES[q.dtype]
+    a.eps, a.base = eps, base
+    return a
+
+
+def _rope_fwd(q, k, wq, wk, pos, rot, base, eps):
+    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    ko = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    if qo.numel():
+        a = _rope_args(q, k, wq, wk, pos, rot, base, eps)
+        a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
+        with _on(q.device):
+            check(_lib.load().asr_qk_norm_rope_fwd(C.byref(a), _stream(q.device)))
+    return qo, ko
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, pos, rot, base, eps):
+        ctx.save_for_backward(q, k, wq, wk, pos)
+        ctx.aux = (rot, base, eps)
+        return _rope_fwd(q, k, wq, wk, pos, rot, base, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, wq, wk, pos = ctx.saved_tensors
+        lib = _lib.load()
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        if not q.numel():
+            return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk), None, None, None, None
+        gq, gk = _heads(gq), _heads(gk)
+        D = q.shape[-1]
+        dw = torch.empty(2, D, device=q.device, dtype=torch.float32)
+        ws = torch.empty(int(lib.asr_qk_norm_rope_ws_floats(D)), device=q.device, dtype=torch.float32)
+        a = _rope_args(q, k, wq, wk, pos, *ctx.aux)
+        a.gq, a.gk, a.q_out, a.k_out = gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr()
+        a.gq_sb, a.gq_st, a.gq_sh, _ = gq.stride()
+        a.gk_sb, a.gk_st, a.gk_sh, _ = gk.stride()
+        a.dwq, a.dwk, a.ws = dw[0].data_ptr(), dw[1].data_ptr(), ws.data_ptr()
+        with _on(q.device):
+            check(lib.asr_qk_norm_rope_bwd(C.byref(a), _stream(q.device)))
+        return dq, dk, dw[0], dw[1], None, None, None, None
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions=None, rot_dim=None, base=10000.0, eps=1e-6):
+    """Root-mean-square norm of every head of q (B, T, H, D) and k (B, T, Hk, D), times q_weight / k_weight (D, float32),
+    then the rotation by position in the same pass: elements p and p + rot_dim / 2 turn by
+    position * base ** (-2 p / rot_dim); elements from rot_dim (default D) on only pass the norm.  ``positions``: whole
+    numbers (T,) or (B, T) on the GPU, by default 0..T-1; for single new frames of long streams the stream's own (angles
+    are reduced in float64).  D even, at most 128.  Returns contiguous (q, k), differentiable in all four tensors."""
+    who = "qk_norm_rope"
+    _tensor(who, "q", q, 4)
+    _tensor(who, "k", k, 4, like=q)
+    _tensor(who, "q_weight", q_weight, 1, like=q, dtype=torch.float32)
+    _tensor(who, "k_weight", k_weight, 1, like=q, dtype=torch.float32)
+    B, T, H, D = q.shape
+    if k.shape[0] != B or k.shape[1] != T or k.shape[3] != D:
+        raise RuntimeError(f"asr_amd.{who}: q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
+    if q_weight.shape[0] != D or k_weight.shape[0] != D:
+        raise RuntimeError(f"asr_amd.{who}: the weights must hold one value for each of a head's {D} elements")
+    if D % 2 or not 2 <= D <= 128:
+        raise RuntimeError(f"asr_amd.{who}: head width {D}: must be even and in [2, 128]")
+    rot = D if rot_dim is None else int(rot_dim)
+    if rot % 2 or not 0 <= rot <= D:
+        raise RuntimeError(f"asr_amd.{who}: rot_dim {rot}: must be even and in [0, {D}]")
+    if not base > 0.0 or not eps >= 0.0:
+        raise RuntimeError(f"asr_amd.{who}: base must be positive and eps not negative")
+    pos = positions
+    if pos is not None:
+        if not isinstance(pos, torch.Tensor) or pos.device != q.device or pos.dtype not in (torch.int64, torch.int32):
+            raise RuntimeError(f"asr_amd.{who}: positions must be a tensor of whole numbers on {q.device}")
+        if tuple(pos.shape) not in ((T,), (B, T)):
+            raise RuntimeError(f"asr_amd.{who}: positions must be ({T},) or ({B}, {T}), got {tuple(pos.shape)}")
+        if pos.dtype != torch.int64 or (T > 1 and pos.stride(-1) != 1):
+            pos = pos.long().contiguous()
+    q, k, q_weight, k_weight = _heads(q), _heads(k), q_weight.contiguous(), k_weight.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, pos, rot, float(base), float(eps))
+    return _rope_fwd(q, k, q_weight, k_weight, pos, rot, float(base), float(eps))

@@ -77,6 +77,14 @@ class AttDecBwdArgs(C.Structure):
     ]
 
 
+class RopeArgs(C.Structure):
+    _fields_ = ([(n, c_f) for n in ("q", "k", "gq", "gk", "wq", "wk", "pos", "q_out", "k_out", "dwq", "dwk", "ws")]
+                + [(n, c_i64) for n in ("q_sb", "q_st", "q_sh", "k_sb", "k_st", "k_sh", "gq_sb", "gq_st", "gq_sh", "gk_sb",
+                                        "gk_st", "gk_sh", "pos_sb")]
+                + [(n, C.c_int) for n in ("B", "T", "H", "Hk", "D", "rot", "dtype")]
+                + [("eps", C.c_float), ("base", C.c_double)])
+
+
 # name -> (restype, argtypes); every symbol include/asr_amd.h declares
 SYMBOLS = {
     "asr_version": (C.c_int, []),
@@ -173,6 +181,10 @@ SYMBOLS = {
     "asr_col2im_3x3s2": (C.c_int, [c_f, c_f, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
     "asr_col2im_dw_blocks": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "asr_col2im_3x3s2_dw": (C.c_int, [c_f, c_f, c_f, C.c_int, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
+    # encoder-layer operators (csrc/rope.hip)
+    "asr_qk_norm_rope_ws_floats": (c_i64, [C.c_int]),
+    "asr_qk_norm_rope_fwd": (C.c_int, [C.POINTER(RopeArgs), c_f]),
+    "asr_qk_norm_rope_bwd": (C.c_int, [C.POINTER(RopeArgs), c_f]),
 }
 
 _lib = None

@@ -585,6 +585,35 @@ int64_t asr_attdec_bwd_err_offset(int B, int T, int E, int Hd, int L);
  * saved dF and alpha.  Same args as the main call; must be ordered after it (same stream, or an event). */
 int asr_attdec_bwd_tail(const asr_attdec_bwd_args *a, void *stream);
 
+/* ------------------------------------------------ encoder-layer operators --
+ * Not in the reference: forms of the same sub-layers that its Conformer encoder (Models/Transformer_encoder.py:55-137,
+ * 191-209) computes with sinusoidal positions and a plain Swish block.  Element types: dtype 0 = float32, 1 = bfloat16,
+ * 2 = float16; products of all three run on the bf16 matrix cores with 3, 1 and 2 bf16 pieces a value, sums, norms and
+ * softmax statistics are float32. */
+
+/* RMS norm of each head of q (B,T,H,D) and k (B,T,Hk,D), times wq / wk (D floats), rotated: pairs (p, p + rot/2) by
+ * position * base^(-2p/rot); elements from rot on are not rotated.  Any strides with contiguous heads (strides in
+ * elements); q_out / k_out contiguous.  pos: int64, row b at b * pos_sb, NULL = 0..T-1.
+ * _bwd: q_out / k_out receive dq / dk, gq / gk are the upstream gradients, dwq / dwk (D floats) are written, ws holds
+ * asr_qk_norm_rope_ws_floats(D) floats.  D even, <= 128.  Deterministic. */
+typedef struct {
+    const void *q, *k;
+    const void *gq, *gk;
+    const float *wq, *wk;
+    const int64_t *pos;
+    void *q_out, *k_out;
+    float *dwq, *dwk, *ws;
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh;
+    int64_t gq_sb, gq_st, gq_sh, gk_sb, gk_st, gk_sh;
+    int64_t pos_sb;
+    int B, T, H, Hk, D, rot, dtype;
+    float eps;
+    double base;
+} asr_rope_args;
+int64_t asr_qk_norm_rope_ws_floats(int D);
+int asr_qk_norm_rope_fwd(const asr_rope_args *a, void *stream);
+int asr_qk_norm_rope_bwd(const asr_rope_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
