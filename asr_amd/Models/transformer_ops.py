@@ -1,6 +1,7 @@
 """Differentiable operators of Transformer-style encoder layers on the HIP kernels.
 
     q, k = qk_norm_rope(q, k, q_weight, k_weight)      # per-head RMS norm and rotary positions
+    y = gated_feed_forward(x, w_gate, w_up, w_down)    # (act(x Wg^T) * (x Wu^T)) Wd^T
 
 Not in the reference, which has sinusoidal relative positions and a plain Swish block in these places
 (Models/Transformer_encoder.py:55-137,191-209); ``ConformerEncoderLayer`` takes them as options.  Tensors are float32,
@@ -138,3 +139,93 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions=None, rot_dim=None, base=10
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
         return _QkNormRope.apply(q, k, q_weight, k_weight, pos, rot, float(base), float(eps))
     return _rope_fwd(q, k, q_weight, k_weight, pos, rot, float(base), float(eps))
+
+
+# ---------------------------------------------------------------------------------------- gated feed-forward --
+ACTIVATIONS = {"swish": 0, "gelu": 1}
+
+
+def _ff_args(x2, wg, wu, wd, act):
+    a = _lib.GatedFFArgs()
+    a.x, a.wg, a.wu, a.wd = x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr()
+    a.M, a.d = x2.shape
+    a.f, a.n, a.dtype, a.act = wg.shape[0], wd.shape[0], _DTYPES[x2.dtype], act
+    return a
+
+
+def _ff_workspace(lib, a, backward, device):
+    n = int(lib.asr_gated_ff_ws_bytes(C.byref(a), int(backward)))
+    if n < 0:
+        check(-1)
+    return torch.empty(n, device=device, dtype=torch.uint8)
+
+
+def _ff_fwd(x2, wg, wu, wd, act):
+    y = torch.empty(x2.shape[0], wd.shape[0], device=x2.device, dtype=x2.dtype)
+    if y.shape[0]:
+        lib = _lib.load()
+        a = _ff_args(x2, wg, wu, wd, act)
+        a.y = y.data_ptr()
+        with _on(x2.device):
+            ws = _ff_workspace(lib, a, False, x2.device)
+            a.ws = ws.data_ptr()
+            check(lib.asr_gated_ff_fwd(C.byref(a), _stream(x2.device)))
+    return y
+
+
+class _GatedFF(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x2, wg, wu, wd, act):
+        ctx.save_for_backward(x2, wg, wu, wd)
+        ctx.act = act
+        return _ff_fwd(x2, wg, wu, wd, act)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x2, wg, wu, wd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if not x2.shape[0]:
+            return torch.zeros_like(x2), torch.zeros_like(wg), torch.zeros_like(wu), torch.zeros_like(wd), None
+        lib = _lib.load()
+        dy = dy.contiguous()
+        a = _ff_args(x2, wg, wu, wd, ctx.act)
+        a.dy = dy.data_ptr()
+        dx = torch.empty_like(x2) if need[0] else None
+        dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need[1] or need[2] else (None, None)
+        dwd = torch.empty_like(wd) if need[3] else None
+        for n, t in (("dx", dx), ("dwg", dwg), ("dwu", dwu), ("dwd", dwd)):
+            if t is not None:
+                setattr(a, n, t.data_ptr())
+        with _on(x2.device):
+            ws = _ff_workspace(lib, a, True, x2.device)
+            a.ws = ws.data_ptr()
+            check(lib.asr_gated_ff_bwd(C.byref(a), _stream(x2.device)))
+        return dx, dwg, dwu, dwd, None
+
+
+def gated_feed_forward(x, w_gate, w_up, w_down, act="swish"):
+    """(act(x w_gate^T) * (x w_up^T)) w_down^T over the last axis of x: w_gate and w_up (f, d), w_down (n, f), no biases; act
+    "swish" or "gelu" (the exact one).  All four of one type.  The hidden values are formed in float32 and rounded once for
+    the second product (to 8 bits for bfloat16, 16 for float16, 24 for float32).  The backward keeps only the inputs and
+    forms the hidden values again.  Up to 64 rows without gradients take a form that reads the weights once."""
+    who = "gated_feed_forward"
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise RuntimeError(f"asr_amd.{who}: x must be a tensor of at least one dimension")
+    _tensor(who, "x", x, x.dim())
+    for n, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
+        _tensor(who, n, w, 2, like=x)
+    if w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[-1] or w_down.shape[1] != w_gate.shape[0]:
+        raise RuntimeError(f"asr_amd.{who}: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} and "
+                           f"w_down {tuple(w_down.shape)} do not match")
+    if 0 in w_gate.shape or 0 in w_down.shape:
+        raise RuntimeError(f"asr_amd.{who}: empty weights")
+    if act not in ACTIVATIONS:
+        raise RuntimeError(f"asr_amd.{who}: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
+    x2 = x.reshape(-1, x.shape[-1]).contiguous()
+    ws = [w.contiguous() for w in (w_gate, w_up, w_down)]
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
+        y = _GatedFF.apply(x2, *ws, ACTIVATIONS[act])
+    else:
+        y = _ff_fwd(x2, *ws, ACTIVATIONS[act])
+    return y.view(*x.shape[:-1], y.shape[-1])

@@ -85,6 +85,11 @@ class RopeArgs(C.Structure):
                 + [("eps", C.c_float), ("base", C.c_double)])
 
 
+class GatedFFArgs(C.Structure):
+    _fields_ = ([(n, c_f) for n in ("x", "wg", "wu", "wd", "dy", "y", "dx", "dwg", "dwu", "dwd", "ws")] + [("M", c_i64)]
+                + [(n, C.c_int) for n in ("d", "f", "n", "dtype", "act")])
+
+
 # name -> (restype, argtypes); every symbol include/asr_amd.h declares
 SYMBOLS = {
     "asr_version": (C.c_int, []),
@@ -181,10 +186,13 @@ SYMBOLS = {
     "asr_col2im_3x3s2": (C.c_int, [c_f, c_f, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
     "asr_col2im_dw_blocks": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "asr_col2im_3x3s2_dw": (C.c_int, [c_f, c_f, c_f, C.c_int, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
-    # encoder-layer operators (csrc/rope.hip)
+    # encoder-layer operators (csrc/rope.hip, gated_ff.hip)
     "asr_qk_norm_rope_ws_floats": (c_i64, [C.c_int]),
     "asr_qk_norm_rope_fwd": (C.c_int, [C.POINTER(RopeArgs), c_f]),
     "asr_qk_norm_rope_bwd": (C.c_int, [C.POINTER(RopeArgs), c_f]),
+    "asr_gated_ff_ws_bytes": (c_i64, [C.POINTER(GatedFFArgs), C.c_int]),
+    "asr_gated_ff_fwd": (C.c_int, [C.POINTER(GatedFFArgs), c_f]),
+    "asr_gated_ff_bwd": (C.c_int, [C.POINTER(GatedFFArgs), c_f]),
 }
 
 _lib = None

@@ -1,0 +1,843 @@
+// asr_gated_ff: y = (act(x Wg^T) * (x Wu^T)) Wd^T and its gradients; x (M,d), Wg / Wu (f,d), Wd (n,f).
+//
+// forward   1  a, b = x Wg^T, x Wu^T of one tile, h = act(a) b in the epilogue                (gff_gate_kernel)
+//           2  y = h Wd^T                                                                      (gff_nt_kernel)
+// backward  1  a, b again and dh = dy Wd of one tile, epilogue: h, da = dh b act'(a), db = dh act(a)
+//           2  dx = [da db] [Wg; Wu]                                                           (gff_nt_kernel)
+//           3  dWg, dWu = [da db]^T x,  dWd = dy^T h                                           (gff_tn_kernel, split over M)
+// Nothing but x is kept for the backward: computing a and b again costs 4 M d f operations of 22 and saves writing and
+// reading two M x f arrays each way; it also keeps act' on unrounded a and b.  h, da and db are rounded once to the
+// pieces of pieces.h (bfloat16: one piece, 2^-8 relative half step, like the stored type itself; the others 2^-16 and
+// 2^-24) because the next product reads them as matrix operands.
+//
+// Bound: the matrix cores.  128 x 128 tiles (gate and up columns interleaved by 32, so that a wave holds a and b of the same
+// elements), 4 waves of 64 x 64 from v_mfma_f32_32x32x16_bf16, operands staged through registers into LDS one k-tile ahead:
+// two LDS images for one piece, one image (two workgroups a compute unit hide each other's barriers) for two and three.
+// Rows and columns beyond the matrix are read from its last row (clamped) and masked in the epilogues; the arrays h, da, db
+// are padded to whole tiles with zeros, which is what the products over them read past the end.
+#include "pieces.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4g __attribute__((ext_vector_type(4)));
+typedef short s16x8g __attribute__((ext_vector_type(8)));
+
+enum { GFF_SWISH = 0, GFF_GELU = 1 };
+
+// ------------------------------------------------------------------------------------------------- operands --
+// A matrix as NP planes of bf16, row-major; rows are clamped to [0, rows)
+struct Planes {
+    const __bf16 *p;
+    int64_t ld, ps;                      // row pitch, distance of the planes (elements)
+    int64_t rows;
+};
+
+// exp(-|x| .. ) with the product x log2(e) carried to twice float32: relative error 1e-7 over the whole range
+__device__ __forceinline__ float exp_acc(float x) {
+    x = fminf(fmaxf(x, -87.f), 88.f);
+    const float hi = x * 1.44269504088896340736f;
+    const float lo = __builtin_fmaf(x, 1.44269504088896340736f, -hi) + x * 1.92596299112661746887e-8f;
+    const float r = __builtin_amdgcn_exp2f(hi);
+    return __builtin_fmaf(r, lo * 0.693147180559945309417f, r);
+}
+__device__ __forceinline__ void act_both(int kind, float a, float &y, float &dy) {
+    if (kind == GFF_SWISH) {
+        const float s = __builtin_amdgcn_rcpf(1.f + exp_acc(-a));
+        y = a * s;
+        dy = s * (1.f + a * (1.f - s));
+    } else {
+        const float cdf = 0.5f * (1.f + erff(a * 0.70710678118654752440f));
+        y = a * cdf;
+        dy = cdf + a * exp_acc(-0.5f * a * a) * 0.39894228040143267794f;
+    }
+}
+__device__ __forceinline__ float act_fwd(int kind, float a) {
+    float y, dy;
+    act_both(kind, a, y, dy);
+    return y;
+}
+
+// -------------------------------------------------------------------------------------------- LDS images --
+template <int NP> struct GemmK { static constexpr int BK = NP == 1 ? 64 : 32; static constexpr int NBUF = NP == 1 ? 2 : 1; };
+#define NT_PITCH(BK) (2 * (BK) + 16)                 // k-contiguous image: 16 B of padding, conflict-free ds_read_b128
+#define TN_PITCH(R) (2 * (R) + 64)                   // row-contiguous image: 64 B mod 256 B, conflict-free transposed reads
+
+// fragment (row r0 + lane&31, k = 16 ks + 8 (lane>>5) ..+7) of a k-contiguous image
+template <int BK>
+__device__ __forceinline__ bf16x8 frag_nt(const unsigned char *img, int r0, int ks, int lane) {
+    const u32x4p v = *reinterpret_cast<const u32x4p *>(img + (r0 + (lane & 31)) * NT_PITCH(BK) + (ks * 2 + (lane >> 5)) * 16);
+    return __builtin_bit_cast(bf16x8, v);
+}
+// the same of a row-contiguous image [k][R]: two transposing reads of 4 k x 16 rows per 16 lanes
+template <int R>
+__device__ __forceinline__ bf16x8 frag_tn(const unsigned char *img, int r0, int ks, int lane) {
+    const int q = (lane & 15) >> 2, p = lane & 3;
+    const unsigned char *a = img + (16 * ks + 8 * (lane >> 5) + q) * TN_PITCH(R) + (r0 + 16 * ((lane >> 4) & 1) + 4 * p) * 2;
+    typedef __attribute__((address_space(3))) s16x4g *lds_p;
+    const s16x4g v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a));
+    const s16x4g v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 4 * TN_PITCH(R)));
+    const s16x8g v = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+    return __builtin_bit_cast(bf16x8, v);
+}
+
+// One operand tile of R rows x BK k: per thread R * BK / 2048 accesses of 16 bytes a piece
+template <int NP, int R>
+struct NtTile {
+    static constexpr int BK = GemmK<NP>::BK, NS = R * BK / 2048, IMG = R * NT_PITCH(BK);
+    const __bf16 *p[NS];
+    int64_t ps;
+    u32x4p v[NP][NS];
+    // PAIR: row groups of 32 alternate between the two matrices (gate, up): group g holds columns n0 + 32 (g / 2) + ...
+    template <bool PAIR>
+    __device__ __forceinline__ void init(const Planes &m0, const Planes &m1, int64_t r0) {
+        ps = m0.ps;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int f = threadIdx.x + 256 * i, row = f / (BK / 8), kc = f % (BK / 8);
+            const bool second = PAIR && ((row >> 5) & 1);
+            int64_t r = r0 + (PAIR ? ((row >> 6) << 5) + (row & 31) : row);
+            r = r < m0.rows ? r : m0.rows - 1;
+            p[i] = (second ? m1.p : m0.p) + r * m0.ld + kc * 8;
+        }
+    }
+    __device__ __forceinline__ void load(int k0) {
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int i = 0; i < NS; ++i) v[q][i] = *reinterpret_cast<const u32x4p *>(p[i] + q * ps + k0);
+    }
+    __device__ __forceinline__ void store(unsigned char *img) const {
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int f = threadIdx.x + 256 * i;
+                *reinterpret_cast<u32x4p *>(img + q * IMG + (f / (BK / 8)) * NT_PITCH(BK) + (f % (BK / 8)) * 16) = v[q][i];
+            }
+    }
+};
+// BK rows of the matrix (the product's k) x R columns; columns past ld read column 0, rows past the matrix its last row
+template <int NP, int R>
+struct TnTile {
+    static constexpr int BK = GemmK<NP>::BK, NS = R * BK / 2048, IMG = BK * TN_PITCH(R);
+    const __bf16 *p;
+    int64_t ld, ps, rows;
+    int col[NS];
+    u32x4p v[NP][NS];
+    __device__ __forceinline__ void init(const Planes &m, int64_t c0) {
+        p = m.p;
+        ld = m.ld;
+        ps = m.ps;
+        rows = m.rows;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int64_t c = c0 + ((threadIdx.x + 256 * i) % (R / 8)) * 8;
+            col[i] = c < ld ? (int)c : 0;
+        }
+    }
+    __device__ __forceinline__ void load(int64_t k0) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            int64_t r = k0 + (threadIdx.x + 256 * i) / (R / 8);
+            r = r < rows ? r : rows - 1;
+            const __bf16 *a = p + r * ld + col[i];
+#pragma unroll
+            for (int q = 0; q < NP; ++q) v[q][i] = *reinterpret_cast<const u32x4p *>(a + q * ps);
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char *img) const {
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int f = threadIdx.x + 256 * i;
+                *reinterpret_cast<u32x4p *>(img + q * IMG + (f / (R / 8)) * TN_PITCH(R) + (f % (R / 8)) * 16) = v[q][i];
+            }
+    }
+};
+
+// acc += A B over one k-tile; FRAG(operand, piece, tile, ks) delivers fragments.  Smallest pieces first.
+template <int NP, int TM, int TN, typename FA, typename FB>
+__device__ __forceinline__ void mma_tile(f32x16 (&acc)[TM][TN], FA fa, FB fb) {
+    constexpr int KS = GemmK<NP>::BK / 16;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        bf16x8 a[NP][TM], b[NP][TN];
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) a[q][i] = fa(q, i, ks);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) b[q][j] = fb(q, j, ks);
+        }
+#pragma unroll
+        for (int s = NP - 1; s >= 0; --s)
+#pragma unroll
+            for (int q = s; q >= 0; --q)
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[q][i], b[s - q][j], acc[i][j], 0, 0, 0);
+    }
+}
+
+// The main loop: k-tiles [kt0, kt1) of A (TA rows) times B (TB rows); leaves the LDS free to use (ends with a barrier).
+template <int NP, int TM, int TN, typename TA, typename TB, typename FA, typename FB>
+__device__ __forceinline__ void main_loop(f32x16 (&acc)[TM][TN], TA &ta, TB &tb, unsigned char *lds, int64_t kt0, int64_t kt1,
+                                          FA frag_a, FB frag_b) {
+    constexpr int BK = GemmK<NP>::BK, NBUF = GemmK<NP>::NBUF, IA = NP * TA::IMG, IB = NP * TB::IMG;
+    if (kt0 >= kt1) return;
+    ta.load(kt0 * BK);
+    tb.load(kt0 * BK);
+    ta.store(lds);
+    tb.store(lds + IA);
+    __syncthreads();
+    int buf = 0;
+    for (int64_t kt = kt0; kt < kt1; ++kt) {
+        const bool more = kt + 1 < kt1;
+        if (more) {
+            ta.load((kt + 1) * BK);
+            tb.load((kt + 1) * BK);
+        }
+        unsigned char *img = lds + (NBUF == 2 ? buf * (IA + IB) : 0);
+        mma_tile<NP, TM, TN>(acc, [&](int q, int i, int ks) { return frag_a(img + q * TA::IMG, i, ks); },
+                             [&](int q, int j, int ks) { return frag_b(img + IA + q * TB::IMG, j, ks); });
+        if (NBUF == 1) __syncthreads();
+        if (more) {
+            buf ^= 1;
+            unsigned char *nxt = lds + (NBUF == 2 ? buf * (IA + IB) : 0);
+            ta.store(nxt);
+            tb.store(nxt + IA);
+        }
+        __syncthreads();
+    }
+}
+
+template <int TM, int TN>
+__device__ __forceinline__ void zero_acc(f32x16 (&acc)[TM][TN]) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+}
+
+// A 32 x 32 accumulator tile (lane = column, registers = rows) turned through a wave's 4 KB of LDS: put(row, col, v) gets four
+// consecutive columns of a row at a time, eight rows of 128 B per step.
+template <typename F>
+__device__ __forceinline__ void turn_tile(const f32x16 &t, float *S, F put) {
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) S[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * 32 + (lane & 31)] = t[r];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int p = 0; p < 4; ++p) put(p * 8 + (lane >> 3), (lane & 7) * 4, *reinterpret_cast<const float4 *>(&S[(p * 8 + (lane >> 3)) * 32 + (lane & 7) * 4]));
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+}
+
+template <int NP>
+__device__ __forceinline__ void put_pieces(__bf16 *dst, int64_t ps, float4 v) {
+    unsigned lo[NP], hi[NP];
+    split_pair<NP>(v.x, v.y, lo);
+    split_pair<NP>(v.z, v.w, hi);
+#pragma unroll
+    for (int q = 0; q < NP; ++q) *reinterpret_cast<u32x2p *>(dst + q * ps) = u32x2p{lo[q], hi[q]};
+}
+template <typename E>
+__device__ __forceinline__ void put_row4(E *row, int64_t col, int64_t n, bool vec, float4 v) {
+    const float t[4] = {v.x, v.y, v.z, v.w};
+    if (vec && col + 3 < n) {
+        store_vec<E, 4>(row + col, t);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < n) row[col + e] = (E)t[e];
+    }
+}
+
+// Workgroups go to the 8 XCDs round-robin by linear id: XCD x works through one contiguous run of the tiles, column
+// tiles fastest, so that the tiles that share an operand's rows share an L2.
+__device__ __forceinline__ void tile_of(int id, int ntiles, int ncol, int &row, int &col) {
+    const int q = ntiles >> 3, r = ntiles & 7, x = id & 7, loc = id >> 3;
+    const int t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + loc;
+    row = t / ncol;
+    col = t - row * ncol;
+}
+
+// ------------------------------------------------------------------- a, b (and dh) of one tile, elementwise part --
+struct GateParams {
+    Planes x, wg, wu;                    // x (M, dp), weights (f, dp)
+    Planes dy, wdt;                      // backward: dy (M, np), Wd^T (f, np)
+    __bf16 *h, *dab;                     // (Mp, fp) and (Mp, 2 fp) in pieces
+    int64_t h_ps, dab_ps;
+    int64_t M, fp;
+    int f, ktx, kty, ncol, ntiles, act;
+};
+
+template <int NP, bool BWD>
+__global__ __launch_bounds__(256, 2) void gff_gate_kernel(GateParams p) {
+    constexpr int BM = 128, BN = 64;
+    typedef NtTile<NP, BM> TA;
+    typedef NtTile<NP, 128> TB;
+    typedef NtTile<NP, BN> TD;
+    constexpr int POOL = GemmK<NP>::NBUF * NP * (TA::IMG + TB::IMG);
+    __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > 16384 ? POOL : 16384];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+    int tm, tn;
+    tile_of(blockIdx.x, p.ntiles, p.ncol, tm, tn);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    f32x16 ab[2][2];
+    zero_acc(ab);
+    {
+        TA ta;
+        TB tb;
+        ta.template init<false>(p.x, p.x, m0);
+        tb.template init<true>(p.wg, p.wu, n0);
+        main_loop<NP>(ab, ta, tb, pool, 0, p.ktx,
+                      [&](const unsigned char *img, int i, int ks) { return frag_nt<TA::BK>(img, wm * 64 + i * 32, ks, lane); },
+                      [&](const unsigned char *img, int j, int ks) { return frag_nt<TA::BK>(img, wn * 64 + j * 32, ks, lane); });
+    }
+    f32x16 dh[2][1];
+    if (BWD) {
+        zero_acc(dh);
+        TA ta;
+        TD tb;
+        ta.template init<false>(p.dy, p.dy, m0);
+        tb.template init<false>(p.wdt, p.wdt, n0);
+        main_loop<NP>(dh, ta, tb, pool, 0, p.kty,
+                      [&](const unsigned char *img, int i, int ks) { return frag_nt<TA::BK>(img, wm * 64 + i * 32, ks, lane); },
+                      [&](const unsigned char *img, int j, int ks) { return frag_nt<TA::BK>(img, wn * 32 + j * 32, ks, lane); });
+    }
+    float *S = reinterpret_cast<float *>(pool) + wave * 1024;
+    const int64_t cb = n0 + wn * 32;
+    const bool col_ok = cb + (lane & 31) < p.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int64_t rb = m0 + wm * 64 + i * 32;
+        f32x16 hh, da, db;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const bool ok = col_ok && rb + ((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) < p.M;
+            const float a = ab[i][0][r], b = ab[i][1][r];
+            float y, dy;
+            act_both(p.act, a, y, dy);
+            hh[r] = ok ? y * b : 0.f;
+            if (BWD) {
+                da[r] = ok ? dh[i][0][r] * b * dy : 0.f;
+                db[r] = ok ? dh[i][0][r] * y : 0.f;
+            }
+        }
+        turn_tile(hh, S, [&](int r, int c, float4 v) { put_pieces<NP>(p.h + (rb + r) * p.fp + cb + c, p.h_ps, v); });
+        if (BWD) {
+            turn_tile(da, S, [&](int r, int c, float4 v) { put_pieces<NP>(p.dab + (rb + r) * 2 * p.fp + cb + c, p.dab_ps, v); });
+            turn_tile(db, S, [&](int r, int c, float4 v) { put_pieces<NP>(p.dab + (rb + r) * 2 * p.fp + p.fp + cb + c, p.dab_ps, v); });
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------ C = A B^T, one output --
+struct NtParams {
+    Planes a, b;
+    void *c;
+    int64_t ldc, M, N;
+    int kt, ncol, ntiles, vec;
+};
+template <int DT, int BM, int BN>
+__global__ __launch_bounds__(256, 2) void gff_nt_kernel(NtParams p) {
+    constexpr int NP = ElemOf<DT>::NP, TM = BM / 64, TN = BN / 64;
+    typedef typename ElemOf<DT>::type E;
+    typedef NtTile<NP, BM> TA;
+    typedef NtTile<NP, BN> TB;
+    constexpr int POOL = GemmK<NP>::NBUF * NP * (TA::IMG + TB::IMG);
+    __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > 16384 ? POOL : 16384];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+    int tm, tn;
+    tile_of(blockIdx.x, p.ntiles, p.ncol, tm, tn);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    f32x16 acc[TM][TN];
+    zero_acc(acc);
+    TA ta;
+    TB tb;
+    ta.template init<false>(p.a, p.a, m0);
+    tb.template init<false>(p.b, p.b, n0);
+    main_loop<NP>(acc, ta, tb, pool, 0, p.kt,
+                  [&](const unsigned char *img, int i, int ks) { return frag_nt<TA::BK>(img, wm * (BM / 2) + i * 32, ks, lane); },
+                  [&](const unsigned char *img, int j, int ks) { return frag_nt<TA::BK>(img, wn * (BN / 2) + j * 32, ks, lane); });
+    float *S = reinterpret_cast<float *>(pool) + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int64_t rb = m0 + wm * (BM / 2) + i * 32, cb = n0 + wn * (BN / 2) + j * 32;
+            turn_tile(acc[i][j], S, [&](int r, int c, float4 v) {
+                if (rb + r < p.M) put_row4<E>((E *)p.c + (rb + r) * p.ldc, cb + c, p.N, p.vec, v);
+            });
+        }
+}
+
+// ------------------------------------------------------------- C = A^T B over the rows, split over workgroups --
+// Output row r < half goes to c0, r >= half to c1 (the gate's and the up projection's gradients lie half apart in [da db]);
+// rows from `valid` on of either are padding.  With splits > 1 every split writes float32 partials, gff_sum_kernel adds them in
+// order.
+struct TnParams {
+    Planes a, b;
+    void *c0, *c1;
+    float *part;
+    int64_t half, valid, N, part_sz;
+    int64_t kt, kt_split;
+    int ncol, ntiles, vec;
+};
+template <int DT>
+__global__ __launch_bounds__(256, 2) void gff_tn_kernel(TnParams p) {
+    constexpr int NP = ElemOf<DT>::NP, BM = 128, BN = 128;
+    typedef typename ElemOf<DT>::type E;
+    typedef TnTile<NP, BM> TA;
+    typedef TnTile<NP, BN> TB;
+    constexpr int POOL = GemmK<NP>::NBUF * NP * (TA::IMG + TB::IMG);
+    __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > 16384 ? POOL : 16384];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+    int tm, tn;
+    tile_of(blockIdx.x, p.ntiles, p.ncol, tm, tn);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    f32x16 acc[2][2];
+    zero_acc(acc);
+    TA ta;
+    TB tb;
+    ta.init(p.a, m0);
+    tb.init(p.b, n0);
+    const int64_t k0 = blockIdx.y * p.kt_split;
+    main_loop<NP>(acc, ta, tb, pool, k0, min(p.kt, k0 + p.kt_split),
+                  [&](const unsigned char *img, int i, int ks) { return frag_tn<BM>(img, wm * 64 + i * 32, ks, lane); },
+                  [&](const unsigned char *img, int j, int ks) { return frag_tn<BN>(img, wn * 64 + j * 32, ks, lane); });
+    float *S = reinterpret_cast<float *>(pool) + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int64_t rb = m0 + wm * 64 + i * 32, cb = n0 + wn * 64 + j * 32;
+            turn_tile(acc[i][j], S, [&](int r, int c, float4 v) {
+                int64_t row = rb + r;
+                const bool second = row >= p.half;
+                row -= second ? p.half : 0;
+                if (row >= p.valid || (second && p.c1 == nullptr)) return;
+                if (p.part) {
+                    float *dst = p.part + blockIdx.y * p.part_sz + ((second ? p.valid : 0) + row) * p.N;
+                    put_row4<float>(dst, cb + c, p.N, p.vec, v);
+                } else {
+                    put_row4<E>((E *)(second ? p.c1 : p.c0) + row * p.N, cb + c, p.N, p.vec, v);
+                }
+            });
+        }
+}
+template <int DT, int V>
+__global__ __launch_bounds__(256) void gff_sum_kernel(const float *__restrict__ part, int64_t sz, int splits, int64_t n0, void *c0, void *c1) {
+    typedef typename ElemOf<DT>::type E;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < sz; i += (int64_t)gridDim.x * 256 * V) {
+        float v[V], t[V];
+        load_vec<float, V>(part + i, v);
+        for (int s = 1; s < splits; ++s) {
+            load_vec<float, V>(part + s * sz + i, t);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += t[e];
+        }
+        store_vec<E, V>(i < n0 ? (E *)c0 + i : (E *)c1 + (i - n0), v);
+    }
+}
+
+// ---------------------------------------------------------------------------------------- packing into planes --
+// Up to 8 matrices in one launch: src (R, C) row-major with pitch lds -> pieces, straight (R, >= C, pitch ldd) or transposed
+// (C, >= R); columns of the result from the matrix' end to `wide` are zeros.
+struct PackJob {
+    const void *src;
+    __bf16 *dst;
+    int64_t lds, ldd, ps, R, C, wide;
+    int trans;
+    int64_t blk0;                        // first workgroup of the job
+    int64_t nx;                          // workgroups along the source's columns
+};
+struct PackJobs { PackJob j[8]; int n; };
+
+template <int DT>
+__global__ __launch_bounds__(256) void gff_pack_kernel(PackJobs jobs) {
+    typedef typename ElemOf<DT>::type E;
+    constexpr int NP = ElemOf<DT>::NP;
+    __shared__ float tile[64][65];
+    int k = 0;
+    while (k + 1 < jobs.n && (int64_t)blockIdx.x >= jobs.j[k + 1].blk0) ++k;
+    const PackJob &J = jobs.j[k];
+    const int64_t b = blockIdx.x - J.blk0, by = b / J.nx, bx = b - by * J.nx;
+    const E *src = (const E *)J.src;
+    // a 64 x 64 block; source columns (or, transposed, rows) past the end read as zero
+    const int64_t r0 = by * 64, c0 = bx * 64;
+    const int tc = (threadIdx.x & 15) * 4, tr = threadIdx.x >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + tr + 16 * i;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (r < J.R) {
+            const E *q = src + r * J.lds + c0 + tc;
+            if (c0 + tc + 3 < J.C && (uintptr_t)q % (4 * sizeof(E)) == 0) {
+                load_vec<E, 4>(q, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c0 + tc + e < J.C) v[e] = (float)q[e];
+            }
+        }
+        if (!J.trans) {
+            if (r < J.R && c0 + tc < J.wide) put_pieces<NP>(J.dst + r * J.ldd + c0 + tc, J.ps, make_float4(v[0], v[1], v[2], v[3]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tile[tr + 16 * i][tc + e] = v[e];
+        }
+    }
+    if (J.trans) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t c = c0 + tr + 16 * i;                      // a row of the result
+            if (c < J.C && r0 + tc < J.wide)
+                put_pieces<NP>(J.dst + c * J.ldd + r0 + tc, J.ps,
+                               make_float4(tile[tc][tr + 16 * i], tile[tc + 1][tr + 16 * i], tile[tc + 2][tr + 16 * i], tile[tc + 3][tr + 16 * i]));
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------- a few rows: tokens --
+// M <= 64 rows, forward only: the weights are read once from memory, which bounds it.  16 weight rows a workgroup, its waves
+// split k, products exact in v_mfma_f32_16x16x4_f32 (weights widened in registers: at 16 rows the matrix time is half of the
+// weights' memory time), rows of x in groups of 16.  GATE: two weight matrices and h = act(a) b to float32 h; else y.
+template <int DT, int NM, bool GATE>
+__device__ __forceinline__ void few_rows_body(const typename ElemOf<DT>::type *wa, const typename ElemOf<DT>::type *wb,
+                                              const void *xin, bool x_is_float, bool vec, int64_t K, int M, int64_t N, int act,
+                                              float *h, typename ElemOf<DT>::type *y, int nw, float *red) {
+    typedef typename ElemOf<DT>::type E;
+    constexpr int V = 8;                                             // k per lane and step: 32 k of a row over its four lanes
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int64_t n = (int64_t)blockIdx.x * 16 + c, row = n < N ? n : N - 1;
+    f32x4 acc[GATE ? 2 : 1][NM];
+#pragma unroll
+    for (int s = 0; s < (GATE ? 2 : 1); ++s)
+#pragma unroll
+        for (int m = 0; m < NM; ++m) acc[s][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const E *ra = wa + row * K, *rb = GATE ? wb + row * K : wa;
+    const int64_t ldx = K;
+#pragma unroll 2
+    for (int64_t k0 = (int64_t)wave * 32; k0 < K; k0 += (int64_t)nw * 32) {
+        const int64_t k = k0 + g * V;
+        float va[V], vb[V], vx[NM][V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) va[e] = vb[e] = 0.f;
+        if (vec) {                                                   // K % 8 == 0: a lane's eight are all there or none is
+            if (k < K) {
+                load_vec<E, V>(ra + k, va);
+                if (GATE) load_vec<E, V>(rb + k, vb);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (k + e < K) {
+                    va[e] = (float)ra[k + e];
+                    if (GATE) vb[e] = (float)rb[k + e];
+                }
+        }
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            const int r = min(m * 16 + c, M - 1);
+#pragma unroll
+            for (int e = 0; e < V; ++e) vx[m][e] = 0.f;
+            if (vec) {
+                if (k < K) {
+                    if (x_is_float) load_vec<float, V>((const float *)xin + r * ldx + k, vx[m]);
+                    else load_vec<E, V>((const E *)xin + r * ldx + k, vx[m]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (k + e < K) vx[m][e] = x_is_float ? ((const float *)xin)[r * ldx + k + e] : (float)((const E *)xin)[r * ldx + k + e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+                acc[0][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(va[e], vx[m][e], acc[0][m], 0, 0, 0);
+                if constexpr (GATE) acc[1][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(vb[e], vx[m][e], acc[1][m], 0, 0, 0);
+            }
+    }
+    // D: column = x row (lane & 15), rows 4 g + r = weight rows; partials of the waves through LDS
+    constexpr int NA = (GATE ? 2 : 1) * NM;
+#pragma unroll
+    for (int s = 0; s < (GATE ? 2 : 1); ++s)
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+            *reinterpret_cast<f32x4 *>(red + ((wave * NA + s * NM + m) * 64 + lane) * 4) = acc[s][m];
+    __syncthreads();
+    for (int t = threadIdx.x; t < NM * 64; t += blockDim.x) {
+        const int m = t >> 6, l = t & 63;
+        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+        for (int w = 0; w < nw; ++w) {
+            a += *reinterpret_cast<const f32x4 *>(red + ((w * NA + m) * 64 + l) * 4);
+            if (GATE) b += *reinterpret_cast<const f32x4 *>(red + ((w * NA + NM + m) * 64 + l) * 4);
+        }
+        const int r = m * 16 + (l & 15);
+        if (r >= M) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t o = (int64_t)blockIdx.x * 16 + (l >> 4) * 4 + e;
+            if (o >= N) continue;
+            if (GATE) h[r * N + o] = act_fwd(act, a[e]) * b[e];
+            else y[r * N + o] = (E)a[e];
+        }
+    }
+}
+template <int DT, int NM>
+__global__ __launch_bounds__(256) void gff_few_gate_kernel(const void *x, const void *wg, const void *wu, float *h, int64_t d,
+                                                           int64_t f, int M, int act, int vec) {
+    __shared__ __attribute__((aligned(16))) float red[4 * 2 * NM * 256];
+    typedef typename ElemOf<DT>::type E;
+    few_rows_body<DT, NM, true>((const E *)wg, (const E *)wu, x, false, vec, d, M, f, act, h, nullptr, 4, red);
+}
+template <int DT, int NM>
+__global__ __launch_bounds__(512) void gff_few_down_kernel(const float *h, const void *wd, void *y, int64_t f, int64_t n, int M, int vec) {
+    __shared__ __attribute__((aligned(16))) float red[8 * NM * 256];
+    typedef typename ElemOf<DT>::type E;
+    few_rows_body<DT, NM, false>((const E *)wd, nullptr, h, true, vec, f, M, n, 0, nullptr, (E *)y, 8, red);
+}
+
+// ------------------------------------------------------------------------------------------------------- host --
+static int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+struct GffPlan {
+    int NP;
+    int64_t dp, np, fp, Mp;              // padded widths of x / dy / h and rows of h, [da db]
+    bool direct_x, direct_wgu, direct_wd, direct_dy;
+    int splits_gu, splits_d;
+    int64_t off[16], bytes;              // workspace: byte offsets
+};
+enum { O_X, O_WG, O_WU, O_WD, O_H, O_DY, O_WDT, O_WGUT, O_DAB, O_PART };
+
+static bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
+
+// Splits of the weight gradients' sum over M: enough workgroups for two a compute unit, each with at least 8 k-tiles
+static int gff_splits(int64_t tiles, int64_t kt) {
+    int64_t s = 512 / (tiles > 0 ? tiles : 1);
+    if (s > kt / 8) s = kt / 8;
+    if (s > 32) s = 32;
+    return s < 1 ? 1 : (int)s;
+}
+
+// A bfloat16 matrix whose k is whole k-tiles is an operand as it lies; every other one is packed into the workspace.
+static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
+    p.NP = a->dtype == ASR_T_F32 ? 3 : a->dtype == ASR_T_F16 ? 2 : 1;
+    p.dp = up_to(a->d, 64);
+    p.np = up_to(a->n, 64);
+    p.fp = up_to(a->f, 64);
+    p.Mp = up_to(a->M, 128);
+    const bool one = p.NP == 1;
+    p.direct_x = one && p.dp == a->d && aligned16(a->x);
+    p.direct_wgu = one && p.dp == a->d && aligned16(a->wg) && aligned16(a->wu);
+    p.direct_wd = one && p.fp == a->f && aligned16(a->wd);
+    p.direct_dy = one && p.np == a->n && aligned16(a->dy);
+    int64_t o = 0;
+    auto take = [&](int k, int64_t bytes) {
+        p.off[k] = o;
+        o += up_to(bytes, 256);
+    };
+    const int64_t e = 2 * p.NP;
+    take(O_X, p.direct_x ? 0 : a->M * p.dp * e);
+    take(O_WG, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * e);
+    take(O_WU, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * e);
+    take(O_H, p.Mp * p.fp * e);
+    take(O_WD, p.direct_wd || bwd ? 0 : (int64_t)a->n * p.fp * e);
+    if (bwd) {
+        take(O_DY, p.direct_dy ? 0 : a->M * p.np * e);
+        take(O_WDT, (int64_t)a->f * p.np * e);
+        take(O_WGUT, (int64_t)a->d * 2 * p.fp * e);
+        take(O_DAB, p.Mp * 2 * p.fp * e);
+        const int64_t bk = one ? 64 : 32, kt = (a->M + bk - 1) / bk;
+        p.splits_gu = gff_splits((int64_t)cdiv(2 * p.fp, 128) * cdiv(a->d, 128), kt);
+        p.splits_d = gff_splits((int64_t)cdiv(a->n, 128) * cdiv(a->f, 128), kt);
+        int64_t part = 0;
+        if (p.splits_gu > 1) part = (int64_t)p.splits_gu * 2 * a->f * a->d;
+        if (p.splits_d > 1 && (int64_t)p.splits_d * a->n * a->f > part) part = (int64_t)p.splits_d * a->n * a->f;
+        take(O_PART, part * 4);
+    }
+    p.bytes = o;
+}
+
+#define GFF_FEW_ROWS 64
+static bool gff_few(const asr_gated_ff_args *a) { return a->M <= GFF_FEW_ROWS; }
+
+static int gff_check(const asr_gated_ff_args *a, const char *who, bool ptrs) {
+    ASR_CHECK_ARG(a, "%s: null pointer", who);
+    ASR_CHECK_ARG(a->dtype >= 0 && a->dtype <= 2, "%s: unknown element type", who);
+    ASR_CHECK_ARG(a->act == GFF_SWISH || a->act == GFF_GELU, "%s: unknown activation", who);
+    ASR_CHECK_ARG(a->M > 0 && a->d > 0 && a->f > 0 && a->n > 0, "%s: empty shape", who);
+    ASR_CHECK_ARG(a->d <= (1 << 20) && a->f <= (1 << 20) && a->n <= (1 << 20), "%s: widths are at most 2^20", who);
+    ASR_CHECK_ARG((int64_t)cdiv(a->M, 128) * cdiv(a->f > a->d ? (a->f > a->n ? a->f : a->n) : (a->d > a->n ? a->d : a->n), 64) < (1ll << 30),
+                  "%s: too many rows", who);
+    if (ptrs) ASR_CHECK_ARG(a->x && a->wg && a->wu && a->wd && a->ws, "%s: null pointer", who);
+    return ASR_OK;
+}
+
+extern "C" int64_t asr_gated_ff_ws_bytes(const asr_gated_ff_args *a, int backward) {
+    if (gff_check(a, "gated_ff_ws_bytes", false) != ASR_OK) return -1;
+    if (!backward && gff_few(a)) return up_to((int64_t)a->M * a->f * 4, 256);
+    GffPlan p;
+    gff_plan(a, backward != 0, p);
+    return p.bytes;
+}
+
+static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, int64_t R, int64_t C, int64_t ldd, int64_t ps, int64_t wide, int trans) {
+    PackJob &k = j.j[j.n++];
+    k.src = src;
+    k.dst = (__bf16 *)dst;
+    k.lds = C;
+    k.ldd = ldd;
+    k.ps = ps;
+    k.R = R;
+    k.C = C;
+    k.wide = wide;
+    k.trans = trans;
+    k.blk0 = blocks;
+    // straight: the padding columns belong to the last blocks of a row; transposed: to the last blocks of a column
+    k.nx = cdiv(trans ? C : wide, 64);
+    blocks += k.nx * cdiv(trans ? wide : R, 64);
+}
+
+template <int DT>
+static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t N, int64_t K, hipStream_t st) {
+    constexpr int NP = ElemOf<DT>::NP;
+    NtParams p{a, b, c, N, M, N, (int)(K / GemmK<NP>::BK), 0, 0, (int)(N % 4 == 0 && aligned16(c))};
+    // narrower tiles where 128 x 128 would leave compute units without one
+    if ((int64_t)cdiv(M, 128) * cdiv(N, 128) >= 256) {
+        p.ncol = cdiv(N, 128);
+        p.ntiles = cdiv(M, 128) * p.ncol;
+        hipLaunchKernelGGL((gff_nt_kernel<DT, 128, 128>), dim3(p.ntiles), dim3(256), 0, st, p);
+    } else {
+        p.ncol = cdiv(N, 64);
+        p.ntiles = cdiv(M, 64) * p.ncol;
+        hipLaunchKernelGGL((gff_nt_kernel<DT, 64, 64>), dim3(p.ntiles), dim3(256), 0, st, p);
+    }
+    ASR_CHECK_LAUNCH("gff_nt_kernel");
+    return ASR_OK;
+}
+
+template <int DT>
+static int gff_tn(const Planes &a, const Planes &b, void *c0, void *c1, int64_t rows, int64_t half, int64_t valid, int64_t N, int64_t M,
+                  int splits, float *part, hipStream_t st) {
+    constexpr int NP = ElemOf<DT>::NP;
+    TnParams p{a, b, c0, c1, splits > 1 ? part : nullptr, half, valid, N, (c1 ? 2 : 1) * valid * N, cdiv(M, GemmK<NP>::BK), 0, cdiv(N, 128), 0,
+               (int)(N % 4 == 0 && aligned16(c0) && aligned16(c1))};
+    p.ntiles = cdiv(rows, 128) * p.ncol;
+    p.kt_split = (p.kt + splits - 1) / splits;
+    hipLaunchKernelGGL((gff_tn_kernel<DT>), dim3(p.ntiles, splits), dim3(256), 0, st, p);
+    ASR_CHECK_LAUNCH("gff_tn_kernel");
+    if (splits > 1) {
+        const int64_t n0 = valid * N;
+        if (n0 % 4 == 0 && aligned16(c0) && aligned16(c1))
+            hipLaunchKernelGGL((gff_sum_kernel<DT, 4>), dim3((unsigned)(cdiv(p.part_sz, 1024) < 4096 ? cdiv(p.part_sz, 1024) : 4096)), dim3(256), 0, st, part,
+                               p.part_sz, splits, n0, c0, c1);
+        else
+            hipLaunchKernelGGL((gff_sum_kernel<DT, 1>), dim3((unsigned)(cdiv(p.part_sz, 256) < 4096 ? cdiv(p.part_sz, 256) : 4096)), dim3(256), 0, st, part,
+                               p.part_sz, splits, n0, c0, c1);
+        ASR_CHECK_LAUNCH("gff_sum_kernel");
+    }
+    return ASR_OK;
+}
+
+template <int DT>
+static int gff_run(const asr_gated_ff_args *a, bool bwd, hipStream_t st) {
+    constexpr int NP = ElemOf<DT>::NP, BK = GemmK<NP>::BK;
+    GffPlan p;
+    gff_plan(a, bwd, p);
+    char *ws = (char *)a->ws;
+    auto at = [&](int k) { return (__bf16 *)(ws + p.off[k]); };
+    Planes x{p.direct_x ? (const __bf16 *)a->x : at(O_X), p.dp, a->M * p.dp, a->M};
+    Planes wg{p.direct_wgu ? (const __bf16 *)a->wg : at(O_WG), p.dp, (int64_t)a->f * p.dp, a->f};
+    Planes wu{p.direct_wgu ? (const __bf16 *)a->wu : at(O_WU), p.dp, (int64_t)a->f * p.dp, a->f};
+    Planes wd{p.direct_wd ? (const __bf16 *)a->wd : at(O_WD), p.fp, (int64_t)a->n * p.fp, a->n};
+    Planes h{at(O_H), p.fp, p.Mp * p.fp, p.Mp};
+    Planes dy{}, wdt{}, wgut{}, dab{};
+    PackJobs jobs;
+    jobs.n = 0;
+    int64_t blocks = 0;
+    if (!p.direct_x) pack_add(jobs, blocks, a->x, at(O_X), a->M, a->d, p.dp, x.ps, p.dp, 0);
+    if (!p.direct_wgu) {
+        pack_add(jobs, blocks, a->wg, at(O_WG), a->f, a->d, p.dp, wg.ps, p.dp, 0);
+        pack_add(jobs, blocks, a->wu, at(O_WU), a->f, a->d, p.dp, wu.ps, p.dp, 0);
+    }
+    if (!bwd && !p.direct_wd) pack_add(jobs, blocks, a->wd, at(O_WD), a->n, a->f, p.fp, wd.ps, p.fp, 0);
+    if (bwd) {
+        dy = Planes{p.direct_dy ? (const __bf16 *)a->dy : at(O_DY), p.np, a->M * p.np, a->M};
+        wdt = Planes{at(O_WDT), p.np, (int64_t)a->f * p.np, a->f};
+        wgut = Planes{at(O_WGUT), 2 * p.fp, (int64_t)a->d * 2 * p.fp, a->d};
+        dab = Planes{at(O_DAB), 2 * p.fp, p.Mp * 2 * p.fp, p.Mp};
+        if (!p.direct_dy) pack_add(jobs, blocks, a->dy, at(O_DY), a->M, a->n, p.np, dy.ps, p.np, 0);
+        pack_add(jobs, blocks, a->wd, at(O_WDT), a->n, a->f, p.np, wdt.ps, p.np, 1);
+        pack_add(jobs, blocks, a->wg, at(O_WGUT), a->f, a->d, 2 * p.fp, wgut.ps, p.fp, 1);
+        pack_add(jobs, blocks, a->wu, at(O_WGUT) + p.fp, a->f, a->d, 2 * p.fp, wgut.ps, p.fp, 1);
+    }
+    if (jobs.n) {
+        ASR_CHECK_ARG(blocks < (1ll << 31), "gated_ff: too many rows");
+        hipLaunchKernelGGL((gff_pack_kernel<DT>), dim3((unsigned)blocks), dim3(256), 0, st, jobs);
+        ASR_CHECK_LAUNCH("gff_pack_kernel");
+    }
+    GateParams g{x, wg, wu, dy, wdt, (__bf16 *)h.p, (__bf16 *)dab.p, h.ps, dab.ps, a->M, p.fp, a->f, (int)(p.dp / BK), (int)(p.np / BK),
+                 (int)(p.fp / 64), 0, a->act};
+    g.ntiles = (int)(p.Mp / 128) * g.ncol;
+    if (!bwd) {
+        hipLaunchKernelGGL((gff_gate_kernel<NP, false>), dim3(g.ntiles), dim3(256), 0, st, g);
+        ASR_CHECK_LAUNCH("gff_gate_kernel");
+        return gff_nt<DT>(h, wd, a->y, a->M, a->n, p.fp, st);
+    }
+    hipLaunchKernelGGL((gff_gate_kernel<NP, true>), dim3(g.ntiles), dim3(256), 0, st, g);
+    ASR_CHECK_LAUNCH("gff_gate_kernel");
+    if (a->dx) ASR_CHECK(gff_nt<DT>(dab, wgut, a->dx, a->M, a->d, 2 * p.fp, st));
+    float *part = (float *)at(O_PART);
+    if (a->dwg) ASR_CHECK(gff_tn<DT>(dab, x, a->dwg, a->dwu, 2 * p.fp, p.fp, a->f, a->d, a->M, p.splits_gu, part, st));
+    if (a->dwd) ASR_CHECK(gff_tn<DT>(dy, h, a->dwd, nullptr, a->n, up_to(a->n, 128), a->n, a->f, a->M, p.splits_d, part, st));
+    return ASR_OK;
+}
+
+template <int DT, int NM>
+static int gff_few_run(const asr_gated_ff_args *a, hipStream_t st) {
+    hipLaunchKernelGGL((gff_few_gate_kernel<DT, NM>), dim3(cdiv(a->f, 16)), dim3(256), 0, st, a->x, a->wg, a->wu, (float *)a->ws,
+                       (int64_t)a->d, (int64_t)a->f, (int)a->M, a->act, (int)(a->d % 8 == 0 && aligned16(a->x) && aligned16(a->wg) && aligned16(a->wu)));
+    hipLaunchKernelGGL((gff_few_down_kernel<DT, NM>), dim3(cdiv(a->n, 16)), dim3(512), 0, st, (const float *)a->ws, a->wd, a->y,
+                       (int64_t)a->f, (int64_t)a->n, (int)a->M, (int)(a->f % 8 == 0 && aligned16(a->wd) && aligned16(a->ws)));
+    ASR_CHECK_LAUNCH("gff_few_kernel");
+    return ASR_OK;
+}
+template <int DT>
+static int gff_few_pick(const asr_gated_ff_args *a, hipStream_t st) {
+    return a->M <= 16 ? gff_few_run<DT, 1>(a, st) : a->M <= 32 ? gff_few_run<DT, 2>(a, st) : gff_few_run<DT, 4>(a, st);
+}
+
+extern "C" int asr_gated_ff_fwd(const asr_gated_ff_args *a, void *stream) {
+    ASR_CHECK(gff_check(a, "gated_ff_fwd", true));
+    ASR_CHECK_ARG(a->y, "gated_ff_fwd: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    const bool few = gff_few(a);
+    switch (a->dtype) {
+        case ASR_T_F32: return few ? gff_few_pick<ASR_T_F32>(a, st) : gff_run<ASR_T_F32>(a, false, st);
+        case ASR_T_BF16: return few ? gff_few_pick<ASR_T_BF16>(a, st) : gff_run<ASR_T_BF16>(a, false, st);
+        default: return few ? gff_few_pick<ASR_T_F16>(a, st) : gff_run<ASR_T_F16>(a, false, st);
+    }
+}
+
+extern "C" int asr_gated_ff_bwd(const asr_gated_ff_args *a, void *stream) {
+    ASR_CHECK(gff_check(a, "gated_ff_bwd", true));
+    ASR_CHECK_ARG(a->dy, "gated_ff_bwd: null pointer");
+    ASR_CHECK_ARG((a->dwg == nullptr) == (a->dwu == nullptr), "gated_ff_bwd: dwg and dwu come together");
+    hipStream_t st = (hipStream_t)stream;
+    switch (a->dtype) {
+        case ASR_T_F32: return gff_run<ASR_T_F32>(a, true, st);
+        case ASR_T_BF16: return gff_run<ASR_T_BF16>(a, true, st);
+        default: return gff_run<ASR_T_F16>(a, true, st);
+    }
+}

@@ -614,6 +614,21 @@ int64_t asr_qk_norm_rope_ws_floats(int D);
 int asr_qk_norm_rope_fwd(const asr_rope_args *a, void *stream);
 int asr_qk_norm_rope_bwd(const asr_rope_args *a, void *stream);
 
+/* Gated feed-forward block y = (act(x wg^T) * (x wu^T)) wd^T: x (M,d), wg / wu (f,d), wd (n,f), y (M,n), all row-major
+ * contiguous and of type dtype; act 0 = swish (a sigmoid(a)), 1 = gelu (a Phi(a)).  ws: asr_gated_ff_ws_bytes(a, backward)
+ * bytes, 16-byte aligned (depends on the shape, the type and the pointers' alignment; -1 for a refused shape).
+ * _bwd recomputes the block from x and writes dx (M,d), dwg, dwu (f,d), dwd (n,f); a NULL gradient is left out (dwg and dwu
+ * together).  Deterministic. */
+typedef struct {
+    const void *x, *wg, *wu, *wd, *dy;
+    void *y, *dx, *dwg, *dwu, *dwd, *ws;
+    int64_t M;
+    int d, f, n, dtype, act;
+} asr_gated_ff_args;
+int64_t asr_gated_ff_ws_bytes(const asr_gated_ff_args *a, int backward);
+int asr_gated_ff_fwd(const asr_gated_ff_args *a, void *stream);
+int asr_gated_ff_bwd(const asr_gated_ff_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
