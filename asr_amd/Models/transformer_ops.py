@@ -1,6 +1,7 @@
 """Differentiable operators of Transformer-style encoder layers on the HIP kernels.
 
     q, k = qk_norm_rope(q, k, q_weight, k_weight)      # per-head RMS norm and rotary positions
+    o = bucket_attention(q, k, v, table)               # softmax attention with a learned bias by distance bucket
     y = gated_feed_forward(x, w_gate, w_up, w_down)    # (act(x Wg^T) * (x Wu^T)) Wd^T
 
 Not in the reference, which has sinusoidal relative positions and a plain Swish block in these places
@@ -12,6 +13,7 @@ kernels too, without atomics: the same call gives the same bits.
 """
 import contextlib
 import ctypes as C
+import functools
 
 import torch
 
@@ -139,6 +141,170 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions=None, rot_dim=None, base=10
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
         return _QkNormRope.apply(q, k, q_weight, k_weight, pos, rot, float(base), float(eps))
     return _rope_fwd(q, k, q_weight, k_weight, pos, rot, float(base), float(eps))
+
+
+# ------------------------------------------------------------------------- attention with a bucketed bias --
+MAX_DISTANCE = 1024
+MAX_BUCKETS = 256
+
+
+@functools.lru_cache(maxsize=None)
+def bucket_edges(num_buckets, max_distance, causal):
+    """The distances at which a direction's buckets number first + 1, first + 2, ... begin.  A direction has n = num_buckets
+    buckets (half of them where keys may follow the query); the first n // 2 hold one distance each, the rest cut
+    [first, max_distance) in equal steps of the logarithm and the last goes on to infinity: edge i is the least whole x with
+    (x / first) ** steps >= (max_distance / first) ** i, found in whole numbers, so that no rounding moves a border."""
+    n = num_buckets if causal else num_buckets // 2
+    first, steps, got = n // 2, n - n // 2, []
+    x = first
+    for i in range(1, steps):
+        want = max_distance ** i * first ** steps
+        lo, hi = x, max_distance
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if mid ** steps * first ** i >= want:
+                hi = mid
+            else:
+                lo = mid + 1
+        x = lo
+        got.append(x)
+    return tuple(got)
+
+
+@functools.lru_cache(maxsize=None)
+def _edges_host(num_buckets, max_distance, causal):
+    e = bucket_edges(num_buckets, max_distance, causal)
+    return (C.c_int32 * max(1, len(e)))(*e)
+
+
+def _attn_args(q, k, v, table, lengths, keep, offset, causal, reach, scale, train):
+    B, Tq, H, D = q.shape
+    a = _lib.BucketAttentionArgs()
+    a.q, a.k, a.v, a.table = q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr()
+    a.edges_host = C.addressof(_edges_host(table.shape[0], reach, causal))
+    if lengths is not None:
+        a.lengths = lengths.data_ptr()
+    if offset is not None:
+        a.offset = offset.data_ptr()
+    if keep is not None:
+        a.keep = keep.data_ptr()
+    a.q_sb, a.q_st, a.q_sh, _ = q.stride()
+    a.k_sb, a.k_st, a.k_sh, _ = k.stride()
+    a.v_sb, a.v_st, a.v_sh, _ = v.stride()
+    a.B, a.Tq, a.Tk, a.H, a.Hk, a.D = B, Tq, k.shape[1], H, k.shape[2], D
+    a.nb, a.causal, a.dtype, a.train, a.scale = table.shape[0], int(causal), _DTYPES[q.dtype], int(train), scale
+    return a
+
+
+def _attn_workspace(lib, a, backward, device):
+    n = int(lib.asr_bucket_attention_ws_bytes(C.byref(a), int(backward)))
+    if n < 0:
+        check(-1)
+    return torch.empty(n, device=device, dtype=torch.uint8)
+
+
+def _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, train):
+    """out, and for training the row statistics and the output in float32 (out itself where it is)."""
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    if not out.numel() or not k.shape[1]:
+        return out.zero_(), None, None
+    lib = _lib.load()
+    a = _attn_args(q, k, v, table, lengths, keep, offset, causal, reach, scale, train)
+    a.out = out.data_ptr()
+    lse = out32 = None
+    if train:
+        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device, dtype=torch.float32)
+        out32 = out if q.dtype == torch.float32 else torch.empty(q.shape, device=q.device, dtype=torch.float32)
+        a.lse, a.out32 = lse.data_ptr(), out32.data_ptr()
+    with _on(q.device):
+        ws = _attn_workspace(lib, a, False, q.device)
+        a.ws = ws.data_ptr()
+        check(lib.asr_bucket_attention_fwd(C.byref(a), _stream(q.device)))
+    return out, lse, out32
+
+
+class _BucketAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, lengths, keep, offset, causal, reach, scale):
+        out, lse, out32 = _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, True)
+        if out32 is out:
+            out32 = None                                       # saved below as an output: a saved input copy would be a cycle
+            ctx.save_for_backward(q, k, v, table, lengths, keep, offset, lse, out)
+        else:
+            ctx.save_for_backward(q, k, v, table, lengths, keep, offset, lse, out32)
+        ctx.aux = (causal, reach, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, table, lengths, keep, offset, lse, out32 = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+        dt = torch.empty_like(table)
+        if not q.numel() or not k.shape[1]:
+            return (*(t.zero_() for t in (dq, dk, dv, dt)), None, None, None, None, None, None)
+        lib = _lib.load()
+        g = _heads(g)
+        a = _attn_args(q, k, v, table, lengths, keep, offset, *ctx.aux, True)
+        a.g, a.lse, a.out32, a.out = g.data_ptr(), lse.data_ptr(), out32.data_ptr(), out32.data_ptr()
+        a.g_sb, a.g_st, a.g_sh, _ = g.stride()
+        a.dq, a.dk, a.dv, a.dtable = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dt.data_ptr()
+        with _on(q.device):
+            ws = _attn_workspace(lib, a, True, q.device)
+            a.ws = ws.data_ptr()
+            check(lib.asr_bucket_attention_bwd(C.byref(a), _stream(q.device)))
+        return dq, dk, dv, dt, None, None, None, None, None, None
+
+
+def _per_utterance(who, name, t, B, q):
+    if not isinstance(t, torch.Tensor) or t.device != q.device or t.dtype not in (torch.int32, torch.int64) or t.shape != (B,):
+        raise RuntimeError(f"asr_amd.{who}: {name} must be ({B},) whole numbers on {q.device}")
+    return t.to(torch.int32).contiguous()
+
+
+def bucket_attention(q, k, v, table, lengths=None, keep=None, offset=None, causal=False, max_distance=128, scale=None):
+    """softmax(scale q k^T + table[bucket of each key's distance from the query]) v, differentiable in q, k, v and table.
+
+    q (B, Tq, H, D), k and v (B, Tk, Hk, D) with H a multiple of Hk (query head h reads key head h // (H / Hk)), table
+    (num_buckets, H) float32, scale 1 / sqrt(D) by default.  Query i of utterance b stands at position offset[b] + i
+    (``offset`` (B,), default zeros) and key j at position j; ``bucket_edges`` says how distances fall into buckets: with
+    ``causal`` a query reads only the keys up to its own position and all buckets are for the past, otherwise the second half
+    of the buckets is for the keys behind the query.  Keys from ``lengths[b]`` on and keys with ``keep[b, j]`` false are left
+    out, whatever they hold (infinities and NaN too); a query that no key is left for gets zeros, and passes no gradient.
+    D at most 128, num_buckets at most 256, max_distance at most 1024.  Without gradients, calls of at most 32 query
+    rows a key head (Tq H / Hk: one new frame against a cache) split the keys over the GPU."""
+    who = "bucket_attention"
+    _tensor(who, "q", q, 4)
+    _tensor(who, "k", k, 4, like=q)
+    _tensor(who, "v", v, 4, like=q)
+    _tensor(who, "table", table, 2, like=q, dtype=torch.float32)
+    B, Tq, H, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or H == 0 or k.shape[2] == 0 or H % k.shape[2]:
+        raise RuntimeError(f"asr_amd.{who}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    if not 1 <= D <= 128:
+        raise RuntimeError(f"asr_amd.{who}: head width {D}: must be in [1, 128]")
+    nb, causal, reach = table.shape[0], bool(causal), int(max_distance)
+    if table.shape[1] != H:
+        raise RuntimeError(f"asr_amd.{who}: table must be (buckets, {H}), got {tuple(table.shape)}")
+    if not 2 <= nb <= MAX_BUCKETS or (not causal and (nb < 4 or nb % 2)):
+        raise RuntimeError(f"asr_amd.{who}: {nb} buckets: 2 to {MAX_BUCKETS}, an even number of at least 4 unless causal")
+    if not (nb if causal else nb // 2) // 2 < reach <= MAX_DISTANCE:
+        raise RuntimeError(f"asr_amd.{who}: max_distance {reach}: must be beyond the single-distance buckets and at most "
+                           f"{MAX_DISTANCE}")
+    if lengths is not None:
+        lengths = _per_utterance(who, "lengths", lengths, B, q)
+    if offset is not None:
+        offset = _per_utterance(who, "offset", offset, B, q)
+    if keep is not None:
+        if (not isinstance(keep, torch.Tensor) or keep.device != q.device or keep.dtype not in (torch.bool, torch.uint8)
+                or keep.shape != (B, k.shape[1])):
+            raise RuntimeError(f"asr_amd.{who}: keep must be ({B}, {k.shape[1]}) truth values on {q.device}")
+        keep = keep.contiguous()
+    scale = D ** -0.5 if scale is None else float(scale)
+    q, k, v, table = _heads(q), _heads(k), _heads(v), table.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
+        return _BucketAttention.apply(q, k, v, table, lengths, keep, offset, causal, reach, scale)
+    return _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, False)[0]
 
 
 # ---------------------------------------------------------------------------------------- gated feed-forward --

@@ -90,6 +90,15 @@ class GatedFFArgs(C.Structure):
                 + [(n, C.c_int) for n in ("d", "f", "n", "dtype", "act")])
 
 
+class BucketAttentionArgs(C.Structure):
+    _fields_ = ([(n, c_f) for n in ("q", "k", "v", "g", "table", "edges_host", "lengths", "offset", "keep", "out", "out32", "lse",
+                                    "dq", "dk", "dv", "dtable", "ws")]
+                + [(n, c_i64) for n in ("q_sb", "q_st", "q_sh", "k_sb", "k_st", "k_sh", "v_sb", "v_st", "v_sh", "g_sb", "g_st",
+                                        "g_sh")]
+                + [(n, C.c_int) for n in ("B", "Tq", "Tk", "H", "Hk", "D", "nb", "causal", "dtype", "train")]
+                + [("scale", C.c_float)])
+
+
 # name -> (restype, argtypes); every symbol include/asr_amd.h declares
 SYMBOLS = {
     "asr_version": (C.c_int, []),
@@ -186,13 +195,16 @@ SYMBOLS = {
     "asr_col2im_3x3s2": (C.c_int, [c_f, c_f, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
     "asr_col2im_dw_blocks": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "asr_col2im_3x3s2_dw": (C.c_int, [c_f, c_f, c_f, C.c_int, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
-    # encoder-layer operators (csrc/rope.hip, gated_ff.hip)
+    # encoder-layer operators (csrc/rope.hip, gated_ff.hip, bucket_attn.hip)
     "asr_qk_norm_rope_ws_floats": (c_i64, [C.c_int]),
     "asr_qk_norm_rope_fwd": (C.c_int, [C.POINTER(RopeArgs), c_f]),
     "asr_qk_norm_rope_bwd": (C.c_int, [C.POINTER(RopeArgs), c_f]),
     "asr_gated_ff_ws_bytes": (c_i64, [C.POINTER(GatedFFArgs), C.c_int]),
     "asr_gated_ff_fwd": (C.c_int, [C.POINTER(GatedFFArgs), c_f]),
     "asr_gated_ff_bwd": (C.c_int, [C.POINTER(GatedFFArgs), c_f]),
+    "asr_bucket_attention_ws_bytes": (c_i64, [C.POINTER(BucketAttentionArgs), C.c_int]),
+    "asr_bucket_attention_fwd": (C.c_int, [C.POINTER(BucketAttentionArgs), c_f]),
+    "asr_bucket_attention_bwd": (C.c_int, [C.POINTER(BucketAttentionArgs), c_f]),
 }
 
 _lib = None

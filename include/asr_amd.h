@@ -629,6 +629,33 @@ int64_t asr_gated_ff_ws_bytes(const asr_gated_ff_args *a, int backward);
 int asr_gated_ff_fwd(const asr_gated_ff_args *a, void *stream);
 int asr_gated_ff_bwd(const asr_gated_ff_args *a, void *stream);
 
+/* Attention with a learned bias by the bucket of the distance between key and query: q (B,Tq,H,D), k / v (B,Tk,Hk,D), any
+ * strides with contiguous heads, table (nb,H) floats.  Query i of utterance b stands at offset[b] + i (offset NULL: 0), key j
+ * at j.  Buckets: nd = nb / 2 of them for each direction (causal: nb, for the past), the first nd / 2 hold one distance each,
+ * edges_host[0 .. nd - nd/2 - 2] (HOST array, rising, <= 1024) are the distances at which the others begin; keys after the
+ * query use the second half.  Keys j >= lengths[b] (NULL: Tk) and keys with keep[b,j] == 0 (NULL: all kept) are never read
+ * into a result; a query that no key is left for gets zeros.  H % Hk == 0, D <= 128, nb <= 256.
+ * _fwd: out (B,Tq,H,D) contiguous; train != 0 also writes lse (B,H,Tq) and, for 16-bit types, out32 (out in float32).
+ * _bwd: g is the upstream gradient, dq / dk / dv contiguous, dtable (nb,H).  ws: asr_bucket_attention_ws_bytes(a, backward)
+ * bytes (0: may be NULL; -1: refused).  Deterministic. */
+typedef struct {
+    const void *q, *k, *v, *g;
+    const float *table;
+    const int32_t *edges_host, *lengths, *offset;
+    const uint8_t *keep;
+    void *out;
+    float *out32, *lse;
+    void *dq, *dk, *dv;
+    float *dtable;
+    void *ws;
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
+    int B, Tq, Tk, H, Hk, D, nb, causal, dtype, train;
+    float scale;
+} asr_bucket_attention_args;
+int64_t asr_bucket_attention_ws_bytes(const asr_bucket_attention_args *a, int backward);
+int asr_bucket_attention_fwd(const asr_bucket_attention_args *a, void *stream);
+int asr_bucket_attention_bwd(const asr_bucket_attention_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

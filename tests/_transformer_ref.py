@@ -83,3 +83,87 @@ def held(got, want):
     bad = ~(err <= tol)
     assert not bad.any(), (int(bad.sum()), float((err / tol.clamp(min=1e-300)).max()), float(err.max()))
     return float((err / tol.clamp(min=1e-300)).max())
+
+
+def bucket64(r, nb, reach, causal):
+    """Bucket of each distance r (int64), by the definition, in whole numbers."""
+    n = nb if causal else nb // 2
+    first, steps = n // 2, n - n // 2
+
+    def one(x):
+        away = max(-x, 0) if causal else abs(x)
+        k = away
+        if away >= first:
+            k = first
+            while k < n - 1 and away ** steps * first ** (k - first + 1) >= reach ** (k - first + 1) * first ** steps:
+                k += 1
+        return k + (0 if causal or x <= 0 else n)
+    lo, hi = int(r.min()), int(r.max())
+    line = torch.tensor([one(x) for x in range(lo, hi + 1)], device=r.device)
+    return line[r - lo]
+
+
+def attention64(q, k, v, table, g, dtype, *, lengths, keep, offset, causal, reach, scale, train):
+    """Float64 attention and gradients with tolerances: [(value, tolerance)] for out, dq, dk, dv, dtable.
+
+    drop / u_p: what the products leave out of a term and the half step of the probabilities and score gradients between two
+    products, by type (pieces.h; bfloat16 probabilities carry 16 bits in training).  A score's absolute error es (its product,
+    the bias and scale in base 2) makes a relative error es of its probability; one exponential, the sum's roundings and
+    the quotient add `own`."""
+    B, Tq, H, D = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    G = H // Hk
+    drop, u_p, u_ds = {torch.float32: (3 * 2.0 ** -24, 2.0 ** -24, 2.0 ** -24), torch.float16: (2.0 ** -16, 2.0 ** -16, 2.0 ** -16),
+                       torch.bfloat16: (0.0, 2.0 ** -16 if train else 2.0 ** -8, 2.0 ** -8)}[dtype]
+    qq, gg = q.transpose(1, 2), None if g is None else g.transpose(1, 2)
+    j = torch.arange(Tk, device=q.device)
+    pos = torch.arange(Tq, device=q.device)[None] + (0 if offset is None else offset.long()[:, None])
+    r = j - pos[..., None]                                               # (B or 1, Tq, Tk)
+    slot = bucket64(r, table.shape[0], reach, causal)
+    ok = torch.ones(B, 1, Tq, Tk, dtype=torch.bool, device=q.device)
+    if lengths is not None:
+        ok = ok & (j < lengths[:, None])[:, None, None]
+    if keep is not None:
+        ok = ok & keep.bool()[:, None, None]
+    if causal:
+        ok = ok & (r <= 0)[:, None]
+    seen = ok.any(2).squeeze(1)                                          # keys that no query may read hold anything
+    kk, vv = (torch.where(seen[:, :, None, None], t, 0.0).transpose(1, 2).repeat_interleave(G, 1) for t in (k, v))
+    bias = table[slot].movedim(-1, 1)
+    s = torch.where(ok, qq @ kk.transpose(-1, -2) * scale + bias, -torch.inf)
+    size = (qq.abs() @ kk.abs().transpose(-1, -2)) * abs(scale)
+    es = (D * U32 + drop) * size + 6 * U32 * (size + bias.abs() + 1) + 4 * U32 * torch.where(ok, s.abs(), 0.0)
+    es = torch.where(ok, es, 0.0)
+    top = torch.where(ok.any(-1, keepdim=True), s.amax(-1, keepdim=True), 0.0)
+    es = es + 4 * U32 * (top.abs() + torch.where(ok, (s - top).abs(), 0.0))   # differences from the running maximum
+    e = torch.exp(s - top) * ok
+    p = e / e.sum(-1, keepdim=True).clamp(min=1e-300)
+    own = (Tk / 16 + 16) * U32
+    # float32 holds nothing below 2^-126 and the running maximum may lag by 2^8: a smaller probability becomes zero
+    ep = p * (es + (p * es).sum(-1, keepdim=True) + own) + 2.0 ** -118 * ok
+    out = p @ vv
+    eo = (ep + u_p * p) @ vv.abs() + (Tk * U32 + drop) * (p @ vv.abs())
+    res = [(out.transpose(1, 2), eo.transpose(1, 2))]
+    if gg is not None:
+        dp = gg @ vv.transpose(-1, -2)
+        edp = (D * U32 + drop) * (gg.abs() @ vv.abs().transpose(-1, -2))
+        delta = (gg * out).sum(-1, keepdim=True)
+        edelta = (gg.abs() * (eo + U32 * out.abs())).sum(-1, keepdim=True) + D * U32 * (gg * out).abs().sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        eds = ep * (dp - delta).abs() + p * (edp + edelta) + 4 * U32 * p * (dp.abs() + delta.abs())
+        back = lambda t: t.unflatten(1, (Hk, G)).sum(2).transpose(1, 2)  # noqa: E731
+        pt, dst, eph, edsh = (t.transpose(-1, -2) for t in (p, ds, ep + u_p * p if dtype != torch.bfloat16 else ep + 2.0 ** -8 * p,
+                                                            eds + u_ds * ds.abs()))
+        res.append(((ds @ kk * scale).transpose(1, 2),
+                    ((edsh.transpose(-1, -2) + (Tk * U32 + drop) * ds.abs()) @ kk.abs() * abs(scale)).transpose(1, 2)))
+        res.append((back(dst @ qq * scale), back((edsh + (G * Tq * U32 + drop) * dst.abs()) @ qq.abs() * abs(scale))))
+        res.append((back(pt @ gg), back((eph + (G * Tq * U32 + drop) * pt) @ gg.abs())))
+        dt, et = torch.zeros_like(table), torch.zeros_like(table)
+        slot = slot.expand(B, Tq, Tk).reshape(-1)
+        n = B * Tq * min(Tk, 4 * reach)
+        dt.index_add_(0, slot, ds.movedim(1, -1).reshape(-1, H))
+        et.index_add_(0, slot, (eds + min(n, 4096) * U32 * ds.abs()).movedim(1, -1).reshape(-1, H))
+        res.append((dt, et))
+    u = U[dtype]
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    return [(a, t + (u if i < 4 else U32) * (a.abs() + t) + (tiny if i < 4 else 0.0)) for i, (a, t) in enumerate(res)]

@@ -1,0 +1,251 @@
+"""GPU: bucket_attention against its definition in float64: element types, head layouts and widths, lengths from one frame on,
+masks that leave rows empty, what masked places hold, strides, few queries against a cache, gradients (the formula's, the
+table's, by differences), streams, captured graphs, refusals."""
+import pytest
+import torch
+
+from tests._transformer_ref import attention64, bucket64, held
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _inputs(B, Tq, Tk, H, Hk, D, dtype, nb=32, seed=0, scale=1.3):
+    g = torch.Generator().manual_seed(seed)
+    q, k, v, up = (torch.randn(B, T, h, D, generator=g) for T, h in ((Tq, H), (Tk, Hk), (Tk, Hk), (Tq, H)))
+    table = torch.randn(nb, H, generator=g)
+    return [t.to(dtype).to(DEV) for t in (q * scale, k * scale, v, up)] + [table.to(DEV)]
+
+
+def _check(q, k, v, up, table, *, lengths=None, keep=None, offset=None, causal=False, reach=128, scale=None, train=True, infer=True):
+    from asr_amd.Models.transformer_ops import bucket_attention
+    kw = dict(lengths=lengths, keep=keep, offset=offset, causal=causal, max_distance=reach, scale=scale)
+    d = [t.double() for t in (q, k, v, table)]
+    ref = dict(lengths=lengths, keep=keep, offset=offset, causal=causal, reach=reach, scale=scale or q.shape[-1] ** -0.5)
+    out = None
+    if infer:
+        out = bucket_attention(q, k, v, table, **kw)
+        assert out.is_contiguous() and out.dtype == q.dtype
+        held(out, attention64(*d, None, q.dtype, train=False, **ref)[0])
+    if not train:
+        return out
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, table)]
+    y = bucket_attention(*leaves, **kw)
+    grads = torch.autograd.grad(y, leaves, up)
+    want = attention64(*d, up.double(), q.dtype, train=True, **ref)
+    for got, w in zip((y.detach(), *grads), want):
+        held(got, w)
+    return grads
+
+
+def test_bucket_borders():
+    """The buckets of every distance up to beyond the last edge, read off a table that counts."""
+    from asr_amd.Models.transformer_ops import bucket_attention, bucket_edges
+    for nb, reach, causal in ((32, 128, False), (32, 128, True), (16, 64, False), (64, 448, True), (4, 2, False), (2, 3, True),
+                              (256, 1024, True), (250, 800, False), (6, 100, False), (7, 1024, True)):
+        T = reach + 70
+        slot = bucket64(torch.arange(-T + 1, T, device=DEV), nb, reach, causal)
+        assert len(bucket_edges(nb, reach, causal)) == (nb if causal else nb // 2) - (nb if causal else nb // 2) // 2 - 1
+        # one query in the middle, values that name their key: softmax weights give the biases back
+        table = torch.arange(nb, device=DEV, dtype=torch.float32)[:, None] * 0.04
+        q = torch.zeros(1, 1, 1, 8, device=DEV)
+        for sign in (-1, 1):
+            if causal and sign > 0:
+                continue
+            for away in sorted({0, 1, 2, *bucket_edges(nb, reach, causal), *(e - 1 for e in bucket_edges(nb, reach, causal)), T - 2}):
+                # two keys left: the one at the query's own place and the one `away` from it
+                at = T if sign < 0 else 0
+                keep = torch.zeros(1, T + 1, dtype=torch.bool, device=DEV)
+                keep[0, at] = keep[0, at + sign * away] = True
+                v = torch.zeros(1, T + 1, 1, 8, device=DEV)
+                v[0, at + sign * away] = 1.0
+                out = bucket_attention(q, torch.zeros_like(v), v, table, keep=keep, offset=torch.tensor([at], device=DEV), causal=causal,
+                                       max_distance=reach)
+                a, b = table[slot[T - 1 + sign * away], 0], table[slot[T - 1], 0]
+                want = 1.0 if away == 0 else float(torch.sigmoid((a - b).double()))
+                assert abs(float(out[0, 0, 0, 0]) - want) < 1e-5, (nb, reach, causal, sign * away)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("B,T,H,Hk,D", [
+    (1, 1, 1, 1, 1), (2, 2, 2, 1, 8), (1, 31, 4, 4, 64), (2, 33, 6, 3, 40), (1, 129, 2, 2, 128), (3, 65, 4, 1, 80), (2, 150, 4, 4, 32),
+    (1, 300, 3, 3, 9), (1, 97, 8, 2, 115), (2, 257, 2, 1, 96)])
+@pytest.mark.parametrize("causal", [False, True], ids=["both-sides", "causal"])
+def test_shapes_and_types(B, T, H, Hk, D, dtype, causal):
+    _check(*_inputs(B, T, T, H, Hk, D, dtype), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("causal", [False, True], ids=["both-sides", "causal"])
+def test_lengths_masks_and_empty_rows(dtype, causal):
+    q, k, v, up, t = _inputs(4, 140, 140, 4, 2, 64, dtype)
+    lengths = torch.tensor([140, 1, 0, 77], device=DEV)
+    _check(q, k, v, up, t, lengths=lengths, causal=causal)
+    keep = torch.rand(4, 140, generator=torch.Generator().manual_seed(1)).to(DEV) < 0.5
+    keep[0, :100] = False
+    keep[3] = False
+    _check(q, k, v, up, t, keep=keep, causal=causal)
+    _check(q, k, v, up, t, keep=keep.to(torch.uint8), lengths=lengths.int(), causal=causal)
+    grads = _check(q, k, v, up, t, lengths=torch.zeros(4, dtype=torch.int64, device=DEV), causal=causal)
+    assert not any(g.any() for g in grads)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_what_masked_places_hold_does_not_matter(dtype):
+    from asr_amd.Models.transformer_ops import bucket_attention
+    q, k, v, up, t = _inputs(2, 70, 70, 2, 1, 40, dtype)
+    lengths = torch.tensor([33, 70], device=DEV)
+    keep = torch.ones(2, 70, dtype=torch.bool, device=DEV)
+    keep[1, 5:9] = False
+    clean = _run(q, k, v, up, t, lengths, keep)
+    for junk in (float("inf"), -float("inf"), float("nan"), torch.finfo(dtype).min, torch.finfo(dtype).max):
+        k2, v2 = k.clone(), v.clone()
+        k2[0, 33:] = v2[0, 33:] = k2[1, 5:9] = v2[1, 5:9] = junk
+        for a, b in zip(clean, _run(q, k2, v2, up, t, lengths, keep)):
+            assert torch.equal(a, b), junk
+        few = bucket_attention(q[:, :3], k2, v2, t, lengths=lengths, keep=keep)
+        assert torch.equal(few, bucket_attention(q[:, :3], k, v, t, lengths=lengths, keep=keep))
+
+
+def _run(q, k, v, up, t, lengths, keep):
+    from asr_amd.Models.transformer_ops import bucket_attention
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, t)]
+    y = bucket_attention(*leaves, lengths=lengths, keep=keep)
+    return [y.detach(), *torch.autograd.grad(y, leaves, up)]
+
+
+def test_layouts():
+    for dtype in (torch.float32, torch.bfloat16):
+        g = torch.Generator().manual_seed(2)
+        p = torch.randn(2, 45, (4 + 2 * 2) * 64, generator=g).to(dtype).to(DEV)              # one packed projection
+        q, k, v = p[..., :256].unflatten(-1, (4, 64)), p[..., 256:384].unflatten(-1, (2, 64)), p[..., 384:].unflatten(-1, (2, 64))
+        _, _, _, up, t = _inputs(2, 45, 45, 4, 2, 64, dtype)
+        _check(q, k, v, up, t)
+        _check(q.transpose(1, 2).contiguous().transpose(1, 2), k, v.transpose(2, 3).contiguous().transpose(2, 3),
+               up.transpose(1, 2).contiguous().transpose(1, 2), t, causal=True)
+        buf = torch.randn(2 * 45 * 4 * 64 + 1, generator=g).to(dtype).to(DEV)                # off the 16-byte grid
+        _check(buf[1:].view(2, 45, 4, 64), k, v, up[:, :, :1].expand(-1, -1, 4, -1), t)
+
+
+def test_far_distances_and_large_scores():
+    q, k, v, up, t = _inputs(1, 600, 600, 2, 2, 32, torch.float32, nb=16)
+    _check(q, k, v, up, t, reach=40)
+    _check(q * 6, k * 6, v, up, t * 20, reach=300, causal=True)
+    _check(q, k, v, up, t, reach=1024, scale=0.01)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,D,causal", [
+    (3, 1, 700, 8, 2, 64, True), (1, 1, 5000, 4, 4, 128, True), (2, 5, 333, 6, 3, 40, False), (2, 4, 100, 8, 1, 96, True),
+    (1, 2, 31, 1, 1, 9, False), (16, 1, 65, 2, 1, 80, True)])
+def test_few_queries_against_a_cache(B, Tq, Tk, H, Hk, D, causal, dtype):
+    q, k, v, up, t = _inputs(B, Tq, Tk, H, Hk, D, dtype)
+    n = torch.randint(Tq, Tk + 1, (B,), generator=torch.Generator().manual_seed(4)).to(DEV)
+    n[0] = Tk
+    _check(q, k, v, up, t, lengths=n, offset=n - Tq, causal=causal)
+    _check(q, k, v, up, t, offset=torch.full((B,), Tk - Tq, device=DEV), causal=causal, train=False,
+           keep=torch.rand(B, Tk, generator=torch.Generator().manual_seed(5)).to(DEV) < 0.3)
+    _check(q, k, v, up, t, lengths=n * 0, offset=n, causal=causal, train=False)
+
+
+def test_chunks_of_a_stream_equal_the_whole():
+    """A causal pass in one call, in chunks against the growing cache, and frame by frame: the same rows."""
+    from asr_amd.Models.transformer_ops import bucket_attention
+    q, k, v, up, t = _inputs(2, 200, 200, 4, 2, 64, torch.float32)
+    whole = bucket_attention(q, k, v, t, causal=True)
+    want = attention64(*(x.double() for x in (q, k, v, t)), None, torch.float32, lengths=None, keep=None, offset=None, causal=True, reach=128,
+                       scale=64 ** -0.5, train=False)[0]
+    held(whole, want)
+    for step in (1, 7, 64):
+        for a in range(0, 200, step):
+            b = min(a + step, 200)
+            n = torch.full((2,), b, device=DEV)
+            got = bucket_attention(q[:, a:b], k, v, t, lengths=n, offset=n - (b - a), causal=True)     # the cache beyond b is not read
+            held(got, (want[0][:, a:b], want[1][:, a:b]))
+
+
+def test_offsets_before_and_beyond_the_keys():
+    q, k, v, up, t = _inputs(3, 40, 60, 2, 1, 32, torch.float32)
+    for off in ([-30, 500, 10], [-60, 2 ** 20, 0]):
+        _check(q, k, v, up, t, offset=torch.tensor(off, device=DEV), causal=True)
+        _check(q, k, v, up, t, offset=torch.tensor(off, device=DEV))
+
+
+def test_gradient_by_differences():
+    from asr_amd.Models.transformer_ops import bucket_attention
+    q, k, v, up, t = _inputs(2, 37, 37, 2, 1, 16, torch.float32, nb=8)
+    ts = [q, k, v, t]
+    leaves = [x.detach().requires_grad_() for x in ts]
+    kw = dict(lengths=torch.tensor([37, 20], device=DEV), max_distance=20)
+    grads = torch.autograd.grad(bucket_attention(*leaves, **kw), leaves, up)
+    for i, grad in enumerate(grads):
+        d = torch.randn(ts[i].shape, generator=torch.Generator().manual_seed(7)).to(DEV)
+        d = d / d.norm()
+        h = 2.0 ** -5
+        with torch.no_grad():
+            f = [(bucket_attention(*[x + s * h * d if j == i else x for j, x in enumerate(ts)], **kw).double() * up.double()).sum() for s in (1, -1)]
+        # h^2 / 6 of a third derivative of the order of the gradient along a unit direction, and float32 outputs over 2 h
+        assert abs(float((f[0] - f[1]) / (2 * h) - (grad.double() * d.double()).sum())) < 4e-3 * float(grad.double().norm())
+
+
+def test_the_same_call_gives_the_same_bits():
+    q, k, v, up, t = _inputs(2, 300, 300, 8, 2, 64, torch.bfloat16)
+    first = _run(q, k, v, up, t, None, None)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, _run(q, k, v, up, t, None, None)))
+
+
+def test_no_frames():
+    from asr_amd.Models.transformer_ops import bucket_attention
+    for B, Tq, Tk in ((0, 3, 3), (2, 0, 3), (2, 3, 0)):
+        q, k, v, up, t = _inputs(B, Tq, Tk, 2, 1, 16, torch.float32)
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, t)]
+        y = bucket_attention(*leaves)
+        assert y.shape == q.shape and not y.any()
+        assert not any(g.any() for g in torch.autograd.grad(y, leaves, up))
+
+
+@pytest.mark.parametrize("Tq", [1, 90])
+def test_another_stream_and_captured_graphs(Tq):
+    from asr_amd.Models.transformer_ops import bucket_attention
+    q, k, v, up, t = _inputs(2, Tq, 300, 4, 2, 64, torch.float32)
+    n = torch.tensor([300, 250], device=DEV, dtype=torch.int32)
+    call = lambda: bucket_attention(q, k, v, t, lengths=n, offset=n - Tq, causal=True)  # noqa: E731
+    want = call()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = call()
+    s.synchronize()
+    assert torch.equal(got, want)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    off = n - Tq
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(bucket_attention(q, k, v, t, lengths=n, offset=off, causal=True))
+    for seed in range(3):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(seed)))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = call()
+        assert all(torch.equal(o, want) for o in outs)
+
+
+def test_refusals():
+    from asr_amd.Models.transformer_ops import bucket_attention
+    q, k, v, up, t = _inputs(2, 5, 7, 4, 2, 16, torch.float32)
+    for bad in ((q.cpu(), k, v, t), (q.half(), k, v, t), (q.double(), k.double(), v.double(), t), (q, k[:, :5], v, t), (q, k[:1], v[:1], t),
+                (q[:, :, :3], k, v, t[:, :3]), (q, k, v, t[:, :2]), (q, k, v, t.half()), (q, k, v, t[:5]), (q, k, v, t[:2]), (q[0], k, v, t),
+                (q, k, v, torch.zeros(300, 4, device=DEV))):
+        with pytest.raises(RuntimeError):
+            bucket_attention(*bad)
+    for kw in (dict(lengths=torch.tensor([1, 2])), dict(lengths=torch.tensor([1], device=DEV)), dict(offset=torch.zeros(2, device=DEV)),
+               dict(keep=torch.ones(2, 5, dtype=torch.bool, device=DEV)), dict(keep=torch.ones(2, 7, device=DEV)), dict(max_distance=8),
+               dict(max_distance=1025), dict(max_distance=16, causal=True)):
+        with pytest.raises(RuntimeError):
+            bucket_attention(q, k, v, t, **kw)
+    big = torch.zeros(1, 1, 1, 129, device=DEV)
+    with pytest.raises(RuntimeError):
+        bucket_attention(big, big, big, torch.zeros(32, 1, device=DEV))
