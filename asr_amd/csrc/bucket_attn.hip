@@ -62,27 +62,33 @@ struct AttnParams {
     Buckets bk;
 };
 
-__device__ __forceinline__ int bucket_of(const Buckets &b, int r) {
+// What a workgroup keeps of the buckets: the edges, and the biases of one head times log2(e)
+struct BucketLds {
+    float tab[256];
+    int16_t edge[MAX_EDGES];
+};
+__device__ __forceinline__ int bucket_of(const Buckets &b, const int16_t *edge, int r) {
     const int away = b.causal ? max(-r, 0) : abs(r);
     int n = away;
     if (away >= b.first) {                       // edges <= away, by halving
         int lo = 0, hi = b.nedge;
         while (lo < hi) {
             const int m = (lo + hi) >> 1;
-            if (b.edge[m] <= away) lo = m + 1;
+            if (edge[m] <= away) lo = m + 1;
             else hi = m;
         }
         n = b.first + lo;
     }
     return n + (!b.causal && r > 0 ? b.nd : 0);
 }
-// biases by distance -R - PAD .. R + PAD of one head, times log2(e)
-__device__ __forceinline__ void fill_lut(float *lut, const AttnParams &p, int h) {
+// biases by distance -R - PAD .. R + PAD of one head, times log2(e); ends with the line written but not yet visible
+__device__ __forceinline__ void fill_lut(float *lut, BucketLds &s, const AttnParams &p, int h) {
     const int R = p.bk.R;
-    for (int i = threadIdx.x; i < 2 * (R + LUT_PAD) + 1; i += blockDim.x) {
-        const int r = min(max(i - R - LUT_PAD, -R), R);
-        lut[i] = p.table[bucket_of(p.bk, r) * p.H + h] * LOG2E;
-    }
+    for (int i = threadIdx.x; i < p.bk.nb; i += 256) s.tab[i] = p.table[i * p.H + h] * LOG2E;
+    if ((int)threadIdx.x < p.bk.nedge) s.edge[threadIdx.x] = p.bk.edge[threadIdx.x];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * (R + LUT_PAD) + 1; i += 256)
+        lut[i] = s.tab[bucket_of(p.bk, s.edge, min(max(i - R - LUT_PAD, -R), R))];
 }
 
 template <int DP> struct Img { static constexpr int PITCH = 2 * DP + 32; };
@@ -128,7 +134,7 @@ struct RowTile {
     const __bf16 *p;
     int64_t st, ps;
     u32x4p v[NP][NS];
-    unsigned ok;
+    unsigned ok, live;                           // live: of row t0 + threadIdx (below ROWS), whether it takes part
     __device__ __forceinline__ void init(const AttnMat &m, int64_t b, int64_t h) {
         p = m.p + b * m.sb + h * m.sh;
         st = m.st;
@@ -145,6 +151,13 @@ struct RowTile {
 #pragma unroll
             for (int q = 0; q < NP; ++q) v[q][i] = *reinterpret_cast<const u32x4p *>(p + q * ps + o);
         }
+    }
+    __device__ __forceinline__ void load_live(int t0, int n, const uint8_t *keep) {
+        const int row = t0 + threadIdx.x;
+        live = threadIdx.x < ROWS && row < n && (keep == nullptr || keep[row]) ? 1u : 0u;
+    }
+    __device__ __forceinline__ void store_live(unsigned char *m) const {
+        if (threadIdx.x < ROWS) m[threadIdx.x] = (unsigned char)live;
     }
     __device__ __forceinline__ void store(unsigned char *img) const {
 #pragma unroll
@@ -268,6 +281,8 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 128 ? 1 : 2) void battn_
     typedef typename ElemOf<DT>::type E;
     typedef RowTile<NP, DP, KT> Tile;
     extern __shared__ __attribute__((aligned(16))) unsigned char pool[];
+    __shared__ BucketLds bl;
+    __shared__ __attribute__((aligned(4))) unsigned char live[KT];
     unsigned char *ki = pool, *vi = pool + NP * Tile::IMG;
     float *lut = reinterpret_cast<float *>(pool + 2 * NP * Tile::IMG);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -282,7 +297,7 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 128 ? 1 : 2) void battn_
     const int R = p.bk.R;
     bf16x8 qf[NP][DP / 16];
     own_rows<NP, DP>(qf, p.q, b, h, min(i, p.Tq - 1), i < p.Tq, p.D, lane);
-    fill_lut(lut, p, h);
+    fill_lut(lut, bl, p, h);
     f32x16 o[DP / 32];
     zero16(o);
     float m = -INFINITY, ms = 0.f, l = 0.f;
@@ -294,15 +309,18 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 128 ? 1 : 2) void battn_
     if (kend > 0) {
         kt.load(0, kend, p.D, keep);
         vt.load(0, kend, p.D, keep);
+        kt.load_live(0, kend, keep);
     }
     for (int j0 = 0; j0 < kend; j0 += KT) {
         __syncthreads();
         kt.store(ki);
         vt.store(vi);
+        kt.store_live(live);
         __syncthreads();
         if (j0 + KT < kend) {
             kt.load(j0 + KT, kend, p.D, keep);
             vt.load(j0 + KT, kend, p.D, keep);
+            kt.load_live(j0 + KT, kend, keep);
         }
 #pragma unroll 1
         for (int s0 = 0; s0 < KT; s0 += 32) {
@@ -313,11 +331,13 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 128 ? 1 : 2) void battn_
             dot_rows<NP, DP>(s[0], ki, Tile::IMG, s0, qf, lane);
             add_bias<1>(s[0], c, lut, R, j + 4 * half - pos, j - pmax, j + 31 - pmin);
             if (j + 32 > kend || keep || (p.bk.causal && j + 31 > pmin)) {
+                const int seen = p.bk.causal ? pos - j - 4 * half : 64;                // register rows up to here are not after the query
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int jj = j + row_of(r, half);
-                    const bool ok = jj < kend && (!p.bk.causal || jj <= pos) && (keep == nullptr || keep[min(jj, p.Tk - 1)]);
-                    s[0][r] = ok ? s[0][r] : -INFINITY;
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const unsigned w = *reinterpret_cast<const unsigned *>(live + s0 + 8 * r4 + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[0][4 * r4 + e] = ((w >> (8 * e)) & 1) && 8 * r4 + e <= seen ? s[0][4 * r4 + e] : -INFINITY;
                 }
             }
             float mx = s[0][0];
@@ -379,11 +399,13 @@ __global__ __launch_bounds__(256) void battn_delta_kernel(const void *dout, int6
 // of the sums is fixed); tiles beyond the last edge add into a register.  At the end the lines are cut into
 // buckets in float64.
 template <int DT, int DP>
-__global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 64 ? 1 : 2) void battn_dq_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void battn_dq_kernel(AttnParams p) {
     constexpr int NP = ElemOf<DT>::NP, KT = KeyTile<NP>::N;
     typedef typename ElemOf<DT>::type E;
     typedef RowTile<NP, DP, KT> Tile;
     extern __shared__ __attribute__((aligned(16))) unsigned char pool[];
+    __shared__ BucketLds bl;
+    __shared__ __attribute__((aligned(4))) unsigned char live[KT];
     const int R = p.bk.R, LN = 2 * (R + LUT_PAD) + 1;
     unsigned char *ki = pool, *vi = pool + NP * Tile::IMG;
     float *lut = reinterpret_cast<float *>(pool + 2 * NP * Tile::IMG);
@@ -402,7 +424,7 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 64 ? 1 : 2) void battn_d
     own_rows<NP, DP>(qf, p.q, b, h, min(i, p.Tq - 1), on, p.D, lane);
     own_rows<NP, DP>(gf, p.g, b, h, min(i, p.Tq - 1), on, p.D, lane);
     const float lse = on ? p.lse[(int64_t)bh * p.Tq + i] : INFINITY, delta = on ? p.delta[(int64_t)bh * p.Tq + i] : 0.f;
-    fill_lut(lut, p, h);
+    fill_lut(lut, bl, p, h);
     for (int t = threadIdx.x; t < 8 * LN + 8; t += 256) line[t] = 0.f;
     float *mine = line + (wave * 2 + half) * LN;
     f32x16 dq[DP / 32];
@@ -416,15 +438,18 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 64 ? 1 : 2) void battn_d
     if (kend > 0) {
         kt.load(0, kend, p.D, keep);
         vt.load(0, kend, p.D, keep);
+        kt.load_live(0, kend, keep);
     }
     for (int j0 = 0; j0 < kend; j0 += KT) {
         __syncthreads();
         kt.store(ki);
         vt.store(vi);
+        kt.store_live(live);
         __syncthreads();
         if (j0 + KT < kend) {
             kt.load(j0 + KT, kend, p.D, keep);
             vt.load(j0 + KT, kend, p.D, keep);
+            kt.load_live(j0 + KT, kend, keep);
         }
 #pragma unroll 1
         for (int s0 = 0; s0 < KT; s0 += 32) {
@@ -439,11 +464,13 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 64 ? 1 : 2) void battn_d
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(s[0][r] - lse) * (s[1][r] - delta);
             if (j + 32 > kend || keep || (p.bk.causal && j + 31 > pmin)) {
+                const int seen = p.bk.causal ? pos - j - 4 * half : 64;                // register rows up to here are not after the query
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int jj = j + row_of(r, half);
-                    const bool ok = jj < kend && (!p.bk.causal || jj <= pos) && (keep == nullptr || keep[min(jj, p.Tk - 1)]);
-                    s[0][r] = ok ? s[0][r] : 0.f;
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const unsigned w = *reinterpret_cast<const unsigned *>(live + s0 + 8 * r4 + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[0][4 * r4 + e] = ((w >> (8 * e)) & 1) && 8 * r4 + e <= seen ? s[0][4 * r4 + e] : 0.f;
                 }
             }
             if (hi <= -R || lo >= R) {
@@ -472,20 +499,25 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 64 ? 1 : 2) void battn_d
     }
     if (on) put_acc<E, DP>((E *)p.dq + (((int64_t)b * p.Tq + i) * p.H + h) * p.D, dq, p.scale, p.D, half);
     __syncthreads();
+    for (int t = threadIdx.x; t < LN; t += 256) {
+        float a = line[t];
+#pragma unroll
+        for (int u = 1; u < 8; ++u) a += line[u * LN + t];
+        line[t] = a;
+    }
+    __syncthreads();
     for (int t = threadIdx.x; t < p.bk.nb; t += 256) {
         const bool right = !p.bk.causal && t >= p.bk.nd;
         const int k = right ? t - p.bk.nd : t;
-        int lo = k < p.bk.first ? k : k == p.bk.first ? k : p.bk.edge[k - p.bk.first - 1];
         const bool tail = k == p.bk.nd - 1;
-        const int hi = tail ? R + LUT_PAD + 1 : k < p.bk.first ? k + 1 : p.bk.edge[k - p.bk.first];
-        if (right) lo = max(lo, 1);
+        const int lo = max(k <= p.bk.first ? k : (int)bl.edge[k - p.bk.first - 1], right ? 1 : 0);
+        const int hi = tail ? R + LUT_PAD + 1 : k < p.bk.first ? k + 1 : (int)bl.edge[k - p.bk.first];
+        const float *x = line + R + LUT_PAD;
         double a = 0.0;
-        for (int w = lo; w < hi; ++w) {
-            const float *x = line + (right ? w : -w) + R + LUT_PAD;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) a += x[u * LN];
-        }
+#pragma unroll 8
+        for (int w = lo; w < hi; ++w) a += x[right ? w : -w];
         if (tail)
+#pragma unroll
             for (int u = 0; u < 4; ++u) a += line[8 * LN + (right ? 4 : 0) + u];
         p.tpart[((int64_t)qt * p.B * p.H + bh) * p.bk.nb + t] = (float)a;
     }
@@ -502,11 +534,12 @@ __global__ __launch_bounds__(64) void battn_table_kernel(const float *__restrict
 
 // ---------------------------------------------------------------------------------------------------- dK and dV --
 template <int DT, int DP>
-__global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 64 ? 1 : 2) void battn_dkv_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 2 : 1) void battn_dkv_kernel(AttnParams p) {
     constexpr int NP = ElemOf<DT>::NP, QT = KeyTile<NP>::N;
     typedef typename ElemOf<DT>::type E;
     typedef RowTile<NP, DP, QT> Tile;
     extern __shared__ __attribute__((aligned(16))) unsigned char pool[];
+    __shared__ BucketLds bl;
     unsigned char *qi = pool, *gi = pool + NP * Tile::IMG;
     float *stat = reinterpret_cast<float *>(pool + 2 * NP * Tile::IMG);                // lse and delta of the tile's queries
     float *lut = stat + 2 * QT;
@@ -532,26 +565,30 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 64 ? 1 : 2) void battn_d
             const int h = hk * p.G + gg;
             const float *lse = p.lse + ((int64_t)b * p.H + h) * p.Tq, *del = p.delta + ((int64_t)b * p.H + h) * p.Tq;
             __syncthreads();
-            fill_lut(lut, p, h);
+            fill_lut(lut, bl, p, h);
             Tile qt, gt;
             qt.init(p.q, b, h);
             gt.init(p.g, b, h);
+            float st = 0.f;                                                            // this thread's lse or delta of the next tile
+            auto load_stat = [&](int t0) {
+                const int i = t0 + (threadIdx.x & (QT - 1));
+                if (threadIdx.x < 2 * QT) st = i >= p.Tq ? (threadIdx.x < QT ? INFINITY : 0.f) : (threadIdx.x < QT ? lse : del)[i];
+            };
             if (i0 < p.Tq) {
                 qt.load(i0, p.Tq, p.D, nullptr);
                 gt.load(i0, p.Tq, p.D, nullptr);
+                load_stat(i0);
             }
             for (int t0 = i0; t0 < p.Tq; t0 += QT) {
                 __syncthreads();
                 qt.store(qi);
                 gt.store(gi);
-                for (int t = threadIdx.x; t < 2 * QT; t += 256) {
-                    const int i = t0 + (t < QT ? t : t - QT);
-                    stat[t] = t < QT ? (i < p.Tq ? lse[i] : INFINITY) : (i < p.Tq ? del[i] : 0.f);
-                }
+                if (threadIdx.x < 2 * QT) stat[threadIdx.x] = st;
                 __syncthreads();
                 if (t0 + QT < p.Tq) {
                     qt.load(t0 + QT, p.Tq, p.D, nullptr);
                     gt.load(t0 + QT, p.Tq, p.D, nullptr);
+                    load_stat(t0 + QT);
                 }
 #pragma unroll 1
                 for (int s0 = 0; s0 < QT; s0 += 32) {
@@ -610,15 +647,19 @@ __global__ __launch_bounds__(256) void battn_kvsum_kernel(const float *__restric
 
 // -------------------------------------------------------------------- a few queries against a long cache, forward --
 // The keys of a (utterance, key head) are cut into nsplit runs, one wave each; the G query heads of the group times the
-// queries are the tile's 32 columns, so the cache is read once.  K comes straight from memory as the left operand, V through
-// the wave's own LDS; float32 and float16 caches are split into pieces in registers on the way.  Bound: the cache's
-// bytes.  battn_join_kernel joins the runs.
+// queries are the tile's 32 columns, so the cache is read once.  A lane loads K as rows (16 bytes of its own key at a time,
+// the left operand as it lies) and V as whole lines for the wave's LDS image; the next 32 keys are in flight under the
+// current ones.  float32 and float16 caches are split into pieces in registers.  Bound: the cache's bytes.
+// battn_join_kernel joins the runs.
 template <int DT, int DP>
 __global__ __launch_bounds__(64) void battn_few_kernel(AttnParams p) {
-    constexpr int NP = ElemOf<DT>::NP, PITCH = Img<DP>::PITCH, IMG = 32 * PITCH;
+    constexpr int NP = ElemOf<DT>::NP, PITCH = Img<DP>::PITCH, IMG = 32 * PITCH, CH = DP / 8, NC = DP / 16;
     typedef typename ElemOf<DT>::type E;
+    constexpr int W = (int)sizeof(E) / 2;                                              // 16-byte words of eight elements
     extern __shared__ __attribute__((aligned(16))) unsigned char pool[];
     float *tab = reinterpret_cast<float *>(pool + NP * IMG);                           // [nb][G] biases of the group's heads
+    uint8_t *slot = reinterpret_cast<uint8_t *>(tab + p.bk.nb * p.G);                  // bucket by distance, -R - PAD .. R + PAD
+    __shared__ int16_t edge[MAX_EDGES];
     const int lane = threadIdx.x, half = lane >> 5, col = lane & 31;
     const int bhk = blockIdx.x, b = bhk / p.Hk, hk = bhk - b * p.Hk, sp = blockIdx.y;
     const int rows = p.G * p.Tq, R = p.bk.R, off = p.offset ? p.offset[b] : 0;
@@ -627,87 +668,116 @@ __global__ __launch_bounds__(64) void battn_few_kernel(AttnParams p) {
     if (p.bk.causal) n = min(n, max(off + p.Tq, 0));
     const int run = ((n + p.nsplit - 1) / p.nsplit + 31) / 32 * 32, jb = min(n, sp * run), je = min(n, jb + run);
     const uint8_t *keep = p.keep ? p.keep + (int64_t)b * p.Tk : nullptr;
-    for (int t = lane; t < p.bk.nb * p.G; t += 64) tab[t] = p.table[(t / p.G) * p.H + hk * p.G + t % p.G] * LOG2E;
-    // element access: 8 consecutive of a row, zeros past D
-    auto row8 = [&](const E *a, int d, float (&v)[8]) {
+    // eight elements of a row at d, raw; zeros past D
+    struct Raw { u32x4p w[W]; };
+    auto raw8 = [&](const E *a, int d) {
+        Raw r;
         if (p.vec) {
-            if (d < p.D) load_vec<E, 8>(a + d, v);
-            else
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.f;
+            for (int u = 0; u < W; ++u) r.w[u] = d < p.D ? reinterpret_cast<const u32x4p *>(a + d)[u] : u32x4p{0u, 0u, 0u, 0u};
         } else {
+            E t[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = d + e < p.D ? (float)a[d + e] : 0.f;
+            for (int e = 0; e < 8; ++e) t[e] = d + e < p.D ? a[d + e] : (E)0.f;
+            __builtin_memcpy(&r, t, sizeof(r));
         }
+        return r;
     };
-    auto pieces8 = [&](const float (&v)[8], u32x4p (&w)[NP]) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            unsigned x[NP];
-            split_pair<NP>(v[2 * e], v[2 * e + 1], x);
-#pragma unroll
-            for (int q = 0; q < NP; ++q) w[q][e] = x[q];
-        }
-    };
-    bf16x8 qf[NP][DP / 16];
-    {
-        const E *a = (const E *)p.qraw + b * p.q.sb + (int64_t)i * p.q.st + h * p.q.sh;
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-            float v[8];
+    auto pieces8 = [&](const Raw &r, bf16x8 (&o)[NP]) {
+        if constexpr (NP == 1) {
+            o[0] = __builtin_bit_cast(bf16x8, r.w[0]);
+        } else {
+            E t[8];
+            __builtin_memcpy(t, &r, sizeof(r));
             u32x4p w[NP];
-            row8(a, 16 * ks + 8 * half, v);
-            pieces8(v, w);
 #pragma unroll
-            for (int q = 0; q < NP; ++q) qf[q][ks] = __builtin_bit_cast(bf16x8, w[q]);
+            for (int e = 0; e < 4; ++e) {
+                unsigned x[NP];
+                split_pair<NP>((float)t[2 * e], (float)t[2 * e + 1], x);
+#pragma unroll
+                for (int q = 0; q < NP; ++q) w[q][e] = x[q];
+            }
+#pragma unroll
+            for (int q = 0; q < NP; ++q) o[q] = __builtin_bit_cast(bf16x8, w[q]);
         }
-    }
+    };
     const E *kb = (const E *)p.kraw + b * p.k.sb + (int64_t)hk * p.k.sh, *vb = (const E *)p.vraw + b * p.v.sb + (int64_t)hk * p.v.sh;
+    Raw kr[NC], vr[NC];
+    bool vok[NC];
+    auto load = [&](int j0) {
+        const E *k = kb + (int64_t)min(j0 + col, je - 1) * p.k.st;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) kr[c] = raw8(k, 16 * c + 8 * half);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int f = lane + 64 * c, j = j0 + f / CH;
+            vok[c] = j < je && (keep == nullptr || keep[j]);
+            vr[c] = raw8(vb + (int64_t)min(j, je - 1) * p.v.st, f % CH * 8);
+        }
+    };
+    if (jb < je) load(jb);
+    bf16x8 qf[NP][NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        bf16x8 w[NP];
+        pieces8(raw8((const E *)p.qraw + b * p.q.sb + (int64_t)i * p.q.st + h * p.q.sh, 16 * c + 8 * half), w);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) qf[q][c] = w[q];
+    }
+    const int pmin = off, pmax = off + p.Tq - 1;
+    const bool near = !(je - 1 - pmin <= -R || jb - pmax >= R);                        // some key of the run within the last edge
+    for (int t = lane; t < p.bk.nb * p.G; t += 64) tab[t] = p.table[(t / p.G) * p.H + hk * p.G + t % p.G] * LOG2E;
+    for (int t = lane; t < p.bk.nedge; t += 64) edge[t] = p.bk.edge[t];
+    __syncthreads();
+    if (near)
+        for (int t = lane; t < 2 * (R + LUT_PAD) + 1; t += 64) slot[t] = (uint8_t)bucket_of(p.bk, edge, min(max(t - R - LUT_PAD, -R), R));
+    __syncthreads();
     f32x16 o[DP / 32];
     zero16(o);
     float m = -INFINITY, ms = 0.f, l = 0.f;
     const float c = p.scale * LOG2E;
-    const float bl = tab[bucket_of(p.bk, -R) * p.G + g], br = tab[bucket_of(p.bk, R) * p.G + g];
-    const int pmin = off, pmax = off + p.Tq - 1;
+    const float bl = tab[(p.bk.nd - 1) * p.G + g], br = tab[(p.bk.causal ? 0 : p.bk.nb - 1) * p.G + g];
     for (int j0 = jb; j0 < je; j0 += 32) {
-        const int jr = j0 + col;                                                       // the key row this lane loads
-        const bool in = jr < je && (keep == nullptr || keep[jr]);
-        const E *kr = kb + (int64_t)min(jr, je - 1) * p.k.st, *vr = vb + (int64_t)min(jr, je - 1) * p.v.st;
         f32x16 s[1];
         zero16(s);
-        float kv[DP / 16][8], vv[DP / 16][8];
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) row8(kr, 16 * ks + 8 * half, kv[ks]);
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) row8(vr, 16 * ks + 8 * half, vv[ks]);
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-            u32x4p w[NP];
-            pieces8(kv[ks], w);
+        for (int ks = 0; ks < NC; ++ks) {
+            bf16x8 w[NP];
+            pieces8(kr[ks], w);
 #pragma unroll
             for (int t = NP - 1; t >= 0; --t)
 #pragma unroll
-                for (int q = t; q >= 0; --q) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w[q]), qf[t - q][ks], s[0], 0, 0, 0);
+                for (int q = t; q >= 0; --q) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[q], qf[t - q][ks], s[0], 0, 0, 0);
         }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-            u32x4p w[NP];
-            pieces8(vv[ks], w);
+        for (int ks = 0; ks < NC; ++ks) {
+            bf16x8 w[NP];
+            pieces8(vr[ks], w);
+            const int f = lane + 64 * ks;
 #pragma unroll
             for (int q = 0; q < NP; ++q)
-                *reinterpret_cast<u32x4p *>(pool + q * IMG + col * PITCH + (ks * 2 + half) * 16) = in ? w[q] : u32x4p{0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4p *>(pool + q * IMG + (f / CH) * PITCH + (f % CH) * 16) = vok[ks] ? __builtin_bit_cast(u32x4p, w[q]) : u32x4p{0u, 0u, 0u, 0u};
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        const bool far = j0 + 31 - pmin <= -R || j0 - pmax >= R;
-        const float bf = j0 - pmax >= R ? br : bl;
+        if (j0 + 32 < je) load(j0 + 32);
+        if (j0 + 31 - pmin <= -R || j0 - pmax >= R) {
+            const float bf = j0 - pmax >= R ? br : bl;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int jj = j0 + row_of(r, half);
-            const float bias = far ? bf : tab[bucket_of(p.bk, min(max(jj - pos, -R), R)) * p.G + g];
-            const bool ok = jj < je && (!p.bk.causal || jj <= pos) && (keep == nullptr || keep[min(jj, p.Tk - 1)]);
-            s[0][r] = ok ? __builtin_fmaf(s[0][r], c, bias) : -INFINITY;
+            for (int r = 0; r < 16; ++r) s[0][r] = __builtin_fmaf(s[0][r], c, bf);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[0][r] = __builtin_fmaf(s[0][r], c, tab[slot[min(max(j0 + row_of(r, half) - pos, -R), R) + R + LUT_PAD] * p.G + g]);
+        }
+        if (j0 + 32 > je || keep || (p.bk.causal && j0 + 31 > pmin)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int jj = j0 + row_of(r, half);
+                const bool ok = jj < je && (!p.bk.causal || jj <= pos) && (keep == nullptr || keep[min(jj, p.Tk - 1)]);
+                s[0][r] = ok ? s[0][r] : -INFINITY;
+            }
         }
         float mx = s[0][0];
 #pragma unroll
@@ -747,22 +817,24 @@ __global__ __launch_bounds__(64) void battn_few_kernel(AttnParams p) {
         p.pml[2 * at + 1] = l;
     }
 }
+// One workgroup a row; nsplit <= 64: a lane of each wave has one run's maximum and sum
 template <int DT>
 __global__ __launch_bounds__(128) void battn_join_kernel(AttnParams p) {
     typedef typename ElemOf<DT>::type E;
+    __shared__ float w[64];
     const int rows = p.G * p.Tq, bhk = blockIdx.x / rows, col = blockIdx.x % rows;
-    const int b = bhk / p.Hk, hk = bhk - b * p.Hk, g = col % p.G, i = col / p.G, d = threadIdx.x;
-    const float *ml = p.pml + 2 * ((int64_t)bhk * p.nsplit * rows + col), *po = p.po + ((int64_t)bhk * p.nsplit * rows + col) * p.D;
-    float m = -INFINITY;
-    for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, ml[2 * (int64_t)s * rows]);
-    const float ms = m == -INFINITY ? 0.f : m;
-    float l = 0.f, a = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float w = __builtin_amdgcn_exp2f(ml[2 * (int64_t)s * rows] - ms);
-        l += w * ml[2 * (int64_t)s * rows + 1];
-        if (d < p.D) a += w * po[(int64_t)s * rows * p.D + d];
-    }
+    const int b = bhk / p.Hk, hk = bhk - b * p.Hk, g = col % p.G, i = col / p.G, d = threadIdx.x, s = threadIdx.x & 63;
+    const int64_t at = (int64_t)bhk * p.nsplit * rows + col;
+    const float *po = p.po + at * p.D + min(d, p.D - 1);
+    const bool in = s < p.nsplit;
+    const float m = in ? p.pml[2 * (at + (int64_t)s * rows)] : -INFINITY, ls = in ? p.pml[2 * (at + (int64_t)s * rows) + 1] : 0.f;
+    const float top = wave_max(m), f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+    const float l = wave_sum(f * ls);
+    if (threadIdx.x < 64) w[s] = f;
+    __syncthreads();
+    float a = 0.f;
+#pragma unroll 16
+    for (int t = 0; t < p.nsplit; ++t) a += w[t] * po[(int64_t)t * rows * p.D];
     if (d < p.D) ((E *)p.out)[(((int64_t)b * p.Tq + i) * p.H + hk * p.G + g) * p.D + d] = (E)(l > 0.f ? a / l : (l == 0.f ? 0.f : l));
 }
 
@@ -808,10 +880,10 @@ static int64_t bup(int64_t v) { return (v + 255) / 256 * 256; }
 static int battn_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 static bool battn_few(const asr_bucket_attention_args *a) { return !a->train && (a->H / a->Hk) * a->Tq <= 32; }
 
-// Runs of a split cache: about four waves a compute unit, each run at least 64 keys long (a shorter one spends more on its
+// Runs of a split cache: about eight waves a compute unit, each run at least 64 keys long (a shorter one spends more on its
 // joined row than on its keys)
 static int battn_runs(const asr_bucket_attention_args *a) {
-    int64_t n = 1024 / ((int64_t)a->B * a->Hk);
+    int64_t n = 2048 / ((int64_t)a->B * a->Hk);
     if (n > a->Tk / 64) n = a->Tk / 64;
     if (n > 64) n = 64;
     return n < 1 ? 1 : (int)n;
@@ -976,7 +1048,7 @@ static int battn_fwd(const asr_bucket_attention_args *a, hipStream_t st) {
         const int64_t rows = (int64_t)p.G * p.Tq * a->B * a->Hk;
         p.po = (float *)a->ws;
         p.pml = p.po + rows * p.nsplit * a->D;
-        const size_t lds = NP * 32 * Img<DP>::PITCH + sizeof(float) * p.bk.nb * p.G;
+        const size_t lds = NP * 32 * Img<DP>::PITCH + sizeof(float) * p.bk.nb * p.G + (2 * (p.bk.R + LUT_PAD) + 1);
         ASR_CHECK(battn_lds(battn_few_kernel<DT, DP>, lds, "bucket_attention_fwd"));
         hipLaunchKernelGGL((battn_few_kernel<DT, DP>), dim3(a->B * a->Hk, p.nsplit), dim3(64), lds, st, p);
         if (p.nsplit > 1) hipLaunchKernelGGL((battn_join_kernel<DT>), dim3((unsigned)rows), dim3(128), 0, st, p);

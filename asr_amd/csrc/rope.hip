@@ -28,9 +28,11 @@ struct RopeParams {
     const int64_t *pos;
     int64_t pos_b;                       // position stride of a batch entry (0: one row for all)
     int64_t ntok;
-    int T, D, rot, hpu, nhb;             // hpu: head rows per unit of work, nhb: units per frame
+    int T, D, rot;
+    int hpu[2], nhb[2];                  // of each side: head rows per unit of work, units per frame
+    int blk[2];                          // workgroups of each side: queries first
     float eps;
-    float *part;                         // backward: [blocks][2][D]
+    float *part;                         // backward: [blocks][D]
 };
 
 // sine and cosine of 2 pi u for |u| <= 1/2: reduced to an eighth of a turn, Taylor to x^9 / x^10 (error below 3e-9)
@@ -84,42 +86,102 @@ struct RopeLane {
 template <int DT, int V, int G>
 __global__ __launch_bounds__(256) void rope_fwd_kernel(RopeParams p, RopeFreq fr) {
     typedef typename ElemOf<DT>::type E;
+    const int side = (int)blockIdx.x >= p.blk[0] ? 1 : 0;
+    const RopeTensor &q = p.t[side];
     const int l = threadIdx.x & (G - 1);
-    const int64_t unit = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t unit = (int64_t)(blockIdx.x - (side ? p.blk[0] : 0)) * (256 / G) + threadIdx.x / G;
     const bool on = l * V * 2 < p.D;             // lanes past the row (D / 2V not a power of two) only keep step
-    if (unit >= p.ntok * p.nhb) return;          // whole groups leave together
-    const int64_t tok = unit / p.nhb;
-    const int h0 = (int)(unit - tok * p.nhb) * p.hpu, Hall = p.t[0].H + p.t[1].H, h1 = min(h0 + p.hpu, Hall);
+    if (unit >= p.ntok * p.nhb[side]) return;    // whole groups leave together
+    const int64_t tok = unit / p.nhb[side];
+    const int h0 = (int)(unit - tok * p.nhb[side]) * p.hpu[side], h1 = min(h0 + p.hpu[side], q.H);
     RopeLane<V> L;
     L.init(p, fr, on ? l : 0);
     float s[V], c[V];
     L.angles(p, tok, s, c);
     const int64_t b = tok / p.T, t = tok - b * p.T;
     const float inv_d = 1.f / p.D;
+    float w1[V], w2[V];
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-        const RopeTensor &q = p.t[side];
-        const int a0 = max(h0 - (side ? p.t[0].H : 0), 0), a1 = min(h1 - (side ? p.t[0].H : 0), q.H);
-        if (a0 >= a1) continue;
-        float w1[V], w2[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) { w1[i] = q.w[L.lo + i]; w2[i] = q.w[L.hi + i]; }
-        const E *x = (const E *)q.x + b * q.xb + t * q.xt;
-        E *y = (E *)q.y + (tok * q.H) * p.D;
+    for (int i = 0; i < V; ++i) { w1[i] = q.w[L.lo + i]; w2[i] = q.w[L.hi + i]; }
+    const E *x = (const E *)q.x + b * q.xb + t * q.xt;
+    E *y = (E *)q.y + (tok * q.H) * p.D;
 #pragma unroll 4
-        for (int h = a0; h < a1; ++h) {
-            float u[V], v[V];
+    for (int h = h0; h < h1; ++h) {
+        float u[V], v[V];
+        load_vec<E, V>(x + h * q.xh + L.lo, u);
+        load_vec<E, V>(x + h * q.xh + L.hi, v);
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) ss += u[i] * u[i] + v[i] * v[i];
+        const float r = 1.f / sqrtf(group_sum<G>(on ? ss : 0.f) * inv_d + p.eps);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float n1 = u[i] * r * w1[i], n2 = v[i] * r * w2[i];
+            u[i] = n1 * c[i] - n2 * s[i];
+            v[i] = n2 * c[i] + n1 * s[i];
+        }
+        if (on) {
+            store_vec<E, V>(y + h * p.D + L.lo, u);
+            store_vec<E, V>(y + h * p.D + L.hi, v);
+        }
+    }
+}
+
+// A workgroup works on one side (half the accumulators and weights in registers: four waves a SIMD instead of two).  The
+// weight gradients stay in the lane over all its units; at the end the workgroup's groups are summed through LDS, one partial
+// row per workgroup, and rope_dw_kernel adds the rows in a fixed order.
+template <int DT, int V, int G>
+__global__ __launch_bounds__(256) void rope_bwd_kernel(RopeParams p, RopeFreq fr) {
+    typedef typename ElemOf<DT>::type E;
+    __shared__ float red[256 * 2 * V];
+    const int side = (int)blockIdx.x >= p.blk[0] ? 1 : 0;
+    const RopeTensor &q = p.t[side];
+    const int l = threadIdx.x & (G - 1);
+    const bool on = l * V * 2 < p.D;
+    RopeLane<V> L;
+    L.init(p, fr, on ? l : 0);
+    const float inv_d = 1.f / p.D;
+    float dw1[V], dw2[V], w1[V], w2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        dw1[i] = dw2[i] = 0.f;
+        w1[i] = q.w[L.lo + i];
+        w2[i] = q.w[L.hi + i];
+    }
+    const int64_t nunit = p.ntok * p.nhb[side], step = (int64_t)p.blk[side] * (256 / G);
+    for (int64_t unit = (int64_t)(blockIdx.x - (side ? p.blk[0] : 0)) * (256 / G) + threadIdx.x / G; unit < nunit; unit += step) {
+        const int64_t tok = unit / p.nhb[side];
+        const int h0 = (int)(unit - tok * p.nhb[side]) * p.hpu[side], h1 = min(h0 + p.hpu[side], q.H);
+        float s[V], c[V];
+        L.angles(p, tok, s, c);
+        const int64_t b = tok / p.T, t = tok - b * p.T;
+        const E *x = (const E *)q.x + b * q.xb + t * q.xt;
+        const E *g = (const E *)q.g + b * q.gb + t * q.gt;
+        E *y = (E *)q.y + (tok * q.H) * p.D;
+#pragma unroll 2
+        for (int h = h0; h < h1; ++h) {
+            float u[V], v[V], gu[V], gv[V];
             load_vec<E, V>(x + h * q.xh + L.lo, u);
             load_vec<E, V>(x + h * q.xh + L.hi, v);
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) ss += u[i] * u[i] + v[i] * v[i];
-            const float r = 1.f / sqrtf(group_sum<G>(on ? ss : 0.f) * inv_d + p.eps);
+            load_vec<E, V>(g + h * q.gh + L.lo, gu);
+            load_vec<E, V>(g + h * q.gh + L.hi, gv);
+            float ss = 0.f, sg = 0.f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float n1 = u[i] * r * w1[i], n2 = v[i] * r * w2[i];
-                u[i] = n1 * c[i] - n2 * s[i];
-                v[i] = n2 * c[i] + n1 * s[i];
+                const float n1 = gu[i] * c[i] + gv[i] * s[i], n2 = gv[i] * c[i] - gu[i] * s[i];
+                gu[i] = n1;
+                gv[i] = n2;
+                ss += u[i] * u[i] + v[i] * v[i];
+                sg += n1 * w1[i] * u[i] + n2 * w2[i] * v[i];
+            }
+            const float r = 1.f / sqrtf(group_sum<G>(on ? ss : 0.f) * inv_d + p.eps);
+            const float m = group_sum<G>(on ? sg : 0.f) * inv_d * r * r;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                dw1[i] += gu[i] * u[i] * r;
+                dw2[i] += gv[i] * v[i] * r;
+                u[i] = r * (gu[i] * w1[i] - u[i] * m);
+                v[i] = r * (gv[i] * w2[i] - v[i] * m);
             }
             if (on) {
                 store_vec<E, V>(y + h * p.D + L.lo, u);
@@ -127,112 +189,42 @@ __global__ __launch_bounds__(256) void rope_fwd_kernel(RopeParams p, RopeFreq fr
             }
         }
     }
-}
-
-// The weight gradients stay in the lane over all its units and are summed over the block's groups at the end, one
-// partial row per block; rope_dw_kernel adds the rows in a fixed order.
-template <int DT, int V, int G>
-__global__ __launch_bounds__(256) void rope_bwd_kernel(RopeParams p, RopeFreq fr) {
-    typedef typename ElemOf<DT>::type E;
-    __shared__ float red[256 * 2 * V];
-    const int l = threadIdx.x & (G - 1);
-    const bool on = l * V * 2 < p.D;
-    RopeLane<V> L;
-    L.init(p, fr, on ? l : 0);
-    const float inv_d = 1.f / p.D;
-    float dw[2][2][V];
+    // red[group][lane][half][i]: column (lane, half, i) of every group at the same offset, one thread a column
 #pragma unroll
-    for (int i = 0; i < V; ++i) dw[0][0][i] = dw[0][1][i] = dw[1][0][i] = dw[1][1][i] = 0.f;
-    float w[2][2][V];
-#pragma unroll
-    for (int side = 0; side < 2; ++side)
-#pragma unroll
-        for (int i = 0; i < V; ++i) { w[side][0][i] = p.t[side].w[L.lo + i]; w[side][1][i] = p.t[side].w[L.hi + i]; }
-    const int64_t nunit = p.ntok * p.nhb;
-    const int Hall = p.t[0].H + p.t[1].H;
-    for (int64_t unit = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G; unit < nunit; unit += (int64_t)gridDim.x * (256 / G)) {
-        const int64_t tok = unit / p.nhb;
-        const int h0 = (int)(unit - tok * p.nhb) * p.hpu, h1 = min(h0 + p.hpu, Hall);
-        float s[V], c[V];
-        L.angles(p, tok, s, c);
-        const int64_t b = tok / p.T, t = tok - b * p.T;
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            const RopeTensor &q = p.t[side];
-            const int a0 = max(h0 - (side ? p.t[0].H : 0), 0), a1 = min(h1 - (side ? p.t[0].H : 0), q.H);
-            const E *x = (const E *)q.x + b * q.xb + t * q.xt;
-            const E *g = (const E *)q.g + b * q.gb + t * q.gt;
-            E *y = (E *)q.y + (tok * q.H) * p.D;
-#pragma unroll 2
-            for (int h = a0; h < a1; ++h) {
-                float u[V], v[V], gu[V], gv[V];
-                load_vec<E, V>(x + h * q.xh + L.lo, u);
-                load_vec<E, V>(x + h * q.xh + L.hi, v);
-                load_vec<E, V>(g + h * q.gh + L.lo, gu);
-                load_vec<E, V>(g + h * q.gh + L.hi, gv);
-                float ss = 0.f, sg = 0.f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float n1 = gu[i] * c[i] + gv[i] * s[i], n2 = gv[i] * c[i] - gu[i] * s[i];
-                    gu[i] = n1;
-                    gv[i] = n2;
-                    ss += u[i] * u[i] + v[i] * v[i];
-                    sg += n1 * w[side][0][i] * u[i] + n2 * w[side][1][i] * v[i];
-                }
-                const float r = 1.f / sqrtf(group_sum<G>(on ? ss : 0.f) * inv_d + p.eps);
-                const float m = group_sum<G>(on ? sg : 0.f) * inv_d * r * r;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    dw[side][0][i] += gu[i] * u[i] * r;
-                    dw[side][1][i] += gv[i] * v[i] * r;
-                    u[i] = r * (gu[i] * w[side][0][i] - u[i] * m);
-                    v[i] = r * (gv[i] * w[side][1][i] - v[i] * m);
-                }
-                if (on) {
-                    store_vec<E, V>(y + h * p.D + L.lo, u);
-                    store_vec<E, V>(y + h * p.D + L.hi, v);
-                }
-            }
-        }
+    for (int i = 0; i < V; ++i) {
+        red[threadIdx.x * 2 * V + i] = on ? dw1[i] : 0.f;
+        red[threadIdx.x * 2 * V + V + i] = on ? dw2[i] : 0.f;
     }
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            red[threadIdx.x * 2 * V + i] = dw[side][0][i];
-            red[threadIdx.x * 2 * V + V + i] = dw[side][1][i];
-        }
-        __syncthreads();
-        if (threadIdx.x < G && on) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float a = 0.f, e = 0.f;
-                for (int k = threadIdx.x; k < 256; k += G) { a += red[k * 2 * V + i]; e += red[k * 2 * V + V + i]; }
-                float *out = p.part + ((int64_t)blockIdx.x * 2 + side) * p.D;
-                out[L.lo + i] = a;
-                out[L.hi + i] = e;
-            }
+    __syncthreads();
+    if (threadIdx.x < G * 2 * V) {
+        const int cl = threadIdx.x / (2 * V), ch = (threadIdx.x / V) & 1, ci = threadIdx.x % V;
+        float a = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < 256 / G; ++k) a += red[k * G * 2 * V + threadIdx.x];
+        if (cl * V * 2 < p.D) {
+            const int pair = cl * V, half = p.rot >> 1;
+            const int lo = pair < half ? pair : p.rot + (pair - half), hi = pair < half ? pair + half : lo + ((p.D - p.rot) >> 1);
+            p.part[(int64_t)blockIdx.x * p.D + (ch ? hi : lo) + ci] = a;
         }
     }
 }
 
-// dw[side][col] = sum over blocks of part[block][side][col]: 16 columns a block, 16 rows of it in parallel
-__global__ __launch_bounds__(256) void rope_dw_kernel(const float *__restrict__ part, int nblk, int D, float *__restrict__ dwq,
-                                                      float *__restrict__ dwk) {
-    __shared__ float red[16][17];
-    const int c = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4;
+// dw[col] = sum over a side's workgroups of part[block][col]: 16 columns a workgroup, 64 rows of it in parallel
+__global__ __launch_bounds__(1024) void rope_dw_kernel(const float *__restrict__ part, int nq, int nk, int D, float *__restrict__ dwq,
+                                                       float *__restrict__ dwk) {
+    __shared__ float red[64][17];
+    const int c = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4, k0 = blockIdx.y ? nq : 0, k1 = blockIdx.y ? nq + nk : nq;
     float a = 0.f;
-    if (c < 2 * D)
-        for (int k = r; k < nblk; k += 16) a += part[(int64_t)k * 2 * D + c];
+    if (c < D)
+#pragma unroll 8
+        for (int k = k0 + r; k < k1; k += 64) a += part[(int64_t)k * D + c];
     red[r][threadIdx.x & 15] = a;
     __syncthreads();
-    if (r == 0 && c < 2 * D) {
+    if (r == 0 && c < D) {
         float s = 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) s += red[k][threadIdx.x];
-        if (c < D) dwq[c] = s;
-        else dwk[c - D] = s;
+#pragma unroll 16
+        for (int k = 0; k < 64; ++k) s += red[k][threadIdx.x];
+        (blockIdx.y ? dwk : dwq)[c] = s;
     }
 }
 
@@ -279,32 +271,41 @@ static void rope_fill(const asr_rope_args *a, bool bwd, RopeParams &p, RopeFreq 
     for (int i = a->rot / 2; i < 64; ++i) fr.f[i] = 0.0;
 }
 
-// Head rows per unit: all of a frame's (one sine per pair and frame), fewer while the launch has less than 2^18 lanes of
-// work (a lane then waits on memory, and more of them in flight matter more than the sines).
+// Head rows per unit: all of a frame's on its side (one sine per pair and frame), fewer while the launch has less than 2^18
+// lanes of work (a lane then waits on memory, and more of them in flight matter more than the sines).
 static void rope_units(RopeParams &p, int G) {
-    const int Hall = p.t[0].H + p.t[1].H;
-    int hpu = Hall;
-    while (hpu > 1 && p.ntok * cdiv(Hall, hpu) * G < (1 << 18)) hpu = (hpu + 1) / 2;
-    p.hpu = hpu;
-    p.nhb = cdiv(Hall, hpu);
+    for (int s = 0; s < 2; ++s) {
+        int hpu = p.t[s].H;
+        const int Hall = p.t[0].H + p.t[1].H;
+        while (hpu > 1 && p.ntok * cdiv(Hall, hpu) * G < (1 << 18)) hpu = (hpu + 1) / 2;
+        p.hpu[s] = hpu;
+        p.nhb[s] = cdiv(p.t[s].H, hpu);
+    }
 }
 
+// Backward: as many workgroups as run at once (four a compute unit), each side its share by heads
 #define ROPE_BWD_BLOCKS 1024
-extern "C" int64_t asr_qk_norm_rope_ws_floats(int D) { return (int64_t)ROPE_BWD_BLOCKS * 2 * D; }
+extern "C" int64_t asr_qk_norm_rope_ws_floats(int D) { return (int64_t)(ROPE_BWD_BLOCKS + 2) * D; }
 
 template <int DT, int V, int G>
 static int rope_launch(RopeParams &p, const RopeFreq &fr, float *dwq, float *dwk, bool bwd, hipStream_t st) {
     rope_units(p, G);
-    const int64_t blocks = (p.ntok * p.nhb + 256 / G - 1) / (256 / G);
-    ASR_CHECK_ARG(blocks <= 0x7fffffff, "qk_norm_rope: too many frames");
+    int64_t need[2];
+    for (int s = 0; s < 2; ++s) need[s] = (p.ntok * p.nhb[s] + 256 / G - 1) / (256 / G);
+    ASR_CHECK_ARG(need[0] + need[1] <= 0x7fffffff, "qk_norm_rope: too many frames");
     if (!bwd) {
-        hipLaunchKernelGGL((rope_fwd_kernel<DT, V, G>), dim3((unsigned)blocks), dim3(256), 0, st, p, fr);
+        p.blk[0] = (int)need[0];
+        p.blk[1] = (int)need[1];
+        hipLaunchKernelGGL((rope_fwd_kernel<DT, V, G>), dim3((unsigned)(need[0] + need[1])), dim3(256), 0, st, p, fr);
         ASR_CHECK_LAUNCH("rope_fwd_kernel");
         return ASR_OK;
     }
-    const int nb = blocks < ROPE_BWD_BLOCKS ? (int)blocks : ROPE_BWD_BLOCKS;
-    hipLaunchKernelGGL((rope_bwd_kernel<DT, V, G>), dim3(nb), dim3(256), 0, st, p, fr);
-    hipLaunchKernelGGL(rope_dw_kernel, dim3(cdiv(2 * p.D, 16)), dim3(256), 0, st, p.part, nb, p.D, dwq, dwk);
+    for (int s = 0; s < 2; ++s) {
+        const int64_t share = (int64_t)ROPE_BWD_BLOCKS * p.t[s].H / (p.t[0].H + p.t[1].H) + 1;
+        p.blk[s] = (int)(need[s] < share ? need[s] : share);
+    }
+    hipLaunchKernelGGL((rope_bwd_kernel<DT, V, G>), dim3(p.blk[0] + p.blk[1]), dim3(256), 0, st, p, fr);
+    hipLaunchKernelGGL(rope_dw_kernel, dim3(cdiv(p.D, 16), 2), dim3(1024), 0, st, p.part, p.blk[0], p.blk[1], p.D, dwq, dwk);
     ASR_CHECK_LAUNCH("rope_bwd_kernel");
     return ASR_OK;
 }
