@@ -31,6 +31,7 @@ typedef short s16x8a __attribute__((ext_vector_type(8)));
 #define LUT_PAD 64
 #define MAX_EDGES 128
 #define MAX_REACH 1024
+#define PATCH 72                        // words of a patch row: four rows apart is half the banks
 
 // A (B, T, H, D) operand as NP planes of bf16
 struct AttnMat {
@@ -91,23 +92,30 @@ __device__ __forceinline__ void fill_lut(float *lut, BucketLds &s, const AttnPar
         lut[i] = s.tab[bucket_of(p.bk, s.edge, min(max(i - R - LUT_PAD, -R), R))];
 }
 
-template <int DP> struct Img { static constexpr int PITCH = 2 * DP + 32; };
-// One image serves both kinds of read without bank conflicts: the pitch is 32 B mod 64 B, so the eight rows of a
-// ds_read_b128 step over all banks in 32-byte steps and the four rows of a transposing read are disjoint.
-// rows r0 + lane&31, d = 16 ks + 8 half ..+7
+// An image holds rows of DP bf16 without padding; the 16-byte chunks of a row are permuted by an exclusive or that depends
+// on the row, so that both kinds of read are free of bank conflicts: the same chunk of 16 consecutive rows (ds_read_b128,
+// 256 B) falls on 16 different sixteenths of the banks, and 64 B of four consecutive rows (the transposing reads of
+// two 16-lane groups) on four different quarters.
+template <int DP>
+__device__ __forceinline__ int swz(int row) {
+    return DP == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : DP == 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3;
+}
+template <int DP>
+__device__ __forceinline__ int img_at(int row, int chunk) { return row * 2 * DP + ((chunk ^ swz<DP>(row)) << 4); }
+// rows r0 + lane&31, d = 16 ks + 8 half ..+7; r0 is a multiple of 16
 template <int DP>
 __device__ __forceinline__ bf16x8 frag_rows(const unsigned char *img, int r0, int ks, int lane) {
-    const u32x4p v = *reinterpret_cast<const u32x4p *>(img + (r0 + (lane & 31)) * Img<DP>::PITCH + (ks * 2 + (lane >> 5)) * 16);
+    const u32x4p v = *reinterpret_cast<const u32x4p *>(img + r0 * 2 * DP + img_at<DP>(lane & 31, ks * 2 + (lane >> 5)));
     return __builtin_bit_cast(bf16x8, v);
 }
 // transposed: rows d = d0 + lane&31; summed index slot (half, e) = image row r0 + 16 c + 8 (e / 4) + 4 half + e % 4
 template <int DP>
 __device__ __forceinline__ bf16x8 frag_cols(const unsigned char *img, int r0, int c, int d0, int lane) {
-    const int q = (lane & 15) >> 2, p = lane & 3;
-    const unsigned char *a = img + (r0 + 16 * c + 4 * (lane >> 5) + q) * Img<DP>::PITCH + (d0 + 16 * ((lane >> 4) & 1) + 4 * p) * 2;
+    const int q = 4 * (lane >> 5) + ((lane & 15) >> 2), p = lane & 3, ch = d0 / 8 + 2 * ((lane >> 4) & 1) + (p >> 1);
+    const unsigned char *a = img + (r0 + 16 * c) * 2 * DP + 8 * (p & 1);
     typedef __attribute__((address_space(3))) s16x4a *lds_p;
-    const s16x4a v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a));
-    const s16x4a v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 8 * Img<DP>::PITCH));
+    const s16x4a v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + img_at<DP>(q, ch)));
+    const s16x4a v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + img_at<DP>(q + 8, ch)));
     const s16x8a v = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
     return __builtin_bit_cast(bf16x8, v);
 }
@@ -130,7 +138,7 @@ __device__ __forceinline__ void own_rows(bf16x8 (&f)[NP][DP / 16], const AttnMat
 // A tile of ROWS rows of one head on its way into LDS; rows from `n` on, rows that `keep` drops and columns past D are zeros
 template <int NP, int DP, int ROWS>
 struct RowTile {
-    static constexpr int CH = DP / 8, NS = (ROWS * CH + 255) / 256, IMG = ROWS * Img<DP>::PITCH;
+    static constexpr int CH = DP / 8, NS = (ROWS * CH + 255) / 256, IMG = ROWS * 2 * DP;
     const __bf16 *p;
     int64_t st, ps;
     u32x4p v[NP][NS];
@@ -167,7 +175,7 @@ struct RowTile {
             const u32x4p z = {0u, 0u, 0u, 0u};
 #pragma unroll
             for (int q = 0; q < NP; ++q)
-                *reinterpret_cast<u32x4p *>(img + q * IMG + (f / CH) * Img<DP>::PITCH + (f % CH) * 16) = (ok >> i) & 1 ? v[q][i] : z;
+                *reinterpret_cast<u32x4p *>(img + q * IMG + img_at<DP>(f / CH, f % CH)) = (ok >> i) & 1 ? v[q][i] : z;
         }
     }
 };
@@ -394,9 +402,10 @@ __global__ __launch_bounds__(256) void battn_delta_kernel(const void *dout, int6
 }
 
 // ------------------------------------------------------------------------------------- dQ and the table's gradient --
-// Sums of dS by distance: each half of a wave adds into a line of its own in LDS (ds_add_f32; the 32 lanes of a half differ
-// in their distance, so no two lanes of an instruction meet, and a wave's LDS instructions keep their order: the order
-// of the sums is fixed); tiles beyond the last edge add into a register.  At the end the lines are cut into
+// Sums of dS by distance: 16 keys of a tile at a time go to a patch of LDS of the wave's own, [16][32 + 16 zeros on both
+// sides], and lane t adds up the diagonal of distance t - 31 along it (consecutive lanes read consecutive words; the
+// zeros stand in for what lies outside), then adds it to the wave's line of sums by distance.  LDS float atomics in its
+// place took 250 cycles an instruction: 112 of 302 us of a float32 step at 32 x 374 frames.  Tiles beyond the last edge add into a register.  At the end the lines are cut into
 // buckets in float64.
 template <int DT, int DP>
 __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void battn_dq_kernel(AttnParams p) {
@@ -409,7 +418,7 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
     const int R = p.bk.R, LN = 2 * (R + LUT_PAD) + 1;
     unsigned char *ki = pool, *vi = pool + NP * Tile::IMG;
     float *lut = reinterpret_cast<float *>(pool + 2 * NP * Tile::IMG);
-    float *line = lut + LN;                                                            // 8 lines, then 2 x 4 far sums
+    float *line = lut + LN;                                                            // 4 lines, 2 x 4 far sums, 4 patches
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int bh = blockIdx.x % (p.B * p.H), b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
     const int qt = p.ntile - 1 - (int)(blockIdx.x / (p.B * p.H)), q0 = qt * 128;
@@ -425,8 +434,8 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
     own_rows<NP, DP>(gf, p.g, b, h, min(i, p.Tq - 1), on, p.D, lane);
     const float lse = on ? p.lse[(int64_t)bh * p.Tq + i] : INFINITY, delta = on ? p.delta[(int64_t)bh * p.Tq + i] : 0.f;
     fill_lut(lut, bl, p, h);
-    for (int t = threadIdx.x; t < 8 * LN + 8; t += 256) line[t] = 0.f;
-    float *mine = line + (wave * 2 + half) * LN;
+    for (int t = threadIdx.x; t < 4 * LN + 8 + 4 * 16 * PATCH; t += 256) line[t] = 0.f;
+    float *mine = line + wave * LN, *patch = line + 4 * LN + 8 + wave * 16 * PATCH;
     f32x16 dq[DP / 32];
     zero16(dq);
     float farl = 0.f, farr = 0.f;
@@ -480,11 +489,22 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
                 if (hi <= -R) farl += t;
                 else farr += t;
             } else {
-                float *d = mine + first + R + LUT_PAD;
+                // lane's diagonal of rows u: distance j + 16 u + t - 31 - (pmin .. ) where t = key row - query column + 31
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    __hip_atomic_fetch_add(d + 8 * (r >> 2) + (r & 3), s[0][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                for (int u = 0; u < 2; ++u) {
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) patch[row_of(r, half) * PATCH + 16 + (lane & 31)] = s[0][8 * u + r];
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    if (lane < 47) {
+                        float a = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) a += patch[k * (PATCH + 1) + 47 - lane];
+                        float *d = mine + (j + 16 * u - pmin) + lane - 31 + R + LUT_PAD;
+                        *d += a;
+                    }
                 }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
             bf16x8 df[NP][2];
             to_operand<NP>(df, s[0]);
@@ -494,15 +514,15 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
     farl = wave_sum(farl);
     farr = wave_sum(farr);
     if (lane == 0) {
-        line[8 * LN + wave] = farl;
-        line[8 * LN + 4 + wave] = farr;
+        line[4 * LN + wave] = farl;
+        line[4 * LN + 4 + wave] = farr;
     }
     if (on) put_acc<E, DP>((E *)p.dq + (((int64_t)b * p.Tq + i) * p.H + h) * p.D, dq, p.scale, p.D, half);
     __syncthreads();
     for (int t = threadIdx.x; t < LN; t += 256) {
         float a = line[t];
 #pragma unroll
-        for (int u = 1; u < 8; ++u) a += line[u * LN + t];
+        for (int u = 1; u < 4; ++u) a += line[u * LN + t];
         line[t] = a;
     }
     __syncthreads();
@@ -518,7 +538,7 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
         for (int w = lo; w < hi; ++w) a += x[right ? w : -w];
         if (tail)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) a += line[8 * LN + (right ? 4 : 0) + u];
+            for (int u = 0; u < 4; ++u) a += line[4 * LN + (right ? 4 : 0) + u];
         p.tpart[((int64_t)qt * p.B * p.H + bh) * p.bk.nb + t] = (float)a;
     }
 }
@@ -544,8 +564,9 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 
     float *stat = reinterpret_cast<float *>(pool + 2 * NP * Tile::IMG);                // lse and delta of the tile's queries
     float *lut = stat + 2 * QT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    // id = (tile, group of heads, utterance and key head): causal, the first keys have most queries and start first
     const int bhk = blockIdx.x % (p.B * p.Hk), b = bhk / p.Hk, hk = bhk - b * p.Hk;
-    const int k0 = (int)(blockIdx.x / (p.B * p.Hk)) * 128;                             // causal: the first keys have most queries
+    const int gs = blockIdx.x / (p.B * p.Hk) % p.gsplit, k0 = (int)(blockIdx.x / (p.B * p.Hk) / p.gsplit) * 128;
     const int off = p.offset ? p.offset[b] : 0;
     const int n = keys_of(p, b);
     const int R = p.bk.R;
@@ -559,7 +580,7 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 
     zero16(dv);
     const float c = p.scale * LOG2E;
     const int i0 = p.bk.causal ? max(0, k0 - off) / QT * QT : 0;                       // the first query that sees the tile's first key
-    const int per = (p.G + p.gsplit - 1) / p.gsplit, g0 = blockIdx.y * per, g1 = min(p.G, g0 + per);
+    const int per = (p.G + p.gsplit - 1) / p.gsplit, g0 = gs * per, g1 = min(p.G, g0 + per);
     if (k0 < n)
         for (int gg = g0; gg < g1; ++gg) {
             const int h = hk * p.G + gg;
@@ -600,7 +621,11 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 
                     dot_rows<NP, DP>(s[0], qi, Tile::IMG, s0, kf, lane);
                     dot_rows<NP, DP>(s[1], gi, Tile::IMG, s0, vf, lane);
                     add_bias<-1>(s[0], c, lut, R, j - (pmin + 4 * half), jw - pmax, jw + 31 - pmin);
-                    const bool edge = p.bk.causal && jw + 31 > pmin;
+                    // (a key that is left out collects what it likes in its own column and is stored as zeros)
+                    if (p.bk.causal && jw + 31 > pmin) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[0][r] = j <= pmin + row_of(r, half) ? s[0][r] : -INFINITY;
+                    }
 #pragma unroll
                     for (int r4 = 0; r4 < 4; ++r4) {
                         const float4 ls = *reinterpret_cast<const float4 *>(stat + s0 + 8 * r4 + 4 * half);
@@ -609,10 +634,8 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = 4 * r4 + e;
-                            const bool ok = on && (!edge || j <= pmin + 8 * r4 + 4 * half + e);
-                            const float pr = ok ? __builtin_amdgcn_exp2f(s[0][r] - lv[e]) : 0.f;
-                            s[0][r] = pr;
-                            s[1][r] = ok ? pr * (s[1][r] - dd[e]) : 0.f;
+                            s[0][r] = __builtin_amdgcn_exp2f(s[0][r] - lv[e]);
+                            s[1][r] = s[0][r] * (s[1][r] - dd[e]);
                         }
                     }
                     bf16x8 f[NP][2];
@@ -625,10 +648,14 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 
         }
     if (j >= p.Tk) return;
     const int64_t row = (((int64_t)b * p.Tk + j) * p.Hk + hk) * p.D;
+    if (!on) {
+        zero16(dk);
+        zero16(dv);
+    }
     if (p.gsplit > 1) {
         const int64_t sz = (int64_t)p.B * p.Tk * p.Hk * p.D;
-        put_acc<float, DP>(p.kvpart + (int64_t)blockIdx.y * 2 * sz + row, dk, p.scale, p.D, half);
-        put_acc<float, DP>(p.kvpart + ((int64_t)blockIdx.y * 2 + 1) * sz + row, dv, 1.f, p.D, half);
+        put_acc<float, DP>(p.kvpart + (int64_t)gs * 2 * sz + row, dk, p.scale, p.D, half);
+        put_acc<float, DP>(p.kvpart + ((int64_t)gs * 2 + 1) * sz + row, dv, 1.f, p.D, half);
     } else {
         put_acc<E, DP>((E *)p.dk + row, dk, p.scale, p.D, half);
         put_acc<E, DP>((E *)p.dv + row, dv, 1.f, p.D, half);
@@ -653,7 +680,7 @@ __global__ __launch_bounds__(256) void battn_kvsum_kernel(const float *__restric
 // battn_join_kernel joins the runs.
 template <int DT, int DP>
 __global__ __launch_bounds__(64) void battn_few_kernel(AttnParams p) {
-    constexpr int NP = ElemOf<DT>::NP, PITCH = Img<DP>::PITCH, IMG = 32 * PITCH, CH = DP / 8, NC = DP / 16;
+    constexpr int NP = ElemOf<DT>::NP, IMG = 32 * 2 * DP, CH = DP / 8, NC = DP / 16;
     typedef typename ElemOf<DT>::type E;
     constexpr int W = (int)sizeof(E) / 2;                                              // 16-byte words of eight elements
     extern __shared__ __attribute__((aligned(16))) unsigned char pool[];
@@ -757,7 +784,7 @@ __global__ __launch_bounds__(64) void battn_few_kernel(AttnParams p) {
             const int f = lane + 64 * ks;
 #pragma unroll
             for (int q = 0; q < NP; ++q)
-                *reinterpret_cast<u32x4p *>(pool + q * IMG + (f / CH) * PITCH + (f % CH) * 16) = vok[ks] ? __builtin_bit_cast(u32x4p, w[q]) : u32x4p{0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4p *>(pool + q * IMG + img_at<DP>(f / CH, f % CH)) = vok[ks] ? __builtin_bit_cast(u32x4p, w[q]) : u32x4p{0u, 0u, 0u, 0u};
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -1048,7 +1075,7 @@ static int battn_fwd(const asr_bucket_attention_args *a, hipStream_t st) {
         const int64_t rows = (int64_t)p.G * p.Tq * a->B * a->Hk;
         p.po = (float *)a->ws;
         p.pml = p.po + rows * p.nsplit * a->D;
-        const size_t lds = NP * 32 * Img<DP>::PITCH + sizeof(float) * p.bk.nb * p.G + (2 * (p.bk.R + LUT_PAD) + 1);
+        const size_t lds = NP * 32 * 2 * DP + sizeof(float) * p.bk.nb * p.G + (2 * (p.bk.R + LUT_PAD) + 1);
         ASR_CHECK(battn_lds(battn_few_kernel<DT, DP>, lds, "bucket_attention_fwd"));
         hipLaunchKernelGGL((battn_few_kernel<DT, DP>), dim3(a->B * a->Hk, p.nsplit), dim3(64), lds, st, p);
         if (p.nsplit > 1) hipLaunchKernelGGL((battn_join_kernel<DT>), dim3((unsigned)rows), dim3(128), 0, st, p);
@@ -1087,13 +1114,13 @@ static int battn_bwd(const asr_bucket_attention_args *a, hipStream_t st) {
                        DT == ASR_T_F32 ? (const float *)a->out : a->out32, delta, a->B, a->Tq, a->H, a->D);
     ASR_CHECK_LAUNCH("battn_delta_kernel");
     const size_t img = 2 * NP * RowTile<NP, DP, KT>::IMG, line = 2 * (p.bk.R + LUT_PAD) + 1;
-    const size_t lds_q = img + sizeof(float) * (9 * line + 8), lds_k = img + sizeof(float) * (2 * KT + line);
+    const size_t lds_q = img + sizeof(float) * (5 * line + 8 + 4 * 16 * PATCH), lds_k = img + sizeof(float) * (2 * KT + line);
     ASR_CHECK(battn_lds(battn_dq_kernel<DT, DP>, lds_q, "bucket_attention_bwd"));
     hipLaunchKernelGGL((battn_dq_kernel<DT, DP>), dim3((unsigned)(a->B * a->H) * pl.ntile), dim3(256), lds_q, st, p);
     ASR_CHECK_LAUNCH("battn_dq_kernel");
     hipLaunchKernelGGL(battn_table_kernel, dim3(a->nb, a->H), dim3(64), 0, st, p.tpart, a->dtable, a->B, a->H, pl.ntile, a->nb);
     ASR_CHECK(battn_lds(battn_dkv_kernel<DT, DP>, lds_k, "bucket_attention_bwd"));
-    hipLaunchKernelGGL((battn_dkv_kernel<DT, DP>), dim3((unsigned)(a->B * a->Hk) * cdiv(a->Tk, 128), pl.gsplit), dim3(256), lds_k, st, p);
+    hipLaunchKernelGGL((battn_dkv_kernel<DT, DP>), dim3((unsigned)(a->B * a->Hk) * cdiv(a->Tk, 128) * pl.gsplit), dim3(256), lds_k, st, p);
     ASR_CHECK_LAUNCH("battn_dkv_kernel");
     if (pl.gsplit > 1) {
         const int64_t sz = (int64_t)a->B * a->Tk * a->Hk * a->D, nb = (2 * sz + 255) / 256;
