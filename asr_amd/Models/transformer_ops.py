@@ -24,7 +24,8 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of the device's current stream (a fifth of the host time of torch.cuda.current_stream's stream object)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _on(device):
@@ -66,8 +67,7 @@ def _rope_args(q, k, wq, wk, pos, rot, base, eps):
 
 
 def _rope_fwd(q, k, wq, wk, pos, rot, base, eps):
-    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    ko = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
     if qo.numel():
         a = _rope_args(q, k, wq, wk, pos, rot, base, eps)
         a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
@@ -88,22 +88,20 @@ class _QkNormRope(torch.autograd.Function):
     def backward(ctx, gq, gk):
         q, k, wq, wk, pos = ctx.saved_tensors
         lib = _lib.load()
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
         if not q.numel():
             return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk), None, None, None, None
         gq, gk = _heads(gq), _heads(gk)
         D = q.shape[-1]
-        dw = torch.empty(2, D, device=q.device, dtype=torch.float32)
-        ws = torch.empty(int(lib.asr_qk_norm_rope_ws_floats(D)), device=q.device, dtype=torch.float32)
+        dwq, dwk, ws = torch.empty_like(wq), torch.empty_like(wk), wq.new_empty(lib.asr_qk_norm_rope_ws_floats(D))
         a = _rope_args(q, k, wq, wk, pos, *ctx.aux)
         a.gq, a.gk, a.q_out, a.k_out = gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr()
         a.gq_sb, a.gq_st, a.gq_sh, _ = gq.stride()
         a.gk_sb, a.gk_st, a.gk_sh, _ = gk.stride()
-        a.dwq, a.dwk, a.ws = dw[0].data_ptr(), dw[1].data_ptr(), ws.data_ptr()
+        a.dwq, a.dwk, a.ws = dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr()
         with _on(q.device):
             check(lib.asr_qk_norm_rope_bwd(C.byref(a), _stream(q.device)))
-        return dq, dk, dw[0], dw[1], None, None, None, None
+        return dq, dk, dwq, dwk, None, None, None, None
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions=None, rot_dim=None, base=10000.0, eps=1e-6):
@@ -205,7 +203,7 @@ def _attn_workspace(lib, a, backward, device):
 
 def _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, train):
     """out, and for training the row statistics and the output in float32 (out itself where it is)."""
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    out = q.new_empty(q.shape)
     if not out.numel() or not k.shape[1]:
         return out.zero_(), None, None
     lib = _lib.load()
@@ -239,7 +237,7 @@ class _BucketAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         q, k, v, table, lengths, keep, offset, lse, out32 = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+        dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
         dt = torch.empty_like(table)
         if not q.numel() or not k.shape[1]:
             return (*(t.zero_() for t in (dq, dk, dv, dt)), None, None, None, None, None, None)
@@ -327,7 +325,7 @@ def _ff_workspace(lib, a, backward, device):
 
 
 def _ff_fwd(x2, wg, wu, wd, act):
-    y = torch.empty(x2.shape[0], wd.shape[0], device=x2.device, dtype=x2.dtype)
+    y = x2.new_empty(x2.shape[0], wd.shape[0])
     if y.shape[0]:
         lib = _lib.load()
         a = _ff_args(x2, wg, wu, wd, act)

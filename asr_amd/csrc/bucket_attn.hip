@@ -59,7 +59,7 @@ struct AttnParams {
     // few queries
     float *po, *pml;
     const void *kraw, *vraw, *qraw;
-    int nsplit, vec;
+    int nsplit;
     Buckets bk;
 };
 
@@ -678,8 +678,8 @@ __global__ __launch_bounds__(256) void battn_kvsum_kernel(const float *__restric
 // the left operand as it lies) and V as whole lines for the wave's LDS image; the next 32 keys are in flight under the
 // current ones.  float32 and float16 caches are split into pieces in registers.  Bound: the cache's bytes.
 // battn_join_kernel joins the runs.
-template <int DT, int DP>
-__global__ __launch_bounds__(64) void battn_few_kernel(AttnParams p) {
+template <int DT, int DP, bool VEC>
+__global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_kernel(AttnParams p) {
     constexpr int NP = ElemOf<DT>::NP, IMG = 32 * 2 * DP, CH = DP / 8, NC = DP / 16;
     typedef typename ElemOf<DT>::type E;
     constexpr int W = (int)sizeof(E) / 2;                                              // 16-byte words of eight elements
@@ -699,7 +699,7 @@ __global__ __launch_bounds__(64) void battn_few_kernel(AttnParams p) {
     struct Raw { u32x4p w[W]; };
     auto raw8 = [&](const E *a, int d) {
         Raw r;
-        if (p.vec) {
+        if constexpr (VEC) {
 #pragma unroll
             for (int u = 0; u < W; ++u) r.w[u] = d < p.D ? reinterpret_cast<const u32x4p *>(a + d)[u] : u32x4p{0u, 0u, 0u, 0u};
         } else {
@@ -1070,14 +1070,14 @@ static int battn_fwd(const asr_bucket_attention_args *a, hipStream_t st) {
         bool vec = a->D % 8 == 0;
         for (int64_t s : {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh}) vec = vec && s % al == 0;
         for (const void *x : {a->q, a->k, a->v}) vec = vec && (uintptr_t)x % 16 == 0;
-        p.vec = vec;
         p.nsplit = battn_runs(a);
         const int64_t rows = (int64_t)p.G * p.Tq * a->B * a->Hk;
         p.po = (float *)a->ws;
         p.pml = p.po + rows * p.nsplit * a->D;
         const size_t lds = NP * 32 * 2 * DP + sizeof(float) * p.bk.nb * p.G + (2 * (p.bk.R + LUT_PAD) + 1);
-        ASR_CHECK(battn_lds(battn_few_kernel<DT, DP>, lds, "bucket_attention_fwd"));
-        hipLaunchKernelGGL((battn_few_kernel<DT, DP>), dim3(a->B * a->Hk, p.nsplit), dim3(64), lds, st, p);
+        ASR_CHECK(vec ? battn_lds(battn_few_kernel<DT, DP, true>, lds, "bucket_attention_fwd") : battn_lds(battn_few_kernel<DT, DP, false>, lds, "bucket_attention_fwd"));
+        if (vec) hipLaunchKernelGGL((battn_few_kernel<DT, DP, true>), dim3(a->B * a->Hk, p.nsplit), dim3(64), lds, st, p);
+        else hipLaunchKernelGGL((battn_few_kernel<DT, DP, false>), dim3(a->B * a->Hk, p.nsplit), dim3(64), lds, st, p);
         if (p.nsplit > 1) hipLaunchKernelGGL((battn_join_kernel<DT>), dim3((unsigned)rows), dim3(128), 0, st, p);
         ASR_CHECK_LAUNCH("battn_few_kernel");
         return ASR_OK;
