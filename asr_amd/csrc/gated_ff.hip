@@ -39,90 +39,105 @@ __device__ __forceinline__ float exp_acc(float x) {
     const float r = __builtin_amdgcn_exp2f(hi);
     return __builtin_fmaf(r, lo * 0.693147180559945309417f, r);
 }
+// FAST: for values that are rounded to bfloat16 right after, exp by one base-2 exponential (relative error 2^-24 |x|)
+template <bool FAST>
+__device__ __forceinline__ float exp_of(float x) { return FAST ? __builtin_amdgcn_exp2f(x * 1.44269504088896340736f) : exp_acc(x); }
+template <bool FAST>
 __device__ __forceinline__ void act_both(int kind, float a, float &y, float &dy) {
     if (kind == GFF_SWISH) {
-        const float s = __builtin_amdgcn_rcpf(1.f + exp_acc(-a));
+        const float s = __builtin_amdgcn_rcpf(1.f + exp_of<FAST>(-a));
         y = a * s;
         dy = s * (1.f + a * (1.f - s));
     } else {
         const float cdf = 0.5f * (1.f + erff(a * 0.70710678118654752440f));
         y = a * cdf;
-        dy = cdf + a * exp_acc(-0.5f * a * a) * 0.39894228040143267794f;
+        dy = cdf + a * exp_of<FAST>(-0.5f * a * a) * 0.39894228040143267794f;
     }
 }
 __device__ __forceinline__ float act_fwd(int kind, float a) {
     float y, dy;
-    act_both(kind, a, y, dy);
+    act_both<false>(kind, a, y, dy);
     return y;
 }
 
 // -------------------------------------------------------------------------------------------- LDS images --
-template <int NP> struct GemmK { static constexpr int BK = NP == 1 ? 64 : 32; static constexpr int NBUF = NP == 1 ? 2 : 1; };
-#define NT_PITCH(BK) (2 * (BK) + 16)                 // k-contiguous image: 16 B of padding, conflict-free ds_read_b128
-#define TN_PITCH(R) (2 * (R) + 64)                   // row-contiguous image: 64 B mod 256 B, conflict-free transposed reads
+// A workgroup of the products: pieces, depth of a k-tile, LDS images of it, register sets on their way, threads, and the waves'
+// grid WM x WN over the tile
+template <int NP_, int BK_, int NBUF_, int NSET_, int NT_, int WM_, int WN_>
+struct GemmCfg {
+    static constexpr int NP = NP_, BK = BK_, NBUF = NBUF_, NSET = NSET_, NT = NT_, WM = WM_, WN = WN_;
+};
+// Images without padding; the 16-byte chunks of a row are permuted by an exclusive or with bits of the row, so that what a
+// read instruction takes at a time falls on different banks: the same chunk of 16 rows (k-contiguous image [row][BK], read with
+// ds_read_b128), 64 B of four rows (row-contiguous image [k][R], read with the transposing ds_read_b64).  With padding in its
+// place the writes of the 64-byte rows met on the banks: 30 % of the LDS cycles of the float32 products.
+template <int BK>
+__device__ __forceinline__ int nt_at(int row, int chunk) {
+    return row * 2 * BK + ((chunk ^ (BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
+}
+template <int R>
+__device__ __forceinline__ int tn_at(int k, int chunk) { return k * 2 * R + ((chunk ^ ((k & 3) << 2)) << 4); }
 
-// fragment (row r0 + lane&31, k = 16 ks + 8 (lane>>5) ..+7) of a k-contiguous image
+// fragment (row r0 + lane&31, k = 16 ks + 8 (lane>>5) ..+7) of a k-contiguous image; r0 a multiple of 32
 template <int BK>
 __device__ __forceinline__ bf16x8 frag_nt(const unsigned char *img, int r0, int ks, int lane) {
-    const u32x4p v = *reinterpret_cast<const u32x4p *>(img + (r0 + (lane & 31)) * NT_PITCH(BK) + (ks * 2 + (lane >> 5)) * 16);
+    const u32x4p v = *reinterpret_cast<const u32x4p *>(img + r0 * 2 * BK + nt_at<BK>(lane & 31, ks * 2 + (lane >> 5)));
     return __builtin_bit_cast(bf16x8, v);
 }
 // the same of a row-contiguous image [k][R]: two transposing reads of 4 k x 16 rows per 16 lanes
 template <int R>
 __device__ __forceinline__ bf16x8 frag_tn(const unsigned char *img, int r0, int ks, int lane) {
-    const int q = (lane & 15) >> 2, p = lane & 3;
-    const unsigned char *a = img + (16 * ks + 8 * (lane >> 5) + q) * TN_PITCH(R) + (r0 + 16 * ((lane >> 4) & 1) + 4 * p) * 2;
+    const int q = (lane & 15) >> 2, p = lane & 3, ch = r0 / 8 + 2 * ((lane >> 4) & 1) + (p >> 1);
+    const unsigned char *a = img + (16 * ks + 8 * (lane >> 5)) * 2 * R + 8 * (p & 1);
     typedef __attribute__((address_space(3))) s16x4g *lds_p;
-    const s16x4g v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a));
-    const s16x4g v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 4 * TN_PITCH(R)));
+    const s16x4g v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + tn_at<R>(q, ch)));
+    const s16x4g v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + tn_at<R>(q + 4, ch)));
     const s16x8g v = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
     return __builtin_bit_cast(bf16x8, v);
 }
 
-// One operand tile of R rows x BK k: per thread R * BK / 2048 accesses of 16 bytes a piece
-template <int NP, int R>
+// One operand tile of R rows x BK k: per thread R * BK / (8 NT) accesses of 16 bytes a piece
+template <typename C, int R>
 struct NtTile {
-    static constexpr int BK = GemmK<NP>::BK, NS = R * BK / 2048, IMG = R * NT_PITCH(BK);
+    static constexpr int NP = C::NP, BK = C::BK, NS = R * BK / 8 / C::NT, IMG = R * 2 * BK;
+    static_assert(NS * 8 * C::NT == R * BK, "whole accesses");
     const __bf16 *p[NS];
     int64_t ps;
-    u32x4p v[NP][NS];
+    u32x4p v[C::NSET][NP][NS];
     // PAIR: row groups of 32 alternate between the two matrices (gate, up): group g holds columns n0 + 32 (g / 2) + ...
     template <bool PAIR>
     __device__ __forceinline__ void init(const Planes &m0, const Planes &m1, int64_t r0) {
         ps = m0.ps;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const int f = threadIdx.x + 256 * i, row = f / (BK / 8), kc = f % (BK / 8);
+            const int f = threadIdx.x + C::NT * i, row = f / (BK / 8), kc = f % (BK / 8);
             const bool second = PAIR && ((row >> 5) & 1);
             int64_t r = r0 + (PAIR ? ((row >> 6) << 5) + (row & 31) : row);
             r = r < m0.rows ? r : m0.rows - 1;
             p[i] = (second ? m1.p : m0.p) + r * m0.ld + kc * 8;
         }
     }
-    __device__ __forceinline__ void load(int k0) {
+    template <int S>
+    __device__ __forceinline__ void load_slot(int i, int64_t k0) {
 #pragma unroll
-        for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int i = 0; i < NS; ++i) v[q][i] = *reinterpret_cast<const u32x4p *>(p[i] + q * ps + k0);
+        for (int q = 0; q < NP; ++q) v[S][q][i] = *reinterpret_cast<const u32x4p *>(p[i] + q * ps + k0);
     }
-    __device__ __forceinline__ void store(unsigned char *img) const {
+    template <int S>
+    __device__ __forceinline__ void store_slot(int i, unsigned char *img) const {
+        const int f = threadIdx.x + C::NT * i;
 #pragma unroll
-        for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                const int f = threadIdx.x + 256 * i;
-                *reinterpret_cast<u32x4p *>(img + q * IMG + (f / (BK / 8)) * NT_PITCH(BK) + (f % (BK / 8)) * 16) = v[q][i];
-            }
+        for (int q = 0; q < NP; ++q) *reinterpret_cast<u32x4p *>(img + q * IMG + nt_at<BK>(f / (BK / 8), f % (BK / 8))) = v[S][q][i];
     }
 };
 // BK rows of the matrix (the product's k) x R columns; columns past ld read column 0, rows past the matrix its last row
-template <int NP, int R>
+template <typename C, int R>
 struct TnTile {
-    static constexpr int BK = GemmK<NP>::BK, NS = R * BK / 2048, IMG = BK * TN_PITCH(R);
+    static constexpr int NP = C::NP, BK = C::BK, NS = R * BK / 8 / C::NT, IMG = BK * 2 * R;
+    static_assert(NS * 8 * C::NT == R * BK, "whole accesses");
     const __bf16 *p;
     int64_t ld, ps, rows;
     int col[NS];
-    u32x4p v[NP][NS];
+    u32x4p v[C::NSET][NP][NS];
     __device__ __forceinline__ void init(const Planes &m, int64_t c0) {
         p = m.p;
         ld = m.ld;
@@ -130,35 +145,39 @@ struct TnTile {
         rows = m.rows;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const int64_t c = c0 + ((threadIdx.x + 256 * i) % (R / 8)) * 8;
+            const int64_t c = c0 + ((threadIdx.x + C::NT * i) % (R / 8)) * 8;
             col[i] = c < ld ? (int)c : 0;
         }
     }
-    __device__ __forceinline__ void load(int64_t k0) {
+    template <int S>
+    __device__ __forceinline__ void load_slot(int i, int64_t k0) {
+        int64_t r = k0 + (threadIdx.x + C::NT * i) / (R / 8);
+        r = r < rows ? r : rows - 1;
+        const __bf16 *a = p + r * ld + col[i];
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            int64_t r = k0 + (threadIdx.x + 256 * i) / (R / 8);
-            r = r < rows ? r : rows - 1;
-            const __bf16 *a = p + r * ld + col[i];
-#pragma unroll
-            for (int q = 0; q < NP; ++q) v[q][i] = *reinterpret_cast<const u32x4p *>(a + q * ps);
-        }
+        for (int q = 0; q < NP; ++q) v[S][q][i] = *reinterpret_cast<const u32x4p *>(a + q * ps);
     }
-    __device__ __forceinline__ void store(unsigned char *img) const {
+    template <int S>
+    __device__ __forceinline__ void store_slot(int i, unsigned char *img) const {
+        const int f = threadIdx.x + C::NT * i;
 #pragma unroll
-        for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                const int f = threadIdx.x + 256 * i;
-                *reinterpret_cast<u32x4p *>(img + q * IMG + (f / (R / 8)) * TN_PITCH(R) + (f % (R / 8)) * 16) = v[q][i];
-            }
+        for (int q = 0; q < NP; ++q) *reinterpret_cast<u32x4p *>(img + q * IMG + tn_at<R>(f / (R / 8), f % (R / 8))) = v[S][q][i];
     }
 };
+template <int S, typename T>
+__device__ __forceinline__ void load_all(T &t, int64_t k0) {
+#pragma unroll
+    for (int i = 0; i < T::NS; ++i) t.template load_slot<S>(i, k0);
+}
+template <int S, typename T>
+__device__ __forceinline__ void store_all(const T &t, unsigned char *img) {
+#pragma unroll
+    for (int i = 0; i < T::NS; ++i) t.template store_slot<S>(i, img);
+}
 
-// acc += A B over one k-tile; FRAG(operand, piece, tile, ks) delivers fragments.  Smallest pieces first.
-template <int NP, int TM, int TN, typename FA, typename FB>
+// acc += A B over one k-tile; fa / fb (piece, tile, ks) deliver fragments.  Smallest pieces first.
+template <int NP, int KS, int TM, int TN, typename FA, typename FB>
 __device__ __forceinline__ void mma_tile(f32x16 (&acc)[TM][TN], FA fa, FB fb) {
-    constexpr int KS = GemmK<NP>::BK / 16;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
         bf16x8 a[NP][TM], b[NP][TN];
@@ -182,34 +201,84 @@ __device__ __forceinline__ void mma_tile(f32x16 (&acc)[TM][TN], FA fa, FB fb) {
 }
 
 // The main loop: k-tiles [kt0, kt1) of A (TA rows) times B (TB rows); leaves the LDS free to use (ends with a barrier).
-template <int NP, int TM, int TN, typename TA, typename TB, typename FA, typename FB>
+// Past the end the last tile is loaded again: its reads stay in bounds and nothing uses them.
+// One image: a tile's loads run under the previous tile's products.  Two images and two register sets: while a tile is
+// multiplied the next one goes from its registers to the other image and the one after it is loaded, slot by slot between the
+// matrix instructions, as are the fragments of the next 16 k: one barrier a tile, and nothing waits in front of it.
+template <int N> struct IntC { static constexpr int value = N; };
+template <typename C, int TM, int TN, typename TA, typename TB, typename FA, typename FB>
 __device__ __forceinline__ void main_loop(f32x16 (&acc)[TM][TN], TA &ta, TB &tb, unsigned char *lds, int64_t kt0, int64_t kt1,
                                           FA frag_a, FB frag_b) {
-    constexpr int BK = GemmK<NP>::BK, NBUF = GemmK<NP>::NBUF, IA = NP * TA::IMG, IB = NP * TB::IMG;
+    constexpr int NP = C::NP, IA = NP * TA::IMG, IB = NP * TB::IMG;
     if (kt0 >= kt1) return;
-    ta.load(kt0 * BK);
-    tb.load(kt0 * BK);
-    ta.store(lds);
-    tb.store(lds + IA);
-    __syncthreads();
-    int buf = 0;
-    for (int64_t kt = kt0; kt < kt1; ++kt) {
-        const bool more = kt + 1 < kt1;
-        if (more) {
-            ta.load((kt + 1) * BK);
-            tb.load((kt + 1) * BK);
+    load_all<0>(ta, kt0 * C::BK);
+    load_all<0>(tb, kt0 * C::BK);
+    if constexpr (C::NBUF == 1) {
+        for (int64_t kt = kt0; kt < kt1; ++kt) {
+            store_all<0>(ta, lds);
+            store_all<0>(tb, lds + IA);
+            __syncthreads();
+            if (kt + 1 < kt1) {
+                load_all<0>(ta, (kt + 1) * C::BK);
+                load_all<0>(tb, (kt + 1) * C::BK);
+            }
+            mma_tile<NP, C::BK / 16, TM, TN>(acc, [&](int q, int i, int ks) { return frag_a(lds + q * TA::IMG, i, ks); },
+                                             [&](int q, int j, int ks) { return frag_b(lds + IA + q * TB::IMG, j, ks); });
+            __syncthreads();
         }
-        unsigned char *img = lds + (NBUF == 2 ? buf * (IA + IB) : 0);
-        mma_tile<NP, TM, TN>(acc, [&](int q, int i, int ks) { return frag_a(img + q * TA::IMG, i, ks); },
-                             [&](int q, int j, int ks) { return frag_b(img + IA + q * TB::IMG, j, ks); });
-        if (NBUF == 1) __syncthreads();
-        if (more) {
-            buf ^= 1;
-            unsigned char *nxt = lds + (NBUF == 2 ? buf * (IA + IB) : 0);
-            ta.store(nxt);
-            tb.store(nxt + IA);
-        }
+    } else {
+        constexpr int KS = C::BK / 16, NM = TM * TN, NCH = KS * NM, NF = TM + TN, NSL = TA::NS + TB::NS;
+        auto k_of = [&](int64_t kt) { return (kt < kt1 ? kt : kt1 - 1) * C::BK; };
+        auto body = [&](auto tag, int64_t kt) {
+            constexpr int P = decltype(tag)::value;
+            const unsigned char *img = lds + P * (IA + IB);
+            unsigned char *nxt = lds + (P ^ 1) * (IA + IB);
+            const int64_t k2 = k_of(kt + 2);
+            bf16x8 a[2][NP][TM], b[2][NP][TN];
+            auto frag = [&](int s, int ks, int f) {
+#pragma unroll
+                for (int q = 0; q < NP; ++q) {
+                    if (f < TM) a[s][q][f] = frag_a(img + q * TA::IMG, f, ks);
+                    else b[s][q][f - TM] = frag_b(img + IA + q * TB::IMG, f - TM, ks);
+                }
+            };
+#pragma unroll
+            for (int f = 0; f < NF; ++f) frag(0, 0, f);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const int ks = c / NM, m = c % NM, i = m / TN, j = m % TN;
+                if (ks + 1 < KS) {
+#pragma unroll
+                    for (int f = m * NF / NM; f < (m + 1) * NF / NM; ++f) frag((ks + 1) & 1, ks + 1, f);
+                }
+#pragma unroll
+                for (int s = NP - 1; s >= 0; --s)
+#pragma unroll
+                    for (int q = s; q >= 0; --q)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks & 1][q][i], b[ks & 1][s - q][j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int sl = c * NSL / NCH; sl < (c + 1) * NSL / NCH; ++sl) {
+                    if (sl < TA::NS) {
+                        ta.template store_slot<P ^ 1>(sl, nxt);
+                        ta.template load_slot<P>(sl, k2);
+                    } else {
+                        tb.template store_slot<P ^ 1>(sl - TA::NS, nxt + IA);
+                        tb.template load_slot<P>(sl - TA::NS, k2);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __syncthreads();
+        };
+        load_all<1>(ta, k_of(kt0 + 1));
+        load_all<1>(tb, k_of(kt0 + 1));
+        store_all<0>(ta, lds);
+        store_all<0>(tb, lds + IA);
         __syncthreads();
+        for (int64_t kt = kt0; kt < kt1; kt += 2) {
+            body(IntC<0>{}, kt);
+            if (kt + 1 < kt1) body(IntC<1>{}, kt + 1);
+        }
     }
 }
 
@@ -273,67 +342,80 @@ struct GateParams {
     Planes dy, wdt;                      // backward: dy (M, np), Wd^T (f, np)
     __bf16 *h, *dab;                     // (Mp, fp) and (Mp, 2 fp) in pieces
     int64_t h_ps, dab_ps;
-    int64_t M, fp;
-    int f, ktx, kty, ncol, ntiles, act;
+    int64_t M, Mp, fp;
+    int f, dp, np, ncol, ntiles, act;
 };
 
-template <int NP, bool BWD>
-__global__ __launch_bounds__(256, 2) void gff_gate_kernel(GateParams p) {
-    constexpr int BM = 128, BN = 64;
-    typedef NtTile<NP, BM> TA;
-    typedef NtTile<NP, 128> TB;
-    typedef NtTile<NP, BN> TD;
-    constexpr int POOL = GemmK<NP>::NBUF * NP * (TA::IMG + TB::IMG);
-    __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > 16384 ? POOL : 16384];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+// BM rows x BN columns of h: A tile of BM rows, B tile of 2 BN (gate and up rows interleaved), then of BN rows of Wd^T
+template <typename C, int BM, int BN, bool BWD>
+__global__ __launch_bounds__(C::NT, 2) void gff_gate_kernel(GateParams p) {
+    constexpr int NP = C::NP, TM = BM / C::WM / 32, RM = BM / C::WM;
+    static_assert(BN / C::WN == 32, "a wave has the gate and the up values of 32 columns");
+    typedef NtTile<C, BM> TA;
+    typedef NtTile<C, 2 * BN> TB;
+    typedef NtTile<C, BN> TD;
+    constexpr int POOL = C::NBUF * NP * (TA::IMG + TB::IMG), TURN = C::NT / 64 * 4096;
+    __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > TURN ? POOL : TURN];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WN, wn = wave % C::WN;
     int tm, tn;
     tile_of(blockIdx.x, p.ntiles, p.ncol, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-    f32x16 ab[2][2];
+    f32x16 ab[TM][2];
     zero_acc(ab);
     {
         TA ta;
         TB tb;
         ta.template init<false>(p.x, p.x, m0);
         tb.template init<true>(p.wg, p.wu, n0);
-        main_loop<NP>(ab, ta, tb, pool, 0, p.ktx,
-                      [&](const unsigned char *img, int i, int ks) { return frag_nt<TA::BK>(img, wm * 64 + i * 32, ks, lane); },
-                      [&](const unsigned char *img, int j, int ks) { return frag_nt<TA::BK>(img, wn * 64 + j * 32, ks, lane); });
+        main_loop<C>(ab, ta, tb, pool, 0, p.dp / C::BK,
+                     [&](const unsigned char *img, int i, int ks) { return frag_nt<C::BK>(img, wm * RM + i * 32, ks, lane); },
+                     [&](const unsigned char *img, int j, int ks) { return frag_nt<C::BK>(img, wn * 64 + j * 32, ks, lane); });
     }
-    f32x16 dh[2][1];
+    f32x16 dh[TM][1];
     if (BWD) {
         zero_acc(dh);
         TA ta;
         TD tb;
         ta.template init<false>(p.dy, p.dy, m0);
         tb.template init<false>(p.wdt, p.wdt, n0);
-        main_loop<NP>(dh, ta, tb, pool, 0, p.kty,
-                      [&](const unsigned char *img, int i, int ks) { return frag_nt<TA::BK>(img, wm * 64 + i * 32, ks, lane); },
-                      [&](const unsigned char *img, int j, int ks) { return frag_nt<TA::BK>(img, wn * 32 + j * 32, ks, lane); });
+        main_loop<C>(dh, ta, tb, pool, 0, p.np / C::BK,
+                     [&](const unsigned char *img, int i, int ks) { return frag_nt<C::BK>(img, wm * RM + i * 32, ks, lane); },
+                     [&](const unsigned char *img, int j, int ks) { return frag_nt<C::BK>(img, wn * 32 + j * 32, ks, lane); });
     }
     float *S = reinterpret_cast<float *>(pool) + wave * 1024;
     const int64_t cb = n0 + wn * 32;
-    const bool col_ok = cb + (lane & 31) < p.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t rb = m0 + wm * 64 + i * 32;
+    for (int i = 0; i < TM; ++i) {
+        const int64_t rb = m0 + wm * RM + i * 32;
+        if (rb >= p.Mp) break;                                                     // a tile may reach past the padded rows
         f32x16 hh, da, db;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const bool ok = col_ok && rb + ((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) < p.M;
-            const float a = ab[i][0][r], b = ab[i][1][r];
             float y, dy;
-            act_both(p.act, a, y, dy);
-            hh[r] = ok ? y * b : 0.f;
+            act_both<NP == 1>(p.act, ab[i][0][r], y, dy);
+            hh[r] = y * ab[i][1][r];
             if (BWD) {
-                da[r] = ok ? dh[i][0][r] * b * dy : 0.f;
-                db[r] = ok ? dh[i][0][r] * y : 0.f;
+                da[r] = dh[i][0][r] * ab[i][1][r] * dy;
+                db[r] = dh[i][0][r] * y;
             }
         }
-        turn_tile(hh, S, [&](int r, int c, float4 v) { put_pieces<NP>(p.h + (rb + r) * p.fp + cb + c, p.h_ps, v); });
+        if (cb + 32 > p.f || rb + 32 > p.M) {                                      // what lies past the matrix is stored as zeros
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool ok = cb + (lane & 31) < p.f && rb + ((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) < p.M;
+                hh[r] = ok ? hh[r] : 0.f;
+                if (BWD) {
+                    da[r] = ok ? da[r] : 0.f;
+                    db[r] = ok ? db[r] : 0.f;
+                }
+            }
+        }
+        __bf16 *h = p.h + rb * p.fp + cb, *d = BWD ? p.dab + rb * 2 * p.fp + cb : nullptr;
+        const int fp = (int)p.fp;
+        turn_tile(hh, S, [&](int r, int c, float4 v) { put_pieces<NP>(h + (r * fp + c), p.h_ps, v); });
         if (BWD) {
-            turn_tile(da, S, [&](int r, int c, float4 v) { put_pieces<NP>(p.dab + (rb + r) * 2 * p.fp + cb + c, p.dab_ps, v); });
-            turn_tile(db, S, [&](int r, int c, float4 v) { put_pieces<NP>(p.dab + (rb + r) * 2 * p.fp + p.fp + cb + c, p.dab_ps, v); });
+            turn_tile(da, S, [&](int r, int c, float4 v) { put_pieces<NP>(d + (r * 2 * fp + c), p.dab_ps, v); });
+            turn_tile(db, S, [&](int r, int c, float4 v) { put_pieces<NP>(d + (r * 2 * fp + fp + c), p.dab_ps, v); });
         }
     }
 }
@@ -342,18 +424,18 @@ __global__ __launch_bounds__(256, 2) void gff_gate_kernel(GateParams p) {
 struct NtParams {
     Planes a, b;
     void *c;
-    int64_t ldc, M, N;
-    int kt, ncol, ntiles, vec;
+    int64_t ldc, M, N, K;
+    int ncol, ntiles, vec;
 };
-template <int DT, int BM, int BN>
-__global__ __launch_bounds__(256, 2) void gff_nt_kernel(NtParams p) {
-    constexpr int NP = ElemOf<DT>::NP, TM = BM / 64, TN = BN / 64;
+template <int DT, typename C, int BM, int BN>
+__global__ __launch_bounds__(C::NT, 2) void gff_nt_kernel(NtParams p) {
+    constexpr int NP = C::NP, RM = BM / C::WM, RN = BN / C::WN, TM = RM / 32, TN = RN / 32;
     typedef typename ElemOf<DT>::type E;
-    typedef NtTile<NP, BM> TA;
-    typedef NtTile<NP, BN> TB;
-    constexpr int POOL = GemmK<NP>::NBUF * NP * (TA::IMG + TB::IMG);
-    __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > 16384 ? POOL : 16384];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+    typedef NtTile<C, BM> TA;
+    typedef NtTile<C, BN> TB;
+    constexpr int POOL = C::NBUF * NP * (TA::IMG + TB::IMG), TURN = C::NT / 64 * 4096;
+    __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > TURN ? POOL : TURN];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WN, wn = wave % C::WN;
     int tm, tn;
     tile_of(blockIdx.x, p.ntiles, p.ncol, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
@@ -363,15 +445,15 @@ __global__ __launch_bounds__(256, 2) void gff_nt_kernel(NtParams p) {
     TB tb;
     ta.template init<false>(p.a, p.a, m0);
     tb.template init<false>(p.b, p.b, n0);
-    main_loop<NP>(acc, ta, tb, pool, 0, p.kt,
-                  [&](const unsigned char *img, int i, int ks) { return frag_nt<TA::BK>(img, wm * (BM / 2) + i * 32, ks, lane); },
-                  [&](const unsigned char *img, int j, int ks) { return frag_nt<TA::BK>(img, wn * (BN / 2) + j * 32, ks, lane); });
+    main_loop<C>(acc, ta, tb, pool, 0, p.K / C::BK,
+                 [&](const unsigned char *img, int i, int ks) { return frag_nt<C::BK>(img, wm * RM + i * 32, ks, lane); },
+                 [&](const unsigned char *img, int j, int ks) { return frag_nt<C::BK>(img, wn * RN + j * 32, ks, lane); });
     float *S = reinterpret_cast<float *>(pool) + wave * 1024;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            const int64_t rb = m0 + wm * (BM / 2) + i * 32, cb = n0 + wn * (BN / 2) + j * 32;
+            const int64_t rb = m0 + wm * RM + i * 32, cb = n0 + wn * RN + j * 32;
             turn_tile(acc[i][j], S, [&](int r, int c, float4 v) {
                 if (rb + r < p.M) put_row4<E>((E *)p.c + (rb + r) * p.ldc, cb + c, p.N, p.vec, v);
             });
@@ -390,34 +472,34 @@ struct TnParams {
     int64_t kt, kt_split;
     int ncol, ntiles, vec;
 };
-template <int DT>
-__global__ __launch_bounds__(256, 2) void gff_tn_kernel(TnParams p) {
-    constexpr int NP = ElemOf<DT>::NP, BM = 128, BN = 128;
+template <int DT, typename C, int BM, int BN>
+__global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnParams p) {
+    constexpr int NP = C::NP, RM = BM / C::WM, RN = BN / C::WN, TM = RM / 32, TN = RN / 32;
     typedef typename ElemOf<DT>::type E;
-    typedef TnTile<NP, BM> TA;
-    typedef TnTile<NP, BN> TB;
-    constexpr int POOL = GemmK<NP>::NBUF * NP * (TA::IMG + TB::IMG);
-    __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > 16384 ? POOL : 16384];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+    typedef TnTile<C, BM> TA;
+    typedef TnTile<C, BN> TB;
+    constexpr int POOL = C::NBUF * NP * (TA::IMG + TB::IMG), TURN = C::NT / 64 * 4096;
+    __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > TURN ? POOL : TURN];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WN, wn = wave % C::WN;
     int tm, tn;
     tile_of(blockIdx.x, p.ntiles, p.ncol, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-    f32x16 acc[2][2];
+    f32x16 acc[TM][TN];
     zero_acc(acc);
     TA ta;
     TB tb;
     ta.init(p.a, m0);
     tb.init(p.b, n0);
     const int64_t k0 = blockIdx.y * p.kt_split;
-    main_loop<NP>(acc, ta, tb, pool, k0, min(p.kt, k0 + p.kt_split),
-                  [&](const unsigned char *img, int i, int ks) { return frag_tn<BM>(img, wm * 64 + i * 32, ks, lane); },
-                  [&](const unsigned char *img, int j, int ks) { return frag_tn<BN>(img, wn * 64 + j * 32, ks, lane); });
+    main_loop<C>(acc, ta, tb, pool, k0, min(p.kt, k0 + p.kt_split),
+                 [&](const unsigned char *img, int i, int ks) { return frag_tn<BM>(img, wm * RM + i * 32, ks, lane); },
+                 [&](const unsigned char *img, int j, int ks) { return frag_tn<BN>(img, wn * RN + j * 32, ks, lane); });
     float *S = reinterpret_cast<float *>(pool) + wave * 1024;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int64_t rb = m0 + wm * 64 + i * 32, cb = n0 + wn * 64 + j * 32;
+        for (int j = 0; j < TN; ++j) {
+            const int64_t rb = m0 + wm * RM + i * 32, cb = n0 + wn * RN + j * 32;
             turn_tile(acc[i][j], S, [&](int r, int c, float4 v) {
                 int64_t row = rb + r;
                 const bool second = row >= p.half;
@@ -611,24 +693,33 @@ __global__ __launch_bounds__(512) void gff_few_down_kernel(const float *h, const
 // ------------------------------------------------------------------------------------------------------- host --
 static int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
+// A weight gradient (rows x cols, summed over M): the tile, and in how many runs of M it is summed.  A run has at least 8
+// k-tiles, and there are runs until the launch has two workgroups of four waves (or one of eight) for each compute unit.
+struct TnPlan { int big, splits; };
+static TnPlan gff_tn_plan(int NP, int64_t rows, int64_t cols, int64_t M) {
+    const int64_t kt = cdiv(M, NP == 1 ? 64 : 32);
+    auto runs = [&](int64_t tiles, int64_t want) {
+        int64_t s = want / (tiles > 0 ? tiles : 1);
+        if (s > kt / 8) s = kt / 8;
+        if (s > 32) s = 32;
+        return s < 1 ? 1 : (int)s;
+    };
+    const int64_t mid = (int64_t)cdiv(rows, 256) * cdiv(cols, 128), small = (int64_t)cdiv(rows, 128) * cdiv(cols, 128);
+    const int sm = runs(mid, 256);
+    if (NP == 1 && mid * sm >= 192) return TnPlan{1, sm};
+    return TnPlan{0, runs(small, 512)};
+}
+
 struct GffPlan {
     int NP;
     int64_t dp, np, fp, Mp;              // padded widths of x / dy / h and rows of h, [da db]
     bool direct_x, direct_wgu, direct_wd, direct_dy;
-    int splits_gu, splits_d;
+    TnPlan gu, wd;                       // the weight gradients of [gate; up] and down
     int64_t off[16], bytes;              // workspace: byte offsets
 };
 enum { O_X, O_WG, O_WU, O_WD, O_H, O_DY, O_WDT, O_WGUT, O_DAB, O_PART };
 
 static bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
-
-// Splits of the weight gradients' sum over M: enough workgroups for two a compute unit, each with at least 8 k-tiles
-static int gff_splits(int64_t tiles, int64_t kt) {
-    int64_t s = 512 / (tiles > 0 ? tiles : 1);
-    if (s > kt / 8) s = kt / 8;
-    if (s > 32) s = 32;
-    return s < 1 ? 1 : (int)s;
-}
 
 // A bfloat16 matrix whose k is whole k-tiles is an operand as it lies; every other one is packed into the workspace.
 static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
@@ -658,12 +749,11 @@ static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
         take(O_WDT, (int64_t)a->f * p.np * e);
         take(O_WGUT, (int64_t)a->d * 2 * p.fp * e);
         take(O_DAB, p.Mp * 2 * p.fp * e);
-        const int64_t bk = one ? 64 : 32, kt = (a->M + bk - 1) / bk;
-        p.splits_gu = gff_splits((int64_t)cdiv(2 * p.fp, 128) * cdiv(a->d, 128), kt);
-        p.splits_d = gff_splits((int64_t)cdiv(a->n, 128) * cdiv(a->f, 128), kt);
+        p.gu = gff_tn_plan(p.NP, 2 * p.fp, a->d, a->M);
+        p.wd = gff_tn_plan(p.NP, a->n, a->f, a->M);
         int64_t part = 0;
-        if (p.splits_gu > 1) part = (int64_t)p.splits_gu * 2 * a->f * a->d;
-        if (p.splits_d > 1 && (int64_t)p.splits_d * a->n * a->f > part) part = (int64_t)p.splits_d * a->n * a->f;
+        if (p.gu.splits > 1) part = (int64_t)p.gu.splits * 2 * a->f * a->d;
+        if (p.wd.splits > 1 && (int64_t)p.wd.splits * a->n * a->f > part) part = (int64_t)p.wd.splits * a->n * a->f;
         take(O_PART, part * 4);
     }
     p.bytes = o;
@@ -709,33 +799,77 @@ static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, i
     blocks += k.nx * cdiv(trans ? wide : R, 64);
 }
 
-template <int DT>
-static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t N, int64_t K, hipStream_t st) {
-    constexpr int NP = ElemOf<DT>::NP;
-    NtParams p{a, b, c, N, M, N, (int)(K / GemmK<NP>::BK), 0, 0, (int)(N % 4 == 0 && aligned16(c))};
-    // narrower tiles where 128 x 128 would leave compute units without one
-    if ((int64_t)cdiv(M, 128) * cdiv(N, 128) >= 256) {
-        p.ncol = cdiv(N, 128);
-        p.ntiles = cdiv(M, 128) * p.ncol;
-        hipLaunchKernelGGL((gff_nt_kernel<DT, 128, 128>), dim3(p.ntiles), dim3(256), 0, st, p);
-    } else {
-        p.ncol = cdiv(N, 64);
-        p.ntiles = cdiv(M, 64) * p.ncol;
-        hipLaunchKernelGGL((gff_nt_kernel<DT, 64, 64>), dim3(p.ntiles), dim3(256), 0, st, p);
-    }
+// Workgroups of the products.  One piece: eight waves, 256 x 256 or 256 x 128 (a wave's 128 x 64 or 64 x 64): with four waves
+// and 128 x 128 the LDS was the bound, its writes and reads as long as the matrix work (8192 x 1024 x 4096 bfloat16: 133 us
+// a product, 75 without loads and LDS writes).  Several pieces: three to six products an LDS byte, 128 x 128 with four waves.
+// Smaller tiles where larger ones would leave compute units without one.
+typedef GemmCfg<1, 64, 2, 2, 512, 2, 4> CfgBig;             // 256 x 256
+typedef GemmCfg<1, 64, 2, 2, 512, 4, 2> CfgMid;             // 256 x 128
+template <int NP> struct CfgSmall { typedef GemmCfg<NP, NP == 1 ? 64 : 32, NP == 1 ? 2 : 1, NP == 1 ? 2 : 1, 256, 2, 2> T; };
+template <int NP> struct CfgDeep { typedef GemmCfg<NP, 64, 1, 1, 256, 2, 2> T; };
+
+template <int DT, typename C, int BM, int BN>
+static int gff_nt_go(NtParams &p, hipStream_t st) {
+    p.ncol = cdiv(p.N, BN);
+    p.ntiles = cdiv(p.M, BM) * p.ncol;
+    hipLaunchKernelGGL((gff_nt_kernel<DT, C, BM, BN>), dim3(p.ntiles), dim3(C::NT), 0, st, p);
     ASR_CHECK_LAUNCH("gff_nt_kernel");
     return ASR_OK;
 }
+template <int DT>
+static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t N, int64_t K, hipStream_t st) {
+    constexpr int NP = ElemOf<DT>::NP;
+    NtParams p{a, b, c, N, M, N, K, 0, 0, (int)(N % 4 == 0 && aligned16(c))};
+    auto tiles = [&](int bm, int bn) { return (int64_t)cdiv(M, bm) * cdiv(N, bn); };
+    if constexpr (NP == 1) {
+        if (tiles(256, 256) >= 256) return gff_nt_go<DT, CfgBig, 256, 256>(p, st);
+        if (tiles(256, 128) >= 192) return gff_nt_go<DT, CfgMid, 256, 128>(p, st);
+    }
+    if (tiles(128, 128) >= 256) return gff_nt_go<DT, typename CfgSmall<NP>::T, 128, 128>(p, st);
+    if (tiles(128, 64) >= 192) return gff_nt_go<DT, typename CfgDeep<NP>::T, 128, 64>(p, st);
+    return gff_nt_go<DT, typename CfgDeep<NP>::T, 64, 64>(p, st);
+}
 
+template <typename C, int BM, int BN, bool BWD>
+static int gff_gate_go(GateParams &g, hipStream_t st) {
+    g.ncol = cdiv(g.fp, BN);
+    g.ntiles = cdiv(g.Mp, BM) * g.ncol;
+    hipLaunchKernelGGL((gff_gate_kernel<C, BM, BN, BWD>), dim3(g.ntiles), dim3(C::NT), 0, st, g);
+    ASR_CHECK_LAUNCH("gff_gate_kernel");
+    return ASR_OK;
+}
+template <int DT, bool BWD>
+static int gff_gate(GateParams &g, hipStream_t st) {
+    constexpr int NP = ElemOf<DT>::NP;
+    if constexpr (NP == 1) {
+        // backward: a third accumulator leaves room for 128 rows
+        constexpr int BM = BWD ? 128 : 256;
+        if (g.fp % 128 == 0 && (int64_t)cdiv(g.Mp, BM) * (g.fp / 128) >= 256) return gff_gate_go<CfgBig, BM, 128, BWD>(g, st);
+    }
+    return gff_gate_go<typename CfgSmall<NP>::T, 128, 64, BWD>(g, st);
+}
+
+template <int DT, typename C, int BM, int BN>
+static void gff_tn_go(TnParams &p, int64_t rows, int64_t M, int splits, hipStream_t st) {
+    p.ncol = cdiv(p.N, BN);
+    p.ntiles = cdiv(rows, BM) * p.ncol;
+    p.kt = cdiv(M, C::BK);
+    p.kt_split = (p.kt + splits - 1) / splits;
+    hipLaunchKernelGGL((gff_tn_kernel<DT, C, BM, BN>), dim3(p.ntiles, splits), dim3(C::NT), 0, st, p);
+}
 template <int DT>
 static int gff_tn(const Planes &a, const Planes &b, void *c0, void *c1, int64_t rows, int64_t half, int64_t valid, int64_t N, int64_t M,
-                  int splits, float *part, hipStream_t st) {
+                  const TnPlan &pl, float *part, hipStream_t st) {
     constexpr int NP = ElemOf<DT>::NP;
-    TnParams p{a, b, c0, c1, splits > 1 ? part : nullptr, half, valid, N, (c1 ? 2 : 1) * valid * N, cdiv(M, GemmK<NP>::BK), 0, cdiv(N, 128), 0,
+    const int splits = pl.splits;
+    TnParams p{a, b, c0, c1, splits > 1 ? part : nullptr, half, valid, N, (c1 ? 2 : 1) * valid * N, 0, 0, 0, 0,
                (int)(N % 4 == 0 && aligned16(c0) && aligned16(c1))};
-    p.ntiles = cdiv(rows, 128) * p.ncol;
-    p.kt_split = (p.kt + splits - 1) / splits;
-    hipLaunchKernelGGL((gff_tn_kernel<DT>), dim3(p.ntiles, splits), dim3(256), 0, st, p);
+    if constexpr (NP == 1) {
+        if (pl.big) gff_tn_go<DT, CfgMid, 256, 128>(p, rows, M, splits, st);
+        else gff_tn_go<DT, typename CfgSmall<NP>::T, 128, 128>(p, rows, M, splits, st);
+    } else {
+        gff_tn_go<DT, typename CfgSmall<NP>::T, 128, 128>(p, rows, M, splits, st);
+    }
     ASR_CHECK_LAUNCH("gff_tn_kernel");
     if (splits > 1) {
         const int64_t n0 = valid * N;
@@ -752,7 +886,6 @@ static int gff_tn(const Planes &a, const Planes &b, void *c0, void *c1, int64_t 
 
 template <int DT>
 static int gff_run(const asr_gated_ff_args *a, bool bwd, hipStream_t st) {
-    constexpr int NP = ElemOf<DT>::NP, BK = GemmK<NP>::BK;
     GffPlan p;
     gff_plan(a, bwd, p);
     char *ws = (char *)a->ws;
@@ -787,20 +920,16 @@ static int gff_run(const asr_gated_ff_args *a, bool bwd, hipStream_t st) {
         hipLaunchKernelGGL((gff_pack_kernel<DT>), dim3((unsigned)blocks), dim3(256), 0, st, jobs);
         ASR_CHECK_LAUNCH("gff_pack_kernel");
     }
-    GateParams g{x, wg, wu, dy, wdt, (__bf16 *)h.p, (__bf16 *)dab.p, h.ps, dab.ps, a->M, p.fp, a->f, (int)(p.dp / BK), (int)(p.np / BK),
-                 (int)(p.fp / 64), 0, a->act};
-    g.ntiles = (int)(p.Mp / 128) * g.ncol;
+    GateParams g{x, wg, wu, dy, wdt, (__bf16 *)h.p, (__bf16 *)dab.p, h.ps, dab.ps, a->M, p.Mp, p.fp, a->f, (int)p.dp, (int)p.np, 0, 0, a->act};
     if (!bwd) {
-        hipLaunchKernelGGL((gff_gate_kernel<NP, false>), dim3(g.ntiles), dim3(256), 0, st, g);
-        ASR_CHECK_LAUNCH("gff_gate_kernel");
+        ASR_CHECK((gff_gate<DT, false>(g, st)));
         return gff_nt<DT>(h, wd, a->y, a->M, a->n, p.fp, st);
     }
-    hipLaunchKernelGGL((gff_gate_kernel<NP, true>), dim3(g.ntiles), dim3(256), 0, st, g);
-    ASR_CHECK_LAUNCH("gff_gate_kernel");
+    ASR_CHECK((gff_gate<DT, true>(g, st)));
     if (a->dx) ASR_CHECK(gff_nt<DT>(dab, wgut, a->dx, a->M, a->d, 2 * p.fp, st));
     float *part = (float *)at(O_PART);
-    if (a->dwg) ASR_CHECK(gff_tn<DT>(dab, x, a->dwg, a->dwu, 2 * p.fp, p.fp, a->f, a->d, a->M, p.splits_gu, part, st));
-    if (a->dwd) ASR_CHECK(gff_tn<DT>(dy, h, a->dwd, nullptr, a->n, up_to(a->n, 128), a->n, a->f, a->M, p.splits_d, part, st));
+    if (a->dwg) ASR_CHECK(gff_tn<DT>(dab, x, a->dwg, a->dwu, 2 * p.fp, p.fp, a->f, a->d, a->M, p.gu, part, st));
+    if (a->dwd) ASR_CHECK(gff_tn<DT>(dy, h, a->dwd, nullptr, a->n, up_to(a->n, 256), a->n, a->f, a->M, p.wd, part, st));
     return ASR_OK;
 }
 
