@@ -99,8 +99,7 @@ __device__ __forceinline__ bf16x8 frag_tn(const unsigned char *img, int r0, int 
 // One operand tile of R rows x BK k: per thread R * BK / (8 NT) accesses of 16 bytes a piece
 template <typename C, int R>
 struct NtTile {
-    static constexpr int NP = C::NP, BK = C::BK, NS = R * BK / 8 / C::NT, IMG = R * 2 * BK;
-    static_assert(NS * 8 * C::NT == R * BK, "whole accesses");
+    static constexpr int NP = C::NP, BK = C::BK, TOT = R * BK / 8, NS = (TOT + C::NT - 1) / C::NT, IMG = R * 2 * BK;
     const __bf16 *p[NS];
     int64_t ps;
     u32x4p v[C::NSET][NP][NS];
@@ -110,7 +109,7 @@ struct NtTile {
         ps = m0.ps;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const int f = threadIdx.x + C::NT * i, row = f / (BK / 8), kc = f % (BK / 8);
+            const int f = min((int)threadIdx.x + C::NT * i, TOT - 1), row = f / (BK / 8), kc = f % (BK / 8);
             const bool second = PAIR && ((row >> 5) & 1);
             int64_t r = r0 + (PAIR ? ((row >> 6) << 5) + (row & 31) : row);
             r = r < m0.rows ? r : m0.rows - 1;
@@ -125,6 +124,7 @@ struct NtTile {
     template <int S>
     __device__ __forceinline__ void store_slot(int i, unsigned char *img) const {
         const int f = threadIdx.x + C::NT * i;
+        if (TOT % C::NT != 0 && f >= TOT) return;
 #pragma unroll
         for (int q = 0; q < NP; ++q) *reinterpret_cast<u32x4p *>(img + q * IMG + nt_at<BK>(f / (BK / 8), f % (BK / 8))) = v[S][q][i];
     }
@@ -234,7 +234,9 @@ __device__ __forceinline__ void main_loop(f32x16 (&acc)[TM][TN], TA &ta, TB &tb,
             const unsigned char *img = lds + P * (IA + IB);
             unsigned char *nxt = lds + (P ^ 1) * (IA + IB);
             const int64_t k2 = k_of(kt + 2);
-            bf16x8 a[2][NP][TM], b[2][NP][TN];
+            // (several pieces: the fragments of 16 k already fill the registers, and last for three to six times the products)
+            constexpr int NFB = NP == 1 ? 2 : 1;
+            bf16x8 a[NFB][NP][TM], b[NFB][NP][TN];
             auto frag = [&](int s, int ks, int f) {
 #pragma unroll
                 for (int q = 0; q < NP; ++q) {
@@ -247,15 +249,19 @@ __device__ __forceinline__ void main_loop(f32x16 (&acc)[TM][TN], TA &ta, TB &tb,
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
                 const int ks = c / NM, m = c % NM, i = m / TN, j = m % TN;
-                if (ks + 1 < KS) {
+                if (NFB == 2 && ks + 1 < KS) {
 #pragma unroll
                     for (int f = m * NF / NM; f < (m + 1) * NF / NM; ++f) frag((ks + 1) & 1, ks + 1, f);
+                }
+                if (NFB == 1 && ks > 0 && m == 0) {
+#pragma unroll
+                    for (int f = 0; f < NF; ++f) frag(0, ks, f);
                 }
 #pragma unroll
                 for (int s = NP - 1; s >= 0; --s)
 #pragma unroll
                     for (int q = s; q >= 0; --q)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks & 1][q][i], b[ks & 1][s - q][j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks % NFB][q][i], b[ks % NFB][s - q][j], acc[i][j], 0, 0, 0);
 #pragma unroll
                 for (int sl = c * NSL / NCH; sl < (c + 1) * NSL / NCH; ++sl) {
                     if (sl < TA::NS) {
@@ -706,7 +712,7 @@ static TnPlan gff_tn_plan(int NP, int64_t rows, int64_t cols, int64_t M) {
     };
     const int64_t mid = (int64_t)cdiv(rows, 256) * cdiv(cols, 128), small = (int64_t)cdiv(rows, 128) * cdiv(cols, 128);
     const int sm = runs(mid, 256);
-    if (NP == 1 && mid * sm >= 192) return TnPlan{1, sm};
+    if (mid * sm >= 192) return TnPlan{1, sm};
     return TnPlan{0, runs(small, 512)};
 }
 
@@ -804,9 +810,9 @@ static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, i
 // a product, 75 without loads and LDS writes).  Several pieces: three to six products an LDS byte, 128 x 128 with four waves.
 // Smaller tiles where larger ones would leave compute units without one.
 typedef GemmCfg<1, 64, 2, 2, 512, 2, 4> CfgBig;             // 256 x 256
-typedef GemmCfg<1, 64, 2, 2, 512, 4, 2> CfgMid;             // 256 x 128
+template <int NP> struct CfgMid { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 512, 4, 2> T; };             // 256 x 128
 template <int NP> struct CfgSmall { typedef GemmCfg<NP, NP == 1 ? 64 : 32, NP == 1 ? 2 : 1, NP == 1 ? 2 : 1, 256, 2, 2> T; };
-template <int NP> struct CfgDeep { typedef GemmCfg<NP, 64, 1, 1, 256, 2, 2> T; };
+template <int NP> struct CfgDeep { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 256, 2, 2> T; };
 
 template <int DT, typename C, int BM, int BN>
 static int gff_nt_go(NtParams &p, hipStream_t st) {
@@ -821,10 +827,9 @@ static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t 
     constexpr int NP = ElemOf<DT>::NP;
     NtParams p{a, b, c, N, M, N, K, 0, 0, (int)(N % 4 == 0 && aligned16(c))};
     auto tiles = [&](int bm, int bn) { return (int64_t)cdiv(M, bm) * cdiv(N, bn); };
-    if constexpr (NP == 1) {
+    if constexpr (NP == 1)
         if (tiles(256, 256) >= 256) return gff_nt_go<DT, CfgBig, 256, 256>(p, st);
-        if (tiles(256, 128) >= 192) return gff_nt_go<DT, CfgMid, 256, 128>(p, st);
-    }
+    if (tiles(256, 128) >= 192) return gff_nt_go<DT, typename CfgMid<NP>::T, 256, 128>(p, st);
     if (tiles(128, 128) >= 256) return gff_nt_go<DT, typename CfgSmall<NP>::T, 128, 128>(p, st);
     if (tiles(128, 64) >= 192) return gff_nt_go<DT, typename CfgDeep<NP>::T, 128, 64>(p, st);
     return gff_nt_go<DT, typename CfgDeep<NP>::T, 64, 64>(p, st);
@@ -841,11 +846,7 @@ static int gff_gate_go(GateParams &g, hipStream_t st) {
 template <int DT, bool BWD>
 static int gff_gate(GateParams &g, hipStream_t st) {
     constexpr int NP = ElemOf<DT>::NP;
-    if constexpr (NP == 1) {
-        // backward: a third accumulator leaves room for 128 rows
-        constexpr int BM = BWD ? 128 : 256;
-        if (g.fp % 128 == 0 && (int64_t)cdiv(g.Mp, BM) * (g.fp / 128) >= 256) return gff_gate_go<CfgBig, BM, 128, BWD>(g, st);
-    }
+    if ((int64_t)cdiv(g.Mp, 256) * (g.fp / 64) >= 256) return gff_gate_go<typename CfgMid<NP>::T, 256, 64, BWD>(g, st);
     return gff_gate_go<typename CfgSmall<NP>::T, 128, 64, BWD>(g, st);
 }
 
@@ -864,12 +865,8 @@ static int gff_tn(const Planes &a, const Planes &b, void *c0, void *c1, int64_t 
     const int splits = pl.splits;
     TnParams p{a, b, c0, c1, splits > 1 ? part : nullptr, half, valid, N, (c1 ? 2 : 1) * valid * N, 0, 0, 0, 0,
                (int)(N % 4 == 0 && aligned16(c0) && aligned16(c1))};
-    if constexpr (NP == 1) {
-        if (pl.big) gff_tn_go<DT, CfgMid, 256, 128>(p, rows, M, splits, st);
-        else gff_tn_go<DT, typename CfgSmall<NP>::T, 128, 128>(p, rows, M, splits, st);
-    } else {
-        gff_tn_go<DT, typename CfgSmall<NP>::T, 128, 128>(p, rows, M, splits, st);
-    }
+    if (pl.big) gff_tn_go<DT, typename CfgMid<NP>::T, 256, 128>(p, rows, M, splits, st);
+    else gff_tn_go<DT, typename CfgSmall<NP>::T, 128, 128>(p, rows, M, splits, st);
     ASR_CHECK_LAUNCH("gff_tn_kernel");
     if (splits > 1) {
         const int64_t n0 = valid * N;
