@@ -15,6 +15,7 @@
 // two LDS images for one piece, one image (two workgroups a compute unit hide each other's barriers) for two and three.
 // Rows and columns beyond the matrix are read from its last row (clamped) and masked in the epilogues; the arrays h, da, db
 // are padded to whole tiles with zeros, which is what the products over them read past the end.
+#include <type_traits>
 #include "pieces.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -61,11 +62,12 @@ __device__ __forceinline__ float act_fwd(int kind, float a) {
 }
 
 // -------------------------------------------------------------------------------------------- LDS images --
-// A workgroup of the products: pieces, depth of a k-tile, LDS images of it, register sets on their way, threads, and the waves'
-// grid WM x WN over the tile
-template <int NP_, int BK_, int NBUF_, int NSET_, int NT_, int WM_, int WN_>
+// A workgroup of the products: pieces, depth of a k-tile, LDS images of it, register sets on their way, threads, the waves'
+// grid WM x WN over the tile, and WK such grids that share out each k-tile's steps of 16 k
+template <int NP_, int BK_, int NBUF_, int NSET_, int NT_, int WM_, int WN_, int WK_ = 1>
 struct GemmCfg {
-    static constexpr int NP = NP_, BK = BK_, NBUF = NBUF_, NSET = NSET_, NT = NT_, WM = WM_, WN = WN_;
+    static constexpr int NP = NP_, BK = BK_, NBUF = NBUF_, NSET = NSET_, NT = NT_, WM = WM_, WN = WN_, WK = WK_;
+    static_assert(NT == 64 * WM * WN * WK, "threads");
 };
 // Images without padding; the 16-byte chunks of a row are permuted by an exclusive or with bits of the row, so that what a
 // read instruction takes at a time falls on different banks: the same chunk of 16 rows (k-contiguous image [row][BK], read with
@@ -227,7 +229,7 @@ __device__ __forceinline__ void main_loop(f32x16 (&acc)[TM][TN], TA &ta, TB &tb,
             __syncthreads();
         }
     } else {
-        constexpr int KS = C::BK / 16, NM = TM * TN, NCH = KS * NM, NF = TM + TN, NSL = TA::NS + TB::NS;
+        constexpr int KS = C::BK / 16 / C::WK, NM = TM * TN, NCH = KS * NM, NF = TM + TN, NSL = TA::NS + TB::NS;
         auto k_of = [&](int64_t kt) { return (kt < kt1 ? kt : kt1 - 1) * C::BK; };
         auto body = [&](auto tag, int64_t kt) {
             constexpr int P = decltype(tag)::value;
@@ -435,13 +437,13 @@ struct NtParams {
 };
 template <int DT, typename C, int BM, int BN>
 __global__ __launch_bounds__(C::NT, 2) void gff_nt_kernel(NtParams p) {
-    constexpr int NP = C::NP, RM = BM / C::WM, RN = BN / C::WN, TM = RM / 32, TN = RN / 32;
+    constexpr int NP = C::NP, RM = BM / C::WM, RN = BN / C::WN, TM = RM / 32, TN = RN / 32, GRID = C::WM * C::WN;
     typedef typename ElemOf<DT>::type E;
     typedef NtTile<C, BM> TA;
     typedef NtTile<C, BN> TB;
-    constexpr int POOL = C::NBUF * NP * (TA::IMG + TB::IMG), TURN = C::NT / 64 * 4096;
+    constexpr int POOL = C::NBUF * NP * (TA::IMG + TB::IMG), TURN = GRID * (4096 + (C::WK - 1) * TM * TN * 4096);
     __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > TURN ? POOL : TURN];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WN, wn = wave % C::WN;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave / GRID, wm = wave % GRID / C::WN, wn = wave % C::WN;
     int tm, tn;
     tile_of(blockIdx.x, p.ntiles, p.ncol, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
@@ -452,9 +454,27 @@ __global__ __launch_bounds__(C::NT, 2) void gff_nt_kernel(NtParams p) {
     ta.template init<false>(p.a, p.a, m0);
     tb.template init<false>(p.b, p.b, n0);
     main_loop<C>(acc, ta, tb, pool, 0, p.K / C::BK,
-                 [&](const unsigned char *img, int i, int ks) { return frag_nt<C::BK>(img, wm * RM + i * 32, ks, lane); },
-                 [&](const unsigned char *img, int j, int ks) { return frag_nt<C::BK>(img, wn * RN + j * 32, ks, lane); });
-    float *S = reinterpret_cast<float *>(pool) + wave * 1024;
+                 [&](const unsigned char *img, int i, int ks) { return frag_nt<C::BK>(img, wm * RM + i * 32, ks * C::WK + wk, lane); },
+                 [&](const unsigned char *img, int j, int ks) { return frag_nt<C::BK>(img, wn * RN + j * 32, ks * C::WK + wk, lane); });
+    float *S = reinterpret_cast<float *>(pool) + wave % GRID * 1024;
+    if constexpr (C::WK == 2) {                                                    // the second grid's sums join the first's
+        float *J = reinterpret_cast<float *>(pool) + GRID * 1024 + wave % GRID * TM * TN * 1024;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (wk == 1) J[((i * TN + j) * 16 + r) * 64 + lane] = acc[i][j][r];
+        __syncthreads();
+        if (wk == 1) return;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] += J[((i * TN + j) * 16 + r) * 64 + lane];
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -596,104 +616,135 @@ __global__ __launch_bounds__(256) void gff_pack_kernel(PackJobs jobs) {
 
 // ------------------------------------------------------------------------------------------- a few rows: tokens --
 // M <= 64 rows, forward only: the weights are read once from memory, which bounds it.  16 weight rows a workgroup, its waves
-// split k, products exact in v_mfma_f32_16x16x4_f32 (weights widened in registers: at 16 rows the matrix time is half of the
-// weights' memory time), rows of x in groups of 16.  GATE: two weight matrices and h = act(a) b to float32 h; else y.
-template <int DT, int NM, bool GATE>
+// (and, for the second product, `splits` workgroups) share k, rows of x in groups of 16; the loads of four steps of 32 k are
+// in flight.  16-bit weights are multiplied as their bf16 pieces (v_mfma_f32_16x16x32_bf16), the hidden values, which stay
+// float32 in between, as two; float32 weights exactly in v_mfma_f32_16x16x4_f32.  GATE: two weight matrices and h =
+// act(a) b to float32 h.  Otherwise y, or, with several workgroups a tile, float32 parts that gff_few_join_kernel adds in their
+// order (a last-arriver sum in the same launch took 65 us more: its device-wide fences write back the L2s).
+template <int DT> struct FewPieces { static constexpr int W = DT == ASR_T_BF16 ? 1 : 2; };
+template <int P>
+__device__ __forceinline__ void few_split(const float (&v)[8], bf16x8 (&o)[P]) {
+    u32x4p w[P];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        unsigned x[P];
+        split_pair<P>(v[2 * e], v[2 * e + 1], x);
+#pragma unroll
+        for (int q = 0; q < P; ++q) w[q][e] = x[q];
+    }
+#pragma unroll
+    for (int q = 0; q < P; ++q) o[q] = __builtin_bit_cast(bf16x8, w[q]);
+}
+template <int DT, int NM, int NW, bool GATE>
 __device__ __forceinline__ void few_rows_body(const typename ElemOf<DT>::type *wa, const typename ElemOf<DT>::type *wb,
-                                              const void *xin, bool x_is_float, bool vec, int64_t K, int M, int64_t N, int act,
-                                              float *h, typename ElemOf<DT>::type *y, int nw, float *red) {
+                                              const void *xin, bool vec, int64_t K, int64_t kb, int64_t ke, int M, int64_t N, int act,
+                                              float *h, typename ElemOf<DT>::type *y, float *part, float *red) {
     typedef typename ElemOf<DT>::type E;
-    constexpr int V = 8;                                             // k per lane and step: 32 k of a row over its four lanes
+    constexpr int V = 8, NS = GATE ? 2 : 1, NA = NS * NM;            // k per lane and step: 32 k of a row over its four lanes
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     const int64_t n = (int64_t)blockIdx.x * 16 + c, row = n < N ? n : N - 1;
-    f32x4 acc[GATE ? 2 : 1][NM];
+    f32x4 acc[NS][NM];
 #pragma unroll
-    for (int s = 0; s < (GATE ? 2 : 1); ++s)
+    for (int s = 0; s < NS; ++s)
 #pragma unroll
         for (int m = 0; m < NM; ++m) acc[s][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const E *ra = wa + row * K, *rb = GATE ? wb + row * K : wa;
-    const int64_t ldx = K;
-#pragma unroll 2
-    for (int64_t k0 = (int64_t)wave * 32; k0 < K; k0 += (int64_t)nw * 32) {
-        const int64_t k = k0 + g * V;
-        float va[V], vb[V], vx[NM][V];
+    const E *rw[2] = {wa + row * K, GATE ? wb + row * K : wa};
+    auto fetch = [&](const auto *a, int64_t k, float (&v)[V]) {      // eight of a row, zeros past the end
 #pragma unroll
-        for (int e = 0; e < V; ++e) va[e] = vb[e] = 0.f;
+        for (int e = 0; e < V; ++e) v[e] = 0.f;
         if (vec) {                                                   // K % 8 == 0: a lane's eight are all there or none is
-            if (k < K) {
-                load_vec<E, V>(ra + k, va);
-                if (GATE) load_vec<E, V>(rb + k, vb);
-            }
+            if (k < ke) load_vec<std::remove_const_t<std::remove_pointer_t<decltype(a)>>, V>(a + k, v);
         } else {
 #pragma unroll
             for (int e = 0; e < V; ++e)
-                if (k + e < K) {
-                    va[e] = (float)ra[k + e];
-                    if (GATE) vb[e] = (float)rb[k + e];
-                }
+                if (k + e < ke) v[e] = (float)a[k + e];
         }
+    };
+#pragma unroll 4
+    for (int64_t k0 = kb + (int64_t)wave * 32; k0 < ke; k0 += NW * 32) {
+        const int64_t k = k0 + g * V;
+        float vw[NS][V], vx[NM][V];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) fetch(rw[s], k, vw[s]);
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-            const int r = min(m * 16 + c, M - 1);
-#pragma unroll
-            for (int e = 0; e < V; ++e) vx[m][e] = 0.f;
-            if (vec) {
-                if (k < K) {
-                    if (x_is_float) load_vec<float, V>((const float *)xin + r * ldx + k, vx[m]);
-                    else load_vec<E, V>((const E *)xin + r * ldx + k, vx[m]);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (k + e < K) vx[m][e] = x_is_float ? ((const float *)xin)[r * ldx + k + e] : (float)((const E *)xin)[r * ldx + k + e];
-            }
+            const int64_t r = min(m * 16 + c, M - 1);
+            if constexpr (GATE) fetch((const E *)xin + r * K, k, vx[m]);
+            else fetch((const float *)xin + r * K, k, vx[m]);
         }
+        if constexpr (DT == ASR_T_F32) {
 #pragma unroll
-        for (int e = 0; e < V; ++e)
+            for (int e = 0; e < V; ++e)
+#pragma unroll
+                for (int m = 0; m < NM; ++m)
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) acc[s][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(vw[s][e], vx[m][e], acc[s][m], 0, 0, 0);
+        } else {
+            constexpr int PW = FewPieces<DT>::W, PX = GATE ? PW : 2, TOP = (PW > PX ? PW : PX) - 1;
+            bf16x8 w[NS][PW], x[PX];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) few_split<PW>(vw[s], w[s]);
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
-                acc[0][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(va[e], vx[m][e], acc[0][m], 0, 0, 0);
-                if constexpr (GATE) acc[1][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(vb[e], vx[m][e], acc[1][m], 0, 0, 0);
+                few_split<PX>(vx[m], x);
+#pragma unroll
+                for (int u = TOP; u >= 0; --u)
+#pragma unroll
+                    for (int q = 0; q < PW; ++q)
+#pragma unroll
+                        for (int s = 0; s < NS; ++s)
+                            if (u - q >= 0 && u - q < PX) acc[s][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[s][q], x[u - q], acc[s][m], 0, 0, 0);
             }
+        }
     }
     // D: column = x row (lane & 15), rows 4 g + r = weight rows; partials of the waves through LDS
-    constexpr int NA = (GATE ? 2 : 1) * NM;
 #pragma unroll
-    for (int s = 0; s < (GATE ? 2 : 1); ++s)
+    for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int m = 0; m < NM; ++m)
-            *reinterpret_cast<f32x4 *>(red + ((wave * NA + s * NM + m) * 64 + lane) * 4) = acc[s][m];
+        for (int m = 0; m < NM; ++m) *reinterpret_cast<f32x4 *>(red + ((wave * NA + s * NM + m) * 64 + lane) * 4) = acc[s][m];
     __syncthreads();
-    for (int t = threadIdx.x; t < NM * 64; t += blockDim.x) {
-        const int m = t >> 6, l = t & 63;
-        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-        for (int w = 0; w < nw; ++w) {
-            a += *reinterpret_cast<const f32x4 *>(red + ((w * NA + m) * 64 + l) * 4);
-            if (GATE) b += *reinterpret_cast<const f32x4 *>(red + ((w * NA + NM + m) * 64 + l) * 4);
-        }
-        const int r = m * 16 + (l & 15);
-        if (r >= M) continue;
+    const int t = threadIdx.x, m = t >> 6, l = t & 63, r = m * 16 + (l & 15);
+    if (t >= NM * 64) return;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t o = (int64_t)blockIdx.x * 16 + (l >> 4) * 4 + e;
-            if (o >= N) continue;
-            if (GATE) h[r * N + o] = act_fwd(act, a[e]) * b[e];
-            else y[r * N + o] = (E)a[e];
-        }
+    for (int w = 0; w < NW; ++w) {
+        a += *reinterpret_cast<const f32x4 *>(red + ((w * NA + m) * 64 + l) * 4);
+        if (GATE) b += *reinterpret_cast<const f32x4 *>(red + ((w * NA + NM + m) * 64 + l) * 4);
+    }
+    if (r >= M) return;
+    const int64_t o = (int64_t)blockIdx.x * 16 + (l >> 4) * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (o + e >= N) continue;
+        if (GATE) h[r * N + o + e] = act_fwd(act, a[e]) * b[e];
+        else if (gridDim.y > 1) part[((int64_t)blockIdx.y * M + r) * N + o + e] = a[e];
+        else y[r * N + o + e] = (E)a[e];
     }
 }
+#define FEW_NW 8
 template <int DT, int NM>
-__global__ __launch_bounds__(256) void gff_few_gate_kernel(const void *x, const void *wg, const void *wu, float *h, int64_t d,
-                                                           int64_t f, int M, int act, int vec) {
-    __shared__ __attribute__((aligned(16))) float red[4 * 2 * NM * 256];
+__global__ __launch_bounds__(64 * FEW_NW) void gff_few_gate_kernel(const void *x, const void *wg, const void *wu, float *h, int64_t d,
+                                                                   int64_t f, int M, int act, int vec) {
+    __shared__ __attribute__((aligned(16))) float red[FEW_NW * 2 * NM * 256];
     typedef typename ElemOf<DT>::type E;
-    few_rows_body<DT, NM, true>((const E *)wg, (const E *)wu, x, false, vec, d, M, f, act, h, nullptr, 4, red);
+    few_rows_body<DT, NM, FEW_NW, true>((const E *)wg, (const E *)wu, x, vec, d, 0, d, M, f, act, h, nullptr, nullptr, red);
 }
 template <int DT, int NM>
-__global__ __launch_bounds__(512) void gff_few_down_kernel(const float *h, const void *wd, void *y, int64_t f, int64_t n, int M, int vec) {
-    __shared__ __attribute__((aligned(16))) float red[8 * NM * 256];
+__global__ __launch_bounds__(64 * FEW_NW) void gff_few_down_kernel(const float *h, const void *wd, void *y, int64_t f, int64_t n, int M,
+                                                                   int vec, int64_t run, float *part) {
+    __shared__ __attribute__((aligned(16))) float red[FEW_NW * NM * 256];
     typedef typename ElemOf<DT>::type E;
-    few_rows_body<DT, NM, false>((const E *)wd, nullptr, h, true, vec, f, M, n, 0, nullptr, (E *)y, 8, red);
+    const int64_t kb = min(f, (int64_t)blockIdx.y * run), ke = min(f, kb + run);
+    few_rows_body<DT, NM, FEW_NW, false>((const E *)wd, nullptr, h, vec, f, kb, ke, M, n, 0, nullptr, (E *)y, part, red);
+}
+template <int DT>
+__global__ __launch_bounds__(256) void gff_few_join_kernel(const float *__restrict__ part, void *y, int64_t sz, int splits) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= sz) return;
+    float a = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) a += part[s * sz + i];
+    ((typename ElemOf<DT>::type *)y)[i] = (typename ElemOf<DT>::type)a;
 }
 
 // ------------------------------------------------------------------------------------------------------- host --
@@ -767,6 +818,21 @@ static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
 
 #define GFF_FEW_ROWS 64
 static bool gff_few(const asr_gated_ff_args *a) { return a->M <= GFF_FEW_ROWS; }
+// The second product's workgroups: two for each compute unit, each with at least 256 k
+struct FewPlan { int64_t h, part, bytes, run; int splits, tiles; };
+static FewPlan gff_few_plan(const asr_gated_ff_args *a) {
+    FewPlan p;
+    p.tiles = cdiv(a->n, 16);
+    int64_t s = 512 / p.tiles;
+    if (s > a->f / 256) s = a->f / 256;
+    if (s < 1) s = 1;
+    p.run = up_to((a->f + s - 1) / s, 32);
+    p.splits = cdiv(a->f, p.run);
+    p.h = 0;
+    p.part = up_to((int64_t)a->M * a->f * 4, 256);
+    p.bytes = p.part + (p.splits > 1 ? (int64_t)p.splits * a->M * a->n * 4 : 0);
+    return p;
+}
 
 static int gff_check(const asr_gated_ff_args *a, const char *who, bool ptrs) {
     ASR_CHECK_ARG(a, "%s: null pointer", who);
@@ -782,7 +848,7 @@ static int gff_check(const asr_gated_ff_args *a, const char *who, bool ptrs) {
 
 extern "C" int64_t asr_gated_ff_ws_bytes(const asr_gated_ff_args *a, int backward) {
     if (gff_check(a, "gated_ff_ws_bytes", false) != ASR_OK) return -1;
-    if (!backward && gff_few(a)) return up_to((int64_t)a->M * a->f * 4, 256);
+    if (!backward && gff_few(a)) return gff_few_plan(a).bytes;
     GffPlan p;
     gff_plan(a, backward != 0, p);
     return p.bytes;
@@ -811,6 +877,7 @@ static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, i
 // Smaller tiles where larger ones would leave compute units without one.
 typedef GemmCfg<1, 64, 2, 2, 512, 2, 4> CfgBig;             // 256 x 256
 template <int NP> struct CfgMid { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 512, 4, 2> T; };             // 256 x 128
+template <int NP> struct CfgHalf { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 512, 1, 4, 2> T; };      // 96 x 128, two grids of waves
 template <int NP> struct CfgSmall { typedef GemmCfg<NP, NP == 1 ? 64 : 32, NP == 1 ? 2 : 1, NP == 1 ? 2 : 1, 256, 2, 2> T; };
 template <int NP> struct CfgDeep { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 256, 2, 2> T; };
 
@@ -826,12 +893,22 @@ template <int DT>
 static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t N, int64_t K, hipStream_t st) {
     constexpr int NP = ElemOf<DT>::NP;
     NtParams p{a, b, c, N, M, N, K, 0, 0, (int)(N % 4 == 0 && aligned16(c))};
-    auto tiles = [&](int bm, int bn) { return (int64_t)cdiv(M, bm) * cdiv(N, bn); };
+    // The tile that is done first: the compute unit with most tiles has ceil(tiles / 256) of them; `rate` is the matrix work a
+    // unit does in a time, `one` the share of it that a lone workgroup reaches where two or three are meant to share the unit
+    // (from float32 products of 11968 x 256, k 2048 and 4096, bfloat16 ones of 8192 x 1024: 256 x 128 reaches 1.4 PFLOP/s
+    // scaled to all units, 128 x 64 two a unit 0.9)
+    auto time = [&](int bm, int bn, double rate, double one) {
+        const int64_t n = ((int64_t)cdiv(M, bm) * cdiv(N, bn) + 255) / 256;
+        return (double)n * bm * bn / (n == 1 ? rate * one : rate);
+    };
+    const double t256 = NP == 1 ? time(256, 256, 1.0, 1.0) : 1e300, tmid = time(256, 128, 0.95, 1.0), t96 = time(96, 128, 0.85, 1.0),
+                 t128 = time(128, 64, 0.6, 0.7), t64 = time(64, 64, 0.55, 0.9);
+    const double best = fmin(fmin(fmin(t256, tmid), fmin(t96, t128)), t64);
     if constexpr (NP == 1)
-        if (tiles(256, 256) >= 256) return gff_nt_go<DT, CfgBig, 256, 256>(p, st);
-    if (tiles(256, 128) >= 192) return gff_nt_go<DT, typename CfgMid<NP>::T, 256, 128>(p, st);
-    if (tiles(128, 128) >= 256) return gff_nt_go<DT, typename CfgSmall<NP>::T, 128, 128>(p, st);
-    if (tiles(128, 64) >= 192) return gff_nt_go<DT, typename CfgDeep<NP>::T, 128, 64>(p, st);
+        if (t256 == best) return gff_nt_go<DT, CfgBig, 256, 256>(p, st);
+    if (tmid == best) return gff_nt_go<DT, typename CfgMid<NP>::T, 256, 128>(p, st);
+    if (t96 == best) return gff_nt_go<DT, typename CfgHalf<NP>::T, 96, 128>(p, st);
+    if (t128 == best) return gff_nt_go<DT, typename CfgDeep<NP>::T, 128, 64>(p, st);
     return gff_nt_go<DT, typename CfgDeep<NP>::T, 64, 64>(p, st);
 }
 
@@ -932,10 +1009,16 @@ static int gff_run(const asr_gated_ff_args *a, bool bwd, hipStream_t st) {
 
 template <int DT, int NM>
 static int gff_few_run(const asr_gated_ff_args *a, hipStream_t st) {
-    hipLaunchKernelGGL((gff_few_gate_kernel<DT, NM>), dim3(cdiv(a->f, 16)), dim3(256), 0, st, a->x, a->wg, a->wu, (float *)a->ws,
-                       (int64_t)a->d, (int64_t)a->f, (int)a->M, a->act, (int)(a->d % 8 == 0 && aligned16(a->x) && aligned16(a->wg) && aligned16(a->wu)));
-    hipLaunchKernelGGL((gff_few_down_kernel<DT, NM>), dim3(cdiv(a->n, 16)), dim3(512), 0, st, (const float *)a->ws, a->wd, a->y,
-                       (int64_t)a->f, (int64_t)a->n, (int)a->M, (int)(a->f % 8 == 0 && aligned16(a->wd) && aligned16(a->ws)));
+    const FewPlan p = gff_few_plan(a);
+    char *ws = (char *)a->ws;
+    float *h = (float *)(ws + p.h), *part = (float *)(ws + p.part);
+    hipLaunchKernelGGL((gff_few_gate_kernel<DT, NM>), dim3(cdiv(a->f, 16)), dim3(64 * FEW_NW), 0, st, a->x, a->wg, a->wu, h, (int64_t)a->d,
+                       (int64_t)a->f, (int)a->M, a->act, (int)(a->d % 8 == 0 && aligned16(a->x) && aligned16(a->wg) && aligned16(a->wu)));
+    hipLaunchKernelGGL((gff_few_down_kernel<DT, NM>), dim3(p.tiles, p.splits), dim3(64 * FEW_NW), 0, st, (const float *)h, a->wd, a->y,
+                       (int64_t)a->f, (int64_t)a->n, (int)a->M, (int)(a->f % 8 == 0 && aligned16(a->wd) && aligned16(a->ws)), p.run, part);
+    if (p.splits > 1)
+        hipLaunchKernelGGL((gff_few_join_kernel<DT>), dim3(cdiv((int64_t)a->M * a->n, 256)), dim3(256), 0, st, (const float *)part, a->y,
+                           (int64_t)a->M * a->n, p.splits);
     ASR_CHECK_LAUNCH("gff_few_kernel");
     return ASR_OK;
 }
