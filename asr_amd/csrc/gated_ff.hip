@@ -561,10 +561,10 @@ __global__ __launch_bounds__(256) void gff_sum_kernel(const float *__restrict__ 
 struct PackJob {
     const void *src;
     __bf16 *dst;
-    int64_t lds, ldd, ps, R, C, wide;
-    int trans;
-    int64_t blk0;                        // first workgroup of the job
-    int64_t nx;                          // workgroups along the source's columns
+    int64_t lds, ldd, ps;
+    int R, C, wide, trans, vec;
+    int blk0;                            // first workgroup of the job
+    int nx;                              // workgroups along the source's columns
 };
 struct PackJobs { PackJob j[8]; int n; };
 
@@ -574,43 +574,45 @@ __global__ __launch_bounds__(256) void gff_pack_kernel(PackJobs jobs) {
     constexpr int NP = ElemOf<DT>::NP;
     __shared__ float tile[64][65];
     int k = 0;
-    while (k + 1 < jobs.n && (int64_t)blockIdx.x >= jobs.j[k + 1].blk0) ++k;
+    while (k + 1 < jobs.n && (int)blockIdx.x >= jobs.j[k + 1].blk0) ++k;
     const PackJob &J = jobs.j[k];
-    const int64_t b = blockIdx.x - J.blk0, by = b / J.nx, bx = b - by * J.nx;
+    const int b = (int)blockIdx.x - J.blk0, by = b / J.nx, bx = b - by * J.nx;
     const E *src = (const E *)J.src;
-    // a 64 x 64 block; source columns (or, transposed, rows) past the end read as zero
-    const int64_t r0 = by * 64, c0 = bx * 64;
-    const int tc = (threadIdx.x & 15) * 4, tr = threadIdx.x >> 4;
+    // a 64 x 64 block; source columns (or, transposed, rows) past the end read as zero.  All loads of a thread go out together.
+    const int tc = (threadIdx.x & 15) * 4, tr = threadIdx.x >> 4, r0 = by * 64 + tr, c0 = bx * 64 + tc;
+    float v[4][4];
+    if (J.vec != 0 && by * 64 + 64 <= J.R && bx * 64 + 64 <= J.C) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_vec<E, 4>(src + (int64_t)(r0 + 16 * i) * J.lds + c0, v[i]);
+    } else {
+        E t[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[i][e] = src[(int64_t)min(r0 + 16 * i, J.R - 1) * J.lds + min(c0 + e, J.C - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = r0 + 16 * i < J.R && c0 + e < J.C ? (float)t[i][e] : 0.f;
+    }
+    if (J.trans == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (r0 + 16 * i < J.R && c0 < J.wide)
+                put_pieces<NP>(J.dst + (int64_t)(r0 + 16 * i) * J.ldd + c0, J.ps, make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tile[tr + 16 * i][tc + e] = v[i][e];
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t r = r0 + tr + 16 * i;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (r < J.R) {
-            const E *q = src + r * J.lds + c0 + tc;
-            if (c0 + tc + 3 < J.C && (uintptr_t)q % (4 * sizeof(E)) == 0) {
-                load_vec<E, 4>(q, v);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c0 + tc + e < J.C) v[e] = (float)q[e];
-            }
-        }
-        if (!J.trans) {
-            if (r < J.R && c0 + tc < J.wide) put_pieces<NP>(J.dst + r * J.ldd + c0 + tc, J.ps, make_float4(v[0], v[1], v[2], v[3]));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) tile[tr + 16 * i][tc + e] = v[e];
-        }
-    }
-    if (J.trans) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t c = c0 + tr + 16 * i;                      // a row of the result
-            if (c < J.C && r0 + tc < J.wide)
-                put_pieces<NP>(J.dst + c * J.ldd + r0 + tc, J.ps,
-                               make_float4(tile[tc][tr + 16 * i], tile[tc + 1][tr + 16 * i], tile[tc + 2][tr + 16 * i], tile[tc + 3][tr + 16 * i]));
-        }
+        const int c = bx * 64 + tr + 16 * i, r = by * 64 + tc;                 // row and column of the result
+        if (c < J.C && r < J.wide)
+            put_pieces<NP>(J.dst + (int64_t)c * J.ldd + r, J.ps,
+                           make_float4(tile[tc][tr + 16 * i], tile[tc + 1][tr + 16 * i], tile[tc + 2][tr + 16 * i], tile[tc + 3][tr + 16 * i]));
     }
 }
 
@@ -842,6 +844,7 @@ static int gff_check(const asr_gated_ff_args *a, const char *who, bool ptrs) {
     ASR_CHECK_ARG(a->d <= (1 << 20) && a->f <= (1 << 20) && a->n <= (1 << 20), "%s: widths are at most 2^20", who);
     ASR_CHECK_ARG((int64_t)cdiv(a->M, 128) * cdiv(a->f > a->d ? (a->f > a->n ? a->f : a->n) : (a->d > a->n ? a->d : a->n), 64) < (1ll << 30),
                   "%s: too many rows", who);
+    ASR_CHECK_ARG(a->M <= (1ll << 30), "%s: at most 2^30 rows", who);
     if (ptrs) ASR_CHECK_ARG(a->x && a->wg && a->wu && a->wd && a->ws, "%s: null pointer", who);
     return ASR_OK;
 }
@@ -861,14 +864,15 @@ static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, i
     k.lds = C;
     k.ldd = ldd;
     k.ps = ps;
-    k.R = R;
-    k.C = C;
-    k.wide = wide;
+    k.R = (int)R;
+    k.C = (int)C;
+    k.wide = (int)wide;
     k.trans = trans;
-    k.blk0 = blocks;
+    k.vec = C % 4 == 0 && (uintptr_t)src % 16 == 0;
+    k.blk0 = (int)blocks;
     // straight: the padding columns belong to the last blocks of a row; transposed: to the last blocks of a column
     k.nx = cdiv(trans ? C : wide, 64);
-    blocks += k.nx * cdiv(trans ? wide : R, 64);
+    blocks += (int64_t)k.nx * cdiv(trans ? wide : R, 64);
 }
 
 // Workgroups of the products.  One piece: eight waves, 256 x 256 or 256 x 128 (a wave's 128 x 64 or 64 x 64): with four waves

@@ -4,7 +4,7 @@ table's, by differences), streams, captured graphs, refusals."""
 import pytest
 import torch
 
-from tests._transformer_ref import attention64, bucket64, held
+from tests._transformer_ref import attention64, bucket64, held, poison
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -24,6 +24,7 @@ def _check(q, k, v, up, table, *, lengths=None, keep=None, offset=None, causal=F
     d = [t.double() for t in (q, k, v, table)]
     ref = dict(lengths=lengths, keep=keep, offset=offset, causal=causal, reach=reach, scale=scale or q.shape[-1] ** -0.5)
     out = None
+    poison()
     if infer:
         out = bucket_attention(q, k, v, table, **kw)
         assert out.is_contiguous() and out.dtype == q.dtype

@@ -3,7 +3,7 @@ widths, few rows, gradients (the formula's and by differences), streams, capture
 import pytest
 import torch
 
-from tests._transformer_ref import gated_ff64, held
+from tests._transformer_ref import gated_ff64, held, poison
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -19,6 +19,7 @@ def _inputs(M, d, f, n, dtype, seed=0, scale=1.0):
 
 def _check(x, wg, wu, wd, dy, act="swish"):
     from asr_amd.Models.transformer_ops import gated_feed_forward
+    poison()
     leaves = [t.detach().requires_grad_() for t in (x, wg, wu, wd)]
     y = gated_feed_forward(*leaves, act=act)
     grads = torch.autograd.grad(y, leaves, dy)

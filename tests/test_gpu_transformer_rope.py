@@ -3,7 +3,7 @@ rotation, strides, far positions, single frames, gradients (the formula's and by
 import pytest
 import torch
 
-from tests._transformer_ref import rope64, within
+from tests._transformer_ref import poison, rope64, within
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -28,6 +28,7 @@ def _case(B, T, H, Hk, D, dtype, seed=0, packed=False):
 
 def _check(q, k, w, gr, pos, rot, base=10000.0, eps=1e-6):
     from asr_amd.Models.transformer_ops import qk_norm_rope
+    poison()
     T = q.shape[1]
     p64 = pos if pos is not None else torch.arange(T, device=q.device)
     leaves = [t.detach().requires_grad_() for t in (q, k, *w)]
