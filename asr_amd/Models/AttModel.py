@@ -32,7 +32,9 @@ class AttModel(nn.Module):
         # construction order = the reference's (encoder, then decoder) so a seeded
         # default init draws the same random numbers
         if enc == "Conformer":
-            self.encoder = TransformerEncoder(hp.lmfb_dim, 256, 16, 4, 0.1)     # Models/AttModel.py:17
+            # Models/AttModel.py:17; the two attributes are this package's and select its other sub-layers
+            self.encoder = TransformerEncoder(hp.lmfb_dim, 256, 16, 4, 0.1, getattr(hp, "encoder_attention", "relative"),
+                                              getattr(hp, "encoder_feed_forward", "swish"))
         else:
             self.encoder = Encoder(hp)
         self.decoder = Decoder(hp)

@@ -9,6 +9,11 @@ Every block of a layer is one autograd node with a hand-written backward over li
 matrix products on ``asr_sgemm``, everything else on the kernels of csrc/conformer.hip.
 Activations stay (B, T, C) row-major; no CPU fallback.
 
+Beyond the reference, a layer's attention can be one that is fused and keeps no T x T maps (``attention="rotary"`` or
+``"bucket"``: per-head norms of queries and keys with rotary positions, or with a learned bias by distance bucket) and its
+feed-forward blocks gated (``feed_forward="gated"``); both on the operators of Models/transformer_ops.py.  The defaults are
+the reference's.
+
 Not mirrored: the per-layer attention maps the reference collects and drops (``attns_enc``, :361-364).
 """
 import ctypes as C
@@ -21,10 +26,13 @@ import torch.nn as nn
 
 from .. import _lib, ops, streams
 from .._lib import check
+from . import transformer_ops as tops
 
 KSIZE = 31      # Transformer_encoder.py:215
 LN_EPS = 1e-5   # nn.LayerNorm / nn.BatchNorm1d defaults
 BN_MOMENTUM = 0.1
+ROPE_BASE = 10000.0         # positions of attention="rotary"
+BUCKETS, REACH = 32, 128    # distance buckets of attention="bucket" and the distance from which on the last one holds
 
 
 # Arithmetic of this encoder's matrix products (ops.gemm_precision): the bf16x3 split, like the rest of the model,
@@ -329,6 +337,79 @@ class _RelAttnFunction(torch.autograd.Function):
                 None, None, None, None, None)
 
 
+# ------------------------------------------- attention with head norms, rotation or distance buckets --
+class _HeadNormAttnFunction(torch.autograd.Function):
+    """y = x + drop(out(attention(norm and rotation of q, k; v))), q, k, v = the three Linears of LN(x).  ``rot``: rotated
+    elements of a head (0: none), ``table``: biases by distance bucket or None.  The attention itself passes no dropout:
+    its maps are never formed."""
+
+    @staticmethod
+    @_exact
+    def forward(ctx, x, nw, nb_, wq, bq, wk, bk, wv, bv, gq, gk, table, wo, bo, keep, H, rot, reach, p, training):
+        B, T, d = x.shape
+        x2 = _req(x).view(B * T, d)
+        h, mean, rstd = _ln_fwd(x2, nw, nb_)
+        q, k, v = (_linear(h, w, b).view(B, T, H, d // H) for w, b in ((wq, bq), (wk, bk), (wv, bv)))
+        qr, kr = tops._rope_fwd(q, k, gq, gk, None, rot, ROPE_BASE, LN_EPS)
+        scale = 1.0 / math.sqrt(d // H)
+        cx, lse, _ = tops._attn_fwd(qr, kr, v, table, None, keep, None, False, reach, scale, True)
+        y, m_o, f_o = _residual_drop(x2, _linear(cx.view(B * T, d), wo, bo), 1.0, p, training, 1)
+        ctx.save_for_backward(x2, nw, wq, wk, wv, gq, gk, table, wo, keep, mean, rstd, h, q, k, v, qr, kr, cx, lse)
+        ctx.aux = (rot, reach, scale, m_o, f_o)
+        ctx.wparams = (wq, bq, wk, bk, wv, bv, wo, bo, nw, nb_)
+        return y.view_as(x)
+
+    @staticmethod
+    @_exact
+    def backward(ctx, dy):
+        (x2, nw, wq, wk, wv, gq, gk, table, wo, keep, mean, rstd, h, q, k, v, qr, kr, cx, lse) = ctx.saved_tensors
+        rot, reach, scale, m_o, f_o = ctx.aux
+        dy2 = dy.contiguous().view_as(x2)
+        d = x2.shape[1]
+        do = _scale_mask(dy2, m_o, f_o)
+        dcx = _linear_dx(do, wo)
+        dqr, dkr, dv, dtable = tops._attn_bwd(qr, kr, v, table, None, keep, None, lse, cx, False, reach, scale, dcx.view_as(cx))
+        dq, dk, dgq, dgk = tops._rope_bwd(q, k, gq, gk, None, rot, ROPE_BASE, LN_EPS, dqr, dkr)
+        dq, dk, dv = (t.view_as(x2) for t in (dq, dk, dv))
+        dh = _linear_dx(dq, wq)
+        _linear_dx(dk, wk, dx_out=dh, accumulate=True)
+        _linear_dx(dv, wv, dx_out=dh, accumulate=True)
+        dx, lnpart = _ln_bwd(dh, x2, nw, mean, rstd, dy2)
+        with streams.on_side(dy2.device, do, cx, dq, dk, dv, h, lnpart, params=ctx.wparams):
+            dg, dbeta = _ln_bwd_sums(lnpart)
+            (dWo, dWq, dWk, dWv), (dbo, dbq, dbk, dbv) = _linear_dw(
+                [(do, cx.view_as(x2), wo), (dq, h, wq), (dk, h, wk), (dv, h, wv)], [(do, d), (dq, d), (dk, d), (dv, d)])
+        return (dx.view_as(dy), dg, dbeta, dWq, dbq, dWk, dbk, dWv, dbv, dgq, dgk, dtable, dWo, dbo, None, None, None, None,
+                None, None)
+
+
+# ------------------------------------------------------------ gated feed-forward block --
+class _GatedFFFunction(torch.autograd.Function):
+    """y = x + scale * drop^n((swish(h Wg^T) * (h Wu^T)) Wd^T), h = LN(x); the hidden values pass no dropout: they are formed
+    and used inside one operator and formed again in the backward."""
+
+    @staticmethod
+    @_exact
+    def forward(ctx, x, ln_w, ln_b, wg, wu, wd, scale, p, training, n_out_drop):
+        x2 = _req(x).view(-1, x.shape[-1])
+        h, mean, rstd = _ln_fwd(x2, ln_w, ln_b)
+        y, m_o, f = _residual_drop(x2, tops._ff_fwd(h, wg, wu, wd, tops.ACTIVATIONS["swish"]), scale, p, training, n_out_drop)
+        ctx.save_for_backward(x2, ln_w, wg, wu, wd, mean, rstd, h)
+        ctx.aux = (m_o, f)
+        return y.view_as(x)
+
+    @staticmethod
+    @_exact
+    def backward(ctx, dy):
+        x2, ln_w, wg, wu, wd, mean, rstd, h = ctx.saved_tensors
+        m_o, f = ctx.aux
+        dy2 = dy.contiguous().view_as(x2)
+        dh, dwg, dwu, dwd = tops._ff_bwd(h, wg, wu, wd, tops.ACTIVATIONS["swish"], _scale_mask(dy2, m_o, f))
+        dx, lnpart = _ln_bwd(dh, x2, ln_w, mean, rstd, dy2)
+        dg, dbeta = _ln_bwd_sums(lnpart)
+        return dx.view_as(dy), dg, dbeta, dwg, dwu, dwd, None, None, None, None
+
+
 # ------------------------------------------------------------ convolution module --
 class _ConvModuleFunction(torch.autograd.Function):
     """y = x + drop(pw2(swish(BN(conv_out(depthwise(GLU(pw1(LN(x)))))))))  (ConvolutionModule :228-240 inside
@@ -525,6 +606,49 @@ class RelativeMultiHeadAttention(nn.Module):
         self.p = dropout
 
 
+class HeadNormAttention(nn.Module):
+    """Self-attention on normed heads: with rotary positions (``rotary``) or a learned bias by distance bucket."""
+
+    def __init__(self, heads, d_model, rotary, dropout=0.1):
+        super().__init__()
+        self.d_model, self.d_k, self.h = d_model, d_model // heads, heads
+        self.q_linear = nn.Linear(d_model, d_model)
+        self.v_linear = nn.Linear(d_model, d_model)
+        self.k_linear = nn.Linear(d_model, d_model)
+        self.q_norm = nn.Parameter(torch.ones(self.d_k))
+        self.k_norm = nn.Parameter(torch.ones(self.d_k))
+        if rotary:
+            self.register_parameter("distance_bias", None)
+        else:
+            self.distance_bias = nn.Parameter(torch.zeros(BUCKETS, heads))
+        self.out = nn.Linear(d_model, d_model)
+        self.p = dropout
+
+    def run(self, x, norm, keep):
+        return _HeadNormAttnFunction.apply(
+            x, norm.weight, norm.bias, self.q_linear.weight, self.q_linear.bias, self.k_linear.weight, self.k_linear.bias,
+            self.v_linear.weight, self.v_linear.bias, self.q_norm, self.k_norm, self.distance_bias, self.out.weight, self.out.bias,
+            keep, self.h, self.d_k if self.distance_bias is None else 0, REACH, self.p, self.training)
+
+
+class GatedFeedForwardConformer(nn.Module):
+    def __init__(self, d_model, d_ff=2048, dropout=0.1):
+        super().__init__()
+        self.layer_norm = nn.LayerNorm(d_model)
+        self.linear_gate = nn.Linear(d_model, d_ff, bias=False)
+        self.linear_up = nn.Linear(d_model, d_ff, bias=False)
+        self.linear_down = nn.Linear(d_ff, d_model, bias=False)
+        self.p = dropout
+
+    def run(self, x, scale, n_out_drop):
+        return _GatedFFFunction.apply(x, self.layer_norm.weight, self.layer_norm.bias, self.linear_gate.weight, self.linear_up.weight,
+                                      self.linear_down.weight, scale, self.p, self.training, n_out_drop)
+
+
+ATTENTIONS = ("relative", "rotary", "bucket")
+FEED_FORWARDS = ("swish", "gated")
+
+
 class ConvolutionModule(nn.Module):
     def __init__(self, d_model, dropout=0.1):
         super().__init__()
@@ -548,22 +672,27 @@ class ConvolutionModule(nn.Module):
 
 
 class ConformerEncoderLayer(nn.Module):
-    def __init__(self, d_model, heads, dropout=0.1):
+    def __init__(self, d_model, heads, dropout=0.1, attention="relative", feed_forward="swish"):
         super().__init__()
-        self.ff_1 = FeedForwardConformer(d_model, dropout=dropout)
+        ff = FeedForwardConformer if feed_forward == "swish" else GatedFeedForwardConformer
+        self.ff_1 = ff(d_model, dropout=dropout)
         self.norm = nn.LayerNorm(d_model)
-        self.attn = RelativeMultiHeadAttention(heads, d_model, dropout=dropout)
+        self.attn = (RelativeMultiHeadAttention(heads, d_model, dropout=dropout) if attention == "relative"
+                     else HeadNormAttention(heads, d_model, attention == "rotary", dropout=dropout))
         self.conv_module = ConvolutionModule(d_model, dropout=dropout)
-        self.ff_2 = FeedForwardConformer(d_model, dropout=dropout)
+        self.ff_2 = ff(d_model, dropout=dropout)
         self.p = dropout
 
     def forward(self, x, pe, keep):
         at = self.attn
         x = self.ff_1.run(x, 0.5, 1)                                        # :259
-        x = _RelAttnFunction.apply(x, self.norm.weight, self.norm.bias, at.q_linear.weight, at.q_linear.bias,
-                                   at.k_linear.weight, at.k_linear.bias, at.v_linear.weight, at.v_linear.bias,
-                                   at.linear_pos.weight, at.pos_bias_u, at.pos_bias_v, at.out.weight, at.out.bias,
-                                   pe, keep, at.h, self.p, self.training)   # :260-263
+        if isinstance(at, HeadNormAttention):
+            x = at.run(x, self.norm, keep)
+        else:
+            x = _RelAttnFunction.apply(x, self.norm.weight, self.norm.bias, at.q_linear.weight, at.q_linear.bias,
+                                       at.k_linear.weight, at.k_linear.bias, at.v_linear.weight, at.v_linear.bias,
+                                       at.linear_pos.weight, at.pos_bias_u, at.pos_bias_v, at.out.weight, at.out.bias,
+                                       pe, keep, at.h, self.p, self.training)   # :260-263
         x = self.conv_module.run(x)                                         # :264
         return self.ff_2.run(x, 1.0, 2)                                     # :265
 
@@ -606,20 +735,28 @@ class _Dropout(torch.autograd.Function):
 
 
 class ConformerEncoder(nn.Module):
-    def __init__(self, d_model, N, heads, dropout):
+    def __init__(self, d_model, N, heads, dropout, attention="relative", feed_forward="swish"):
         super().__init__()
-        self.N, self.heads = N, heads
+        if attention not in ATTENTIONS or feed_forward not in FEED_FORWARDS:
+            raise ValueError(f"asr_amd ConformerEncoder: attention {attention!r} must be one of {ATTENTIONS}, feed_forward "
+                             f"{feed_forward!r} one of {FEED_FORWARDS}")
+        if attention != "relative" and (d_model % heads or (d_model // heads) % 2 or d_model // heads > 128):
+            raise ValueError(f"asr_amd ConformerEncoder: attention {attention!r} needs heads of an even width of at most 128")
+        self.N, self.heads, self.attention = N, heads, attention
         self.pe = RelativePositionalEncoder(d_model, dropout=dropout)
-        self.layers = nn.Sequential(*[ConformerEncoderLayer(d_model, heads, dropout) for _ in range(N)])
+        self.layers = nn.Sequential(*[ConformerEncoderLayer(d_model, heads, dropout, attention, feed_forward) for _ in range(N)])
 
     def forward(self, src, keep):
         T = src.shape[1]
-        if T > 1024:
-            raise RuntimeError("asr_amd ConformerEncoder: more than 1024 subsampled frames (softmax kernel limit)")
-        pe = self.pe.table(T, src.device)
-        x = src
+        x, pe = src, None
+        if self.attention == "relative":
+            if T > 1024:
+                raise RuntimeError("asr_amd ConformerEncoder: more than 1024 subsampled frames (softmax kernel limit)")
+            pe = self.pe.table(T, src.device)
         if self.training and self.pe.p > 0.0:
-            x, pe = _Dropout.apply(x, self.pe.p), _Dropout.apply(pe.contiguous(), self.pe.p)
+            x = _Dropout.apply(x, self.pe.p)
+            if pe is not None:
+                pe = _Dropout.apply(pe.contiguous(), self.pe.p)
         for layer in self.layers:
             x = layer(x, pe, keep)
         return x
@@ -640,12 +777,13 @@ class CNN_embedding(nn.Module):
 
 
 class TransformerEncoder(nn.Module):
-    """Transformer_encoder.py:441-451."""
+    """Transformer_encoder.py:441-451.  ``attention``: "relative" (the reference's), "rotary" or "bucket"; ``feed_forward``:
+    "swish" (the reference's) or "gated"."""
 
-    def __init__(self, src_vocab, d_model, N_e, heads, dropout):
+    def __init__(self, src_vocab, d_model, N_e, heads, dropout, attention="relative", feed_forward="swish"):
         super().__init__()
         self.cnn_encoder = CNN_embedding(src_vocab, d_model, d_model)
-        self.encoder = ConformerEncoder(d_model, N_e, heads, dropout)
+        self.encoder = ConformerEncoder(d_model, N_e, heads, dropout, attention, feed_forward)
 
     def forward(self, src, src_pos):
         if not src.is_cuda:

@@ -76,6 +76,24 @@ def _rope_fwd(q, k, wq, wk, pos, rot, base, eps):
     return qo, ko
 
 
+def _rope_bwd(q, k, wq, wk, pos, rot, base, eps, gq, gk):
+    """Gradients of q, k and the two weights."""
+    lib = _lib.load()
+    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+    if not q.numel():
+        return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk)
+    gq, gk = _heads(gq), _heads(gk)
+    dwq, dwk, ws = torch.empty_like(wq), torch.empty_like(wk), wq.new_empty(lib.asr_qk_norm_rope_ws_floats(q.shape[-1]))
+    a = _rope_args(q, k, wq, wk, pos, rot, base, eps)
+    a.gq, a.gk, a.q_out, a.k_out = gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr()
+    a.gq_sb, a.gq_st, a.gq_sh, _ = gq.stride()
+    a.gk_sb, a.gk_st, a.gk_sh, _ = gk.stride()
+    a.dwq, a.dwk, a.ws = dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr()
+    with _on(q.device):
+        check(lib.asr_qk_norm_rope_bwd(C.byref(a), _stream(q.device)))
+    return dq, dk, dwq, dwk
+
+
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, pos, rot, base, eps):
@@ -86,22 +104,7 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        q, k, wq, wk, pos = ctx.saved_tensors
-        lib = _lib.load()
-        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
-        if not q.numel():
-            return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk), None, None, None, None
-        gq, gk = _heads(gq), _heads(gk)
-        D = q.shape[-1]
-        dwq, dwk, ws = torch.empty_like(wq), torch.empty_like(wk), wq.new_empty(lib.asr_qk_norm_rope_ws_floats(D))
-        a = _rope_args(q, k, wq, wk, pos, *ctx.aux)
-        a.gq, a.gk, a.q_out, a.k_out = gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr()
-        a.gq_sb, a.gq_st, a.gq_sh, _ = gq.stride()
-        a.gk_sb, a.gk_st, a.gk_sh, _ = gk.stride()
-        a.dwq, a.dwk, a.ws = dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr()
-        with _on(q.device):
-            check(lib.asr_qk_norm_rope_bwd(C.byref(a), _stream(q.device)))
-        return dq, dk, dwq, dwk, None, None, None, None
+        return (*_rope_bwd(*ctx.saved_tensors, *ctx.aux, gq, gk), None, None, None, None)
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions=None, rot_dim=None, base=10000.0, eps=1e-6):
@@ -178,8 +181,11 @@ def _edges_host(num_buckets, max_distance, causal):
 def _attn_args(q, k, v, table, lengths, keep, offset, causal, reach, scale, train):
     B, Tq, H, D = q.shape
     a = _lib.BucketAttentionArgs()
-    a.q, a.k, a.v, a.table = q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr()
-    a.edges_host = C.addressof(_edges_host(table.shape[0], reach, causal))
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    nb = 2 if causal else 4
+    if table is not None:
+        nb, a.table = table.shape[0], table.data_ptr()
+    a.edges_host = C.addressof(_edges_host(nb, reach, causal))
     if lengths is not None:
         a.lengths = lengths.data_ptr()
     if offset is not None:
@@ -190,7 +196,7 @@ def _attn_args(q, k, v, table, lengths, keep, offset, causal, reach, scale, trai
     a.k_sb, a.k_st, a.k_sh, _ = k.stride()
     a.v_sb, a.v_st, a.v_sh, _ = v.stride()
     a.B, a.Tq, a.Tk, a.H, a.Hk, a.D = B, Tq, k.shape[1], H, k.shape[2], D
-    a.nb, a.causal, a.dtype, a.train, a.scale = table.shape[0], int(causal), _DTYPES[q.dtype], int(train), scale
+    a.nb, a.causal, a.dtype, a.train, a.scale = nb, int(causal), _DTYPES[q.dtype], int(train), scale
     return a
 
 
@@ -221,37 +227,39 @@ def _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, train
     return out, lse, out32
 
 
+def _attn_bwd(q, k, v, table, lengths, keep, offset, lse, out32, causal, reach, scale, g):
+    """Gradients of q, k, v and the table (None without one)."""
+    dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
+    dt = torch.empty_like(table) if table is not None else None
+    if not q.numel() or not k.shape[1]:
+        return tuple(t.zero_() if t is not None else None for t in (dq, dk, dv, dt))
+    lib = _lib.load()
+    g = _heads(g)
+    a = _attn_args(q, k, v, table, lengths, keep, offset, causal, reach, scale, True)
+    a.g, a.lse, a.out32, a.out = g.data_ptr(), lse.data_ptr(), out32.data_ptr(), out32.data_ptr()
+    a.g_sb, a.g_st, a.g_sh, _ = g.stride()
+    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    if dt is not None:
+        a.dtable = dt.data_ptr()
+    with _on(q.device):
+        ws = _attn_workspace(lib, a, True, q.device)
+        a.ws = ws.data_ptr()
+        check(lib.asr_bucket_attention_bwd(C.byref(a), _stream(q.device)))
+    return dq, dk, dv, dt
+
+
 class _BucketAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lengths, keep, offset, causal, reach, scale):
         out, lse, out32 = _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, True)
-        if out32 is out:
-            out32 = None                                       # saved below as an output: a saved input copy would be a cycle
-            ctx.save_for_backward(q, k, v, table, lengths, keep, offset, lse, out)
-        else:
-            ctx.save_for_backward(q, k, v, table, lengths, keep, offset, lse, out32)
+        ctx.save_for_backward(q, k, v, table, lengths, keep, offset, lse, out32)
         ctx.aux = (causal, reach, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        q, k, v, table, lengths, keep, offset, lse, out32 = ctx.saved_tensors
-        dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
-        dt = torch.empty_like(table)
-        if not q.numel() or not k.shape[1]:
-            return (*(t.zero_() for t in (dq, dk, dv, dt)), None, None, None, None, None, None)
-        lib = _lib.load()
-        g = _heads(g)
-        a = _attn_args(q, k, v, table, lengths, keep, offset, *ctx.aux, True)
-        a.g, a.lse, a.out32, a.out = g.data_ptr(), lse.data_ptr(), out32.data_ptr(), out32.data_ptr()
-        a.g_sb, a.g_st, a.g_sh, _ = g.stride()
-        a.dq, a.dk, a.dv, a.dtable = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dt.data_ptr()
-        with _on(q.device):
-            ws = _attn_workspace(lib, a, True, q.device)
-            a.ws = ws.data_ptr()
-            check(lib.asr_bucket_attention_bwd(C.byref(a), _stream(q.device)))
-        return dq, dk, dv, dt, None, None, None, None, None, None
+        return (*_attn_bwd(*ctx.saved_tensors, *ctx.aux, g), None, None, None, None, None, None)
 
 
 def _per_utterance(who, name, t, B, q):
@@ -260,11 +268,11 @@ def _per_utterance(who, name, t, B, q):
     return t.to(torch.int32).contiguous()
 
 
-def bucket_attention(q, k, v, table, lengths=None, keep=None, offset=None, causal=False, max_distance=128, scale=None):
+def bucket_attention(q, k, v, table=None, lengths=None, keep=None, offset=None, causal=False, max_distance=128, scale=None):
     """softmax(scale q k^T + table[bucket of each key's distance from the query]) v, differentiable in q, k, v and table.
 
     q (B, Tq, H, D), k and v (B, Tk, Hk, D) with H a multiple of Hk (query head h reads key head h // (H / Hk)), table
-    (num_buckets, H) float32, scale 1 / sqrt(D) by default.  Query i of utterance b stands at position offset[b] + i
+    (num_buckets, H) float32, None for no bias, scale 1 / sqrt(D) by default.  Query i of utterance b stands at position offset[b] + i
     (``offset`` (B,), default zeros) and key j at position j; ``bucket_edges`` says how distances fall into buckets: with
     ``causal`` a query reads only the keys up to its own position and all buckets are for the past, otherwise the second half
     of the buckets is for the keys behind the query.  Keys from ``lengths[b]`` on and keys with ``keep[b, j]`` false are left
@@ -275,15 +283,18 @@ def bucket_attention(q, k, v, table, lengths=None, keep=None, offset=None, causa
     _tensor(who, "q", q, 4)
     _tensor(who, "k", k, 4, like=q)
     _tensor(who, "v", v, 4, like=q)
-    _tensor(who, "table", table, 2, like=q, dtype=torch.float32)
     B, Tq, H, D = q.shape
     if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or H == 0 or k.shape[2] == 0 or H % k.shape[2]:
         raise RuntimeError(f"asr_amd.{who}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
     if not 1 <= D <= 128:
         raise RuntimeError(f"asr_amd.{who}: head width {D}: must be in [1, 128]")
-    nb, causal, reach = table.shape[0], bool(causal), int(max_distance)
-    if table.shape[1] != H:
-        raise RuntimeError(f"asr_amd.{who}: table must be (buckets, {H}), got {tuple(table.shape)}")
+    causal, reach = bool(causal), int(max_distance)
+    nb = 2 if causal else 4
+    if table is not None:
+        _tensor(who, "table", table, 2, like=q, dtype=torch.float32)
+        nb, table = table.shape[0], table.contiguous()
+        if table.shape[1] != H:
+            raise RuntimeError(f"asr_amd.{who}: table must be (buckets, {H}), got {tuple(table.shape)}")
     if not 2 <= nb <= MAX_BUCKETS or (not causal and (nb < 4 or nb % 2)):
         raise RuntimeError(f"asr_amd.{who}: {nb} buckets: 2 to {MAX_BUCKETS}, an even number of at least 4 unless causal")
     if not (nb if causal else nb // 2) // 2 < reach <= MAX_DISTANCE:
@@ -299,8 +310,9 @@ def bucket_attention(q, k, v, table, lengths=None, keep=None, offset=None, causa
             raise RuntimeError(f"asr_amd.{who}: keep must be ({B}, {k.shape[1]}) truth values on {q.device}")
         keep = keep.contiguous()
     scale = D ** -0.5 if scale is None else float(scale)
-    q, k, v, table = _heads(q), _heads(k), _heads(v), table.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
+    q, k, v = _heads(q), _heads(k), _heads(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (table is not None and table.requires_grad)):
         return _BucketAttention.apply(q, k, v, table, lengths, keep, offset, causal, reach, scale)
     return _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, False)[0]
 
@@ -337,6 +349,27 @@ def _ff_fwd(x2, wg, wu, wd, act):
     return y
 
 
+def _ff_bwd(x2, wg, wu, wd, act, dy, need=(True, True, True, True)):
+    """Gradients of x2 and the three weights, None for what `need` leaves out (the two first weights come together)."""
+    if not x2.shape[0]:
+        return torch.zeros_like(x2), torch.zeros_like(wg), torch.zeros_like(wu), torch.zeros_like(wd)
+    lib = _lib.load()
+    dy = dy.contiguous()
+    a = _ff_args(x2, wg, wu, wd, act)
+    a.dy = dy.data_ptr()
+    dx = torch.empty_like(x2) if need[0] else None
+    dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need[1] or need[2] else (None, None)
+    dwd = torch.empty_like(wd) if need[3] else None
+    for n, t in (("dx", dx), ("dwg", dwg), ("dwu", dwu), ("dwd", dwd)):
+        if t is not None:
+            setattr(a, n, t.data_ptr())
+    with _on(x2.device):
+        ws = _ff_workspace(lib, a, True, x2.device)
+        a.ws = ws.data_ptr()
+        check(lib.asr_gated_ff_bwd(C.byref(a), _stream(x2.device)))
+    return dx, dwg, dwu, dwd
+
+
 class _GatedFF(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2, wg, wu, wd, act):
@@ -347,25 +380,7 @@ class _GatedFF(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x2, wg, wu, wd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        if not x2.shape[0]:
-            return torch.zeros_like(x2), torch.zeros_like(wg), torch.zeros_like(wu), torch.zeros_like(wd), None
-        lib = _lib.load()
-        dy = dy.contiguous()
-        a = _ff_args(x2, wg, wu, wd, ctx.act)
-        a.dy = dy.data_ptr()
-        dx = torch.empty_like(x2) if need[0] else None
-        dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need[1] or need[2] else (None, None)
-        dwd = torch.empty_like(wd) if need[3] else None
-        for n, t in (("dx", dx), ("dwg", dwg), ("dwu", dwu), ("dwd", dwd)):
-            if t is not None:
-                setattr(a, n, t.data_ptr())
-        with _on(x2.device):
-            ws = _ff_workspace(lib, a, True, x2.device)
-            a.ws = ws.data_ptr()
-            check(lib.asr_gated_ff_bwd(C.byref(a), _stream(x2.device)))
-        return dx, dwg, dwu, dwd, None
+        return (*_ff_bwd(*ctx.saved_tensors, ctx.act, dy, ctx.needs_input_grad), None)
 
 
 def gated_feed_forward(x, w_gate, w_up, w_down, act="swish"):

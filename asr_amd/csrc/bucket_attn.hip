@@ -85,7 +85,7 @@ __device__ __forceinline__ int bucket_of(const Buckets &b, const int16_t *edge, 
 // biases by distance -R - PAD .. R + PAD of one head, times log2(e); ends with the line written but not yet visible
 __device__ __forceinline__ void fill_lut(float *lut, BucketLds &s, const AttnParams &p, int h) {
     const int R = p.bk.R;
-    for (int i = threadIdx.x; i < p.bk.nb; i += 256) s.tab[i] = p.table[i * p.H + h] * LOG2E;
+    for (int i = threadIdx.x; i < p.bk.nb; i += 256) s.tab[i] = p.table ? p.table[i * p.H + h] * LOG2E : 0.f;
     if ((int)threadIdx.x < p.bk.nedge) s.edge[threadIdx.x] = p.bk.edge[threadIdx.x];
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * (R + LUT_PAD) + 1; i += 256)
@@ -482,7 +482,9 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
                         s[0][4 * r4 + e] = ((w >> (8 * e)) & 1) && 8 * r4 + e <= seen ? s[0][4 * r4 + e] : 0.f;
                 }
             }
-            if (hi <= -R || lo >= R) {
+            if (p.tpart == nullptr) {
+                // no table: no sums by distance
+            } else if (hi <= -R || lo >= R) {
                 float t = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) t += s[0][r];
@@ -518,6 +520,7 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
         line[4 * LN + 4 + wave] = farr;
     }
     if (on) put_acc<E, DP>((E *)p.dq + (((int64_t)b * p.Tq + i) * p.H + h) * p.D, dq, p.scale, p.D, half);
+    if (p.tpart == nullptr) return;
     __syncthreads();
     for (int t = threadIdx.x; t < LN; t += 256) {
         float a = line[t];
@@ -753,7 +756,7 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
     }
     const int pmin = off, pmax = off + p.Tq - 1;
     const bool near = !(je - 1 - pmin <= -R || jb - pmax >= R);                        // some key of the run within the last edge
-    for (int t = lane; t < p.bk.nb * p.G; t += 64) tab[t] = p.table[(t / p.G) * p.H + hk * p.G + t % p.G] * LOG2E;
+    for (int t = lane; t < p.bk.nb * p.G; t += 64) tab[t] = p.table ? p.table[(t / p.G) * p.H + hk * p.G + t % p.G] * LOG2E : 0.f;
     for (int t = lane; t < p.bk.nedge; t += 64) edge[t] = p.bk.edge[t];
     __syncthreads();
     if (near)
@@ -975,7 +978,7 @@ static int battn_check(const asr_bucket_attention_args *a, const char *who, bool
         ASR_CHECK_ARG(a->edges_host[i] >= prev && a->edges_host[i] <= MAX_REACH, "%s: bucket edges must not fall, and stay within %d", who, MAX_REACH);
         prev = a->edges_host[i];
     }
-    if (ptrs) ASR_CHECK_ARG(a->q && a->k && a->v && a->table, "%s: null pointer", who);
+    if (ptrs) ASR_CHECK_ARG(a->q && a->k && a->v, "%s: null pointer", who);
     return ASR_OK;
 }
 
@@ -1106,7 +1109,7 @@ static int battn_bwd(const asr_bucket_attention_args *a, hipStream_t st) {
     char *ws = (char *)a->ws;
     float *delta = (float *)(ws + pl.off[W_DELTA]);
     p.delta = delta;
-    p.tpart = (float *)(ws + pl.off[W_TPART]);
+    p.tpart = a->table ? (float *)(ws + pl.off[W_TPART]) : nullptr;
     p.kvpart = (float *)(ws + pl.off[W_KV]);
     ASR_CHECK(battn_pack<DT>(a, pl, true, st));
     const int64_t rows = (int64_t)a->B * a->Tq * a->H;
@@ -1118,7 +1121,7 @@ static int battn_bwd(const asr_bucket_attention_args *a, hipStream_t st) {
     ASR_CHECK(battn_lds(battn_dq_kernel<DT, DP>, lds_q, "bucket_attention_bwd"));
     hipLaunchKernelGGL((battn_dq_kernel<DT, DP>), dim3((unsigned)(a->B * a->H) * pl.ntile), dim3(256), lds_q, st, p);
     ASR_CHECK_LAUNCH("battn_dq_kernel");
-    hipLaunchKernelGGL(battn_table_kernel, dim3(a->nb, a->H), dim3(64), 0, st, p.tpart, a->dtable, a->B, a->H, pl.ntile, a->nb);
+    if (p.tpart) hipLaunchKernelGGL(battn_table_kernel, dim3(a->nb, a->H), dim3(64), 0, st, p.tpart, a->dtable, a->B, a->H, pl.ntile, a->nb);
     ASR_CHECK(battn_lds(battn_dkv_kernel<DT, DP>, lds_k, "bucket_attention_bwd"));
     hipLaunchKernelGGL((battn_dkv_kernel<DT, DP>), dim3((unsigned)(a->B * a->Hk) * cdiv(a->Tk, 128) * pl.gsplit), dim3(256), lds_k, st, p);
     ASR_CHECK_LAUNCH("battn_dkv_kernel");
@@ -1165,7 +1168,7 @@ extern "C" int asr_bucket_attention_fwd(const asr_bucket_attention_args *a, void
 }
 extern "C" int asr_bucket_attention_bwd(const asr_bucket_attention_args *a, void *stream) {
     ASR_CHECK(battn_check(a, "bucket_attention_bwd", true));
-    ASR_CHECK_ARG(a->g && a->lse && a->dq && a->dk && a->dv && a->dtable && a->ws && (a->dtype == ASR_T_F32 ? a->out != nullptr : a->out32 != nullptr),
+    ASR_CHECK_ARG(a->g && a->lse && a->dq && a->dk && a->dv && (a->dtable || !a->table) && a->ws && (a->dtype == ASR_T_F32 ? a->out != nullptr : a->out32 != nullptr),
                   "bucket_attention_bwd: null pointer");
     return battn_any(a, true, stream);
 }

@@ -634,7 +634,8 @@ int asr_gated_ff_bwd(const asr_gated_ff_args *a, void *stream);
  * at j.  Buckets: nd = nb / 2 of them for each direction (causal: nb, for the past), the first nd / 2 hold one distance each,
  * edges_host[0 .. nd - nd/2 - 2] (HOST array, rising, <= 1024) are the distances at which the others begin; keys after the
  * query use the second half.  Keys j >= lengths[b] (NULL: Tk) and keys with keep[b,j] == 0 (NULL: all kept) are never read
- * into a result; a query that no key is left for gets zeros.  H % Hk == 0, D <= 128, nb <= 256.
+ * into a result; a query that no key is left for gets zeros.  table NULL: no bias (then dtable is not written; nb still says
+ * how distances would be cut, 4, or 2 if causal, is least work).  H % Hk == 0, D <= 128, nb <= 256.
  * _fwd: out (B,Tq,H,D) contiguous; train != 0 also writes lse (B,H,Tq) and, for 16-bit types, out32 (out in float32).
  * _bwd: g is the upstream gradient, dq / dk / dv contiguous, dtable (nb,H).  ws: asr_bucket_attention_ws_bytes(a, backward)
  * bytes (0: may be NULL; -1: refused).  Deterministic. */

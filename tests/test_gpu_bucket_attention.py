@@ -250,3 +250,19 @@ def test_refusals():
     big = torch.zeros(1, 1, 1, 129, device=DEV)
     with pytest.raises(RuntimeError):
         bucket_attention(big, big, big, torch.zeros(32, 1, device=DEV))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_without_a_table(causal):
+    from asr_amd.Models.transformer_ops import bucket_attention
+    q, k, v, up, t = _inputs(2, 200, 200, 4, 2, 64, torch.bfloat16)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    y = bucket_attention(*leaves, causal=causal)
+    grads = torch.autograd.grad(y, leaves, up)
+    want = attention64(q.double(), k.double(), v.double(), torch.zeros_like(t).double(), up.double(), torch.bfloat16, lengths=None, keep=None,
+                       offset=None, causal=causal, reach=128, scale=64 ** -0.5, train=True)
+    for got, w in zip((y.detach(), *grads), want):
+        held(got, w)
+    few = bucket_attention(q[:, :2], k, v)
+    held(few, attention64(q[:, :2].double(), k.double(), v.double(), torch.zeros_like(t).double(), None, torch.bfloat16, lengths=None, keep=None,
+                          offset=None, causal=False, reach=128, scale=64 ** -0.5, train=False)[0])
