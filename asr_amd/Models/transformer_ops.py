@@ -53,26 +53,31 @@ def _heads(t):
 
 
 # ----------------------------------------------------------------------------------------- norm and rotation --
-def _rope_args(q, k, wq, wk, pos, rot, base, eps):
+_ROPE = _lib.packer(_lib.RopeArgs)
+
+
+def _rope_call(fn, q, k, wq, wk, pos, rot, base, eps, gq, gk, qo, ko, dwq, dwk, ws):
     B, T, H, D = q.shape
-    a = _lib.RopeArgs()
-    a.q, a.k, a.wq, a.wk = q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr()
-    a.q_sb, a.q_st, a.q_sh, _ = q.stride()
-    a.k_sb, a.k_st, a.k_sh, _ = k.stride()
-    if pos is not None:
-        a.pos, a.pos_sb = pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0
-    a.B, a.T, a.H, a.Hk, a.D, a.rot, a.dtype = B, T, H, k.shape[2], D, rot, _DTYPES[q.dtype]
-    a.eps, a.base = eps, base
-    return a
+    qs, ks = q.stride(), k.stride()
+    if gq is None:
+        gqp = gkp = 0
+        gqs = gks = (0, 0, 0)
+    else:
+        gqp, gkp, gqs, gks = gq.data_ptr(), gk.data_ptr(), gq.stride(), gk.stride()
+    a = _ROPE.pack(q.data_ptr(), k.data_ptr(), gqp, gkp, wq.data_ptr(), wk.data_ptr(), 0 if pos is None else pos.data_ptr(),
+                   qo.data_ptr(), ko.data_ptr(), 0 if dwq is None else dwq.data_ptr(), 0 if dwk is None else dwk.data_ptr(),
+                   0 if ws is None else ws.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], gqs[0], gqs[1], gqs[2],
+                   gks[0], gks[1], gks[2], 0 if pos is None or pos.dim() == 1 else pos.stride(0), B, T, H, k.shape[2], D, rot,
+                   _DTYPES[q.dtype], eps, base)
+    device = q.device
+    with _on(device):
+        check(fn(a, _stream(device)))
 
 
 def _rope_fwd(q, k, wq, wk, pos, rot, base, eps):
     qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
     if qo.numel():
-        a = _rope_args(q, k, wq, wk, pos, rot, base, eps)
-        a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
-        with _on(q.device):
-            check(_lib.load().asr_qk_norm_rope_fwd(C.byref(a), _stream(q.device)))
+        _rope_call(_lib.load().asr_qk_norm_rope_fwd, q, k, wq, wk, pos, rot, base, eps, None, None, qo, ko, None, None, None)
     return qo, ko
 
 
@@ -82,15 +87,8 @@ def _rope_bwd(q, k, wq, wk, pos, rot, base, eps, gq, gk):
     dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
     if not q.numel():
         return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk)
-    gq, gk = _heads(gq), _heads(gk)
     dwq, dwk, ws = torch.empty_like(wq), torch.empty_like(wk), wq.new_empty(lib.asr_qk_norm_rope_ws_floats(q.shape[-1]))
-    a = _rope_args(q, k, wq, wk, pos, rot, base, eps)
-    a.gq, a.gk, a.q_out, a.k_out = gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr()
-    a.gq_sb, a.gq_st, a.gq_sh, _ = gq.stride()
-    a.gk_sb, a.gk_st, a.gk_sh, _ = gk.stride()
-    a.dwq, a.dwk, a.ws = dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr()
-    with _on(q.device):
-        check(lib.asr_qk_norm_rope_bwd(C.byref(a), _stream(q.device)))
+    _rope_call(lib.asr_qk_norm_rope_bwd, q, k, wq, wk, pos, rot, base, eps, _heads(gq), _heads(gk), dq, dk, dwq, dwk, ws)
     return dq, dk, dwq, dwk
 
 
@@ -178,33 +176,32 @@ def _edges_host(num_buckets, max_distance, causal):
     return (C.c_int32 * max(1, len(e)))(*e)
 
 
-def _attn_args(q, k, v, table, lengths, keep, offset, causal, reach, scale, train):
+_ATTN = _lib.packer(_lib.BucketAttentionArgs)
+_ATTN_WS = [n for n, _ in _lib.BucketAttentionArgs._fields_].index("ws")
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _attn_call(backward, q, k, v, table, lengths, keep, offset, causal, reach, scale, train, g, out, out32, lse, dq, dk, dv, dt):
+    lib = _lib.load()
     B, Tq, H, D = q.shape
-    a = _lib.BucketAttentionArgs()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    nb = 2 if causal else 4
-    if table is not None:
-        nb, a.table = table.shape[0], table.data_ptr()
-    a.edges_host = C.addressof(_edges_host(nb, reach, causal))
-    if lengths is not None:
-        a.lengths = lengths.data_ptr()
-    if offset is not None:
-        a.offset = offset.data_ptr()
-    if keep is not None:
-        a.keep = keep.data_ptr()
-    a.q_sb, a.q_st, a.q_sh, _ = q.stride()
-    a.k_sb, a.k_st, a.k_sh, _ = k.stride()
-    a.v_sb, a.v_st, a.v_sh, _ = v.stride()
-    a.B, a.Tq, a.Tk, a.H, a.Hk, a.D = B, Tq, k.shape[1], H, k.shape[2], D
-    a.nb, a.causal, a.dtype, a.train, a.scale = nb, int(causal), _DTYPES[q.dtype], int(train), scale
-    return a
-
-
-def _attn_workspace(lib, a, backward, device):
-    n = int(lib.asr_bucket_attention_ws_bytes(C.byref(a), int(backward)))
-    if n < 0:
-        check(-1)
-    return torch.empty(n, device=device, dtype=torch.uint8)
+    nb = table.shape[0] if table is not None else 2 if causal else 4
+    qs, ks, vs, gs = q.stride(), k.stride(), v.stride(), (0, 0, 0) if g is None else g.stride()
+    a = [q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(g), _ptr(table), C.addressof(_edges_host(nb, reach, causal)), _ptr(lengths),
+         _ptr(offset), _ptr(keep), _ptr(out), _ptr(out32), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dt), 0, qs[0], qs[1],
+         qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], gs[0], gs[1], gs[2], B, Tq, k.shape[1], H, k.shape[2], D, nb, causal,
+         _DTYPES[q.dtype], train, scale]
+    device = q.device
+    with _on(device):
+        n = lib.asr_bucket_attention_ws_bytes(_ATTN.pack(*a), backward)
+        if n < 0:
+            check(-1)
+        if n:
+            ws = torch.empty(n, device=device, dtype=torch.uint8)
+            a[_ATTN_WS] = ws.data_ptr()
+        check((lib.asr_bucket_attention_bwd if backward else lib.asr_bucket_attention_fwd)(_ATTN.pack(*a), _stream(device)))
 
 
 def _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, train):
@@ -212,39 +209,21 @@ def _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, train
     out = q.new_empty(q.shape)
     if not out.numel() or not k.shape[1]:
         return out.zero_(), None, None
-    lib = _lib.load()
-    a = _attn_args(q, k, v, table, lengths, keep, offset, causal, reach, scale, train)
-    a.out = out.data_ptr()
     lse = out32 = None
     if train:
         lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device, dtype=torch.float32)
         out32 = out if q.dtype == torch.float32 else torch.empty(q.shape, device=q.device, dtype=torch.float32)
-        a.lse, a.out32 = lse.data_ptr(), out32.data_ptr()
-    with _on(q.device):
-        ws = _attn_workspace(lib, a, False, q.device)
-        a.ws = ws.data_ptr()
-        check(lib.asr_bucket_attention_fwd(C.byref(a), _stream(q.device)))
+    _attn_call(0, q, k, v, table, lengths, keep, offset, causal, reach, scale, train, None, out, out32, lse, None, None, None, None)
     return out, lse, out32
 
 
 def _attn_bwd(q, k, v, table, lengths, keep, offset, lse, out32, causal, reach, scale, g):
     """Gradients of q, k, v and the table (None without one)."""
-    dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     dt = torch.empty_like(table) if table is not None else None
     if not q.numel() or not k.shape[1]:
         return tuple(t.zero_() if t is not None else None for t in (dq, dk, dv, dt))
-    lib = _lib.load()
-    g = _heads(g)
-    a = _attn_args(q, k, v, table, lengths, keep, offset, causal, reach, scale, True)
-    a.g, a.lse, a.out32, a.out = g.data_ptr(), lse.data_ptr(), out32.data_ptr(), out32.data_ptr()
-    a.g_sb, a.g_st, a.g_sh, _ = g.stride()
-    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    if dt is not None:
-        a.dtable = dt.data_ptr()
-    with _on(q.device):
-        ws = _attn_workspace(lib, a, True, q.device)
-        a.ws = ws.data_ptr()
-        check(lib.asr_bucket_attention_bwd(C.byref(a), _stream(q.device)))
+    _attn_call(1, q, k, v, table, lengths, keep, offset, causal, reach, scale, True, _heads(g), out32, out32, lse, dq, dk, dv, dt)
     return dq, dk, dv, dt
 
 
@@ -321,31 +300,28 @@ def bucket_attention(q, k, v, table=None, lengths=None, keep=None, offset=None, 
 ACTIVATIONS = {"swish": 0, "gelu": 1}
 
 
-def _ff_args(x2, wg, wu, wd, act):
-    a = _lib.GatedFFArgs()
-    a.x, a.wg, a.wu, a.wd = x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr()
-    a.M, a.d = x2.shape
-    a.f, a.n, a.dtype, a.act = wg.shape[0], wd.shape[0], _DTYPES[x2.dtype], act
-    return a
+_FF = _lib.packer(_lib.GatedFFArgs)
 
 
-def _ff_workspace(lib, a, backward, device):
-    n = int(lib.asr_gated_ff_ws_bytes(C.byref(a), int(backward)))
-    if n < 0:
-        check(-1)
-    return torch.empty(n, device=device, dtype=torch.uint8)
+def _ff_call(backward, x2, wg, wu, wd, act, dy, y, dx, dwg, dwu, dwd):
+    lib = _lib.load()
+    M, d = x2.shape
+    a = [x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), _ptr(dy), _ptr(y), _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd), 0,
+         M, d, wg.shape[0], wd.shape[0], _DTYPES[x2.dtype], act]
+    device = x2.device
+    with _on(device):
+        n = lib.asr_gated_ff_ws_bytes(_FF.pack(*a), backward)
+        if n < 0:
+            check(-1)
+        ws = torch.empty(n, device=device, dtype=torch.uint8)
+        a[10] = ws.data_ptr()
+        check((lib.asr_gated_ff_bwd if backward else lib.asr_gated_ff_fwd)(_FF.pack(*a), _stream(device)))
 
 
 def _ff_fwd(x2, wg, wu, wd, act):
     y = x2.new_empty(x2.shape[0], wd.shape[0])
     if y.shape[0]:
-        lib = _lib.load()
-        a = _ff_args(x2, wg, wu, wd, act)
-        a.y = y.data_ptr()
-        with _on(x2.device):
-            ws = _ff_workspace(lib, a, False, x2.device)
-            a.ws = ws.data_ptr()
-            check(lib.asr_gated_ff_fwd(C.byref(a), _stream(x2.device)))
+        _ff_call(0, x2, wg, wu, wd, act, None, y, None, None, None, None)
     return y
 
 
@@ -353,20 +329,10 @@ def _ff_bwd(x2, wg, wu, wd, act, dy, need=(True, True, True, True)):
     """Gradients of x2 and the three weights, None for what `need` leaves out (the two first weights come together)."""
     if not x2.shape[0]:
         return torch.zeros_like(x2), torch.zeros_like(wg), torch.zeros_like(wu), torch.zeros_like(wd)
-    lib = _lib.load()
-    dy = dy.contiguous()
-    a = _ff_args(x2, wg, wu, wd, act)
-    a.dy = dy.data_ptr()
     dx = torch.empty_like(x2) if need[0] else None
     dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need[1] or need[2] else (None, None)
     dwd = torch.empty_like(wd) if need[3] else None
-    for n, t in (("dx", dx), ("dwg", dwg), ("dwu", dwu), ("dwd", dwd)):
-        if t is not None:
-            setattr(a, n, t.data_ptr())
-    with _on(x2.device):
-        ws = _ff_workspace(lib, a, True, x2.device)
-        a.ws = ws.data_ptr()
-        check(lib.asr_gated_ff_bwd(C.byref(a), _stream(x2.device)))
+    _ff_call(1, x2, wg, wu, wd, act, dy.contiguous(), None, dx, dwg, dwu, dwd)
     return dx, dwg, dwu, dwd
 
 

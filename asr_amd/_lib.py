@@ -6,6 +6,7 @@ module raises -- there is no CPU or eager-PyTorch fallback anywhere in
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libasr_amd.so")
@@ -75,6 +76,15 @@ class AttDecBwdArgs(C.Structure):
         ("ws", c_f),
         ("defer_tail", C.c_int),
     ]
+
+
+def packer(cls):
+    """struct.Struct that writes a ctypes structure's bytes from its values in order, for calls whose host time matters (a third
+    of setting the fields one by one); a function whose argument is declared as a pointer (c_void_p) takes the bytes."""
+    codes = {C.c_void_p: "P", C.c_int64: "q", C.c_int: "i", C.c_float: "f", C.c_double: "d"}
+    s = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
+    pad = C.sizeof(cls) - s.size                    # what the compiler leaves behind the last field
+    return s if pad == 0 else struct.Struct(s.format + "%dx" % pad)
 
 
 class RopeArgs(C.Structure):
@@ -197,14 +207,14 @@ SYMBOLS = {
     "asr_col2im_3x3s2_dw": (C.c_int, [c_f, c_f, c_f, C.c_int, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
     # encoder-layer operators (csrc/rope.hip, gated_ff.hip, bucket_attn.hip)
     "asr_qk_norm_rope_ws_floats": (c_i64, [C.c_int]),
-    "asr_qk_norm_rope_fwd": (C.c_int, [C.POINTER(RopeArgs), c_f]),
-    "asr_qk_norm_rope_bwd": (C.c_int, [C.POINTER(RopeArgs), c_f]),
-    "asr_gated_ff_ws_bytes": (c_i64, [C.POINTER(GatedFFArgs), C.c_int]),
-    "asr_gated_ff_fwd": (C.c_int, [C.POINTER(GatedFFArgs), c_f]),
-    "asr_gated_ff_bwd": (C.c_int, [C.POINTER(GatedFFArgs), c_f]),
-    "asr_bucket_attention_ws_bytes": (c_i64, [C.POINTER(BucketAttentionArgs), C.c_int]),
-    "asr_bucket_attention_fwd": (C.c_int, [C.POINTER(BucketAttentionArgs), c_f]),
-    "asr_bucket_attention_bwd": (C.c_int, [C.POINTER(BucketAttentionArgs), c_f]),
+    "asr_qk_norm_rope_fwd": (C.c_int, [c_f, c_f]),
+    "asr_qk_norm_rope_bwd": (C.c_int, [c_f, c_f]),
+    "asr_gated_ff_ws_bytes": (c_i64, [c_f, C.c_int]),
+    "asr_gated_ff_fwd": (C.c_int, [c_f, c_f]),
+    "asr_gated_ff_bwd": (C.c_int, [c_f, c_f]),
+    "asr_bucket_attention_ws_bytes": (c_i64, [c_f, C.c_int]),
+    "asr_bucket_attention_fwd": (C.c_int, [c_f, c_f]),
+    "asr_bucket_attention_bwd": (C.c_int, [c_f, c_f]),
 }
 
 _lib = None
