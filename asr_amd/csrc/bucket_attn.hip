@@ -494,10 +494,10 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
                 // lane's diagonal of rows u: distance j + 16 u + t - 31 - (pmin .. ) where t = key row - query column + 31
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    wave_sync();
 #pragma unroll
                     for (int r = 0; r < 8; ++r) patch[row_of(r, half) * PATCH + 16 + (lane & 31)] = s[0][8 * u + r];
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    wave_sync();
                     if (lane < 47) {
                         float a = 0.f;
 #pragma unroll
@@ -506,7 +506,7 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
                         *d += a;
                     }
                 }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                wave_sync();
             }
             bf16x8 df[NP][2];
             to_operand<NP>(df, s[0]);
@@ -779,7 +779,7 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
 #pragma unroll
                 for (int q = t; q >= 0; --q) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[q], qf[t - q][ks], s[0], 0, 0, 0);
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
 #pragma unroll
         for (int ks = 0; ks < NC; ++ks) {
             bf16x8 w[NP];
@@ -789,8 +789,7 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
             for (int q = 0; q < NP; ++q)
                 *reinterpret_cast<u32x4p *>(pool + q * IMG + img_at<DP>(f / CH, f % CH)) = vok[ks] ? __builtin_bit_cast(u32x4p, w[q]) : u32x4p{0u, 0u, 0u, 0u};
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         if (j0 + 32 < je) load(j0 + 32);
         if (j0 + 31 - pmin <= -R || j0 - pmax >= R) {
             const float bf = j0 - pmax >= R ? br : bl;
@@ -831,7 +830,7 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
         bf16x8 pf[NP][2];
         to_operand<NP>(pf, s[0]);
         dot_cols<NP, NP, DP>(o, pool, IMG, 0, pf, lane);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        wave_sync();
     }
     l += __shfl_xor(l, 32, 64);
     if (col >= rows) return;

@@ -305,14 +305,13 @@ __device__ __forceinline__ void zero_acc(f32x16 (&acc)[TM][TN]) {
 template <typename F>
 __device__ __forceinline__ void turn_tile(const f32x16 &t, float *S, F put) {
     const int lane = threadIdx.x & 63;
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
 #pragma unroll
     for (int r = 0; r < 16; ++r) S[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * 32 + (lane & 31)] = t[r];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
 #pragma unroll
     for (int p = 0; p < 4; ++p) put(p * 8 + (lane >> 3), (lane & 7) * 4, *reinterpret_cast<const float4 *>(&S[(p * 8 + (lane >> 3)) * 32 + (lane & 7) * 4]));
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    wave_sync();
 }
 
 template <int NP>

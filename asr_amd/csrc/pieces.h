@@ -94,3 +94,12 @@ __device__ __forceinline__ void split_pair_finite(float a, float b, unsigned (&w
     }
     if constexpr (NP > 2) w[2] = pk_bf16(a - __uint_as_float(w[1] << 16), b - __uint_as_float(w[1] & 0xffff0000u));
 }
+
+// What this wave's lanes wrote to LDS is seen by its other lanes.  The barrier costs no instruction, but without it the
+// fences order the accesses of one lane only: the compiler may let the lanes that skip a branch run ahead of those that
+// take it, and overwrite what these have yet to read.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
