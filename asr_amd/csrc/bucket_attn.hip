@@ -236,6 +236,53 @@ __device__ __forceinline__ void dot_cols(f32x16 (&acc)[DP / 32], const unsigned 
                     if (s - q >= 0 && s - q < W) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[q], o[s - q][c], acc[t], 0, 0, 0);
         }
 }
+// The same two products in two parts, so that the fragments of one can be read under the other's matrix instructions: with
+// one wave a SIMD every read that is waited for right away costs its whole latency (dK and dV of the long bfloat16 case: 41
+// such waits a tile, half of its time)
+template <int NP, int DP>
+struct RowFrags {
+    bf16x8 f[NP][DP / 16];
+    __device__ __forceinline__ void read(const unsigned char *img, int imgsz, int r0, int lane) {
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+            for (int q = 0; q < NP; ++q) f[q][ks] = frag_rows<DP>(img + q * imgsz, r0, ks, lane);
+    }
+    __device__ __forceinline__ void dot(f32x16 &t, const bf16x8 (&own)[NP][DP / 16]) const {
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+            for (int s = NP - 1; s >= 0; --s)
+#pragma unroll
+                for (int q = s; q >= 0; --q) t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[q][ks], own[s - q][ks], t, 0, 0, 0);
+    }
+};
+template <int NP, int DP>
+struct ColFrags {
+    bf16x8 f[NP][2][DP / 32];
+    __device__ __forceinline__ void read(const unsigned char *img, int imgsz, int r0, int lane) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int q = 0; q < NP; ++q) f[q][c][t] = frag_cols<DP>(img + q * imgsz, r0, c, t * 32, lane);
+    }
+    template <int W>
+    __device__ __forceinline__ void dot(f32x16 (&acc)[DP / 32], const bf16x8 (&o)[W][2]) const {
+        constexpr int TOP = (NP > W ? NP : W) - 1;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int s = TOP; s >= 0; --s)
+#pragma unroll
+                for (int q = 0; q < NP; ++q)
+#pragma unroll
+                    for (int t = 0; t < DP / 32; ++t)
+                        if (s - q >= 0 && s - q < W) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[q][c][t], o[s - q][c], acc[t], 0, 0, 0);
+    }
+};
+#define PHASE() __builtin_amdgcn_sched_barrier(0)
 __device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
 // 16 scores of a 32 x 32 tile in base 2: scale and bias added; `first`: distance of register 0 (row 4 half) for this lane,
@@ -614,38 +661,68 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 
                     gt.load(t0 + QT, p.Tq, p.D, nullptr);
                     load_stat(t0 + QT);
                 }
-#pragma unroll 1
-                for (int s0 = 0; s0 < QT; s0 += 32) {
-                    const int i = t0 + s0, pmin = off + i, pmax = pmin + 31;
-                    if (i >= p.Tq) break;
-                    if (jw >= n || (p.bk.causal && jw > pmax)) continue;
-                    f32x16 s[2];
-                    zero16(s);
-                    dot_rows<NP, DP>(s[0], qi, Tile::IMG, s0, kf, lane);
-                    dot_rows<NP, DP>(s[1], gi, Tile::IMG, s0, vf, lane);
-                    add_bias<-1>(s[0], c, lut, R, j - (pmin + 4 * half), jw - pmax, jw + 31 - pmin);
-                    // (a key that is left out collects what it likes in its own column and is stored as zeros)
+                // (a key that is left out collects what it likes in its own column and is stored as zeros)
+                auto weigh = [&](f32x16 &s, int s0) {                                  // scores -> probabilities
+                    const int pmin = off + t0 + s0;
+                    add_bias<-1>(s, c, lut, R, j - (pmin + 4 * half), jw - (pmin + 31), jw + 31 - pmin);
                     if (p.bk.causal && jw + 31 > pmin) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[0][r] = j <= pmin + row_of(r, half) ? s[0][r] : -INFINITY;
+                        for (int r = 0; r < 16; ++r) s[r] = j <= pmin + row_of(r, half) ? s[r] : -INFINITY;
                     }
 #pragma unroll
                     for (int r4 = 0; r4 < 4; ++r4) {
-                        const float4 ls = *reinterpret_cast<const float4 *>(stat + s0 + 8 * r4 + 4 * half);
-                        const float4 dl = *reinterpret_cast<const float4 *>(stat + QT + s0 + 8 * r4 + 4 * half);
-                        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dd[4] = {dl.x, dl.y, dl.z, dl.w};
+                        const f32x4 ls = *reinterpret_cast<const f32x4 *>(stat + s0 + 8 * r4 + 4 * half);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int r = 4 * r4 + e;
-                            s[0][r] = __builtin_amdgcn_exp2f(s[0][r] - lv[e]);
-                            s[1][r] = s[0][r] * (s[1][r] - dd[e]);
-                        }
+                        for (int e = 0; e < 4; ++e) s[4 * r4 + e] = __builtin_amdgcn_exp2f(s[4 * r4 + e] - ls[e]);
                     }
+                };
+                auto slope = [&](f32x16 &dp, const f32x16 &s, int s0) {                // dP -> dS
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4) {
+                        const f32x4 dl = *reinterpret_cast<const f32x4 *>(stat + QT + s0 + 8 * r4 + 4 * half);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dp[4 * r4 + e] = s[4 * r4 + e] * (dp[4 * r4 + e] - dl[e]);
+                    }
+                };
+#pragma unroll 1
+                for (int s0 = 0; s0 < QT; s0 += 32) {
+                    const int i = t0 + s0, pmax = off + i + 31;
+                    if (i >= p.Tq) break;
+                    if (jw >= n || (p.bk.causal && jw > pmax)) continue;
+                    f32x16 s[1], dp[1];
+                    zero16(s);
+                    zero16(dp);
                     bf16x8 f[NP][2];
-                    to_operand<NP>(f, s[0]);
-                    dot_cols<NP, NP, DP>(dv, gi, Tile::IMG, s0, f, lane);
-                    to_operand<NP>(f, s[1]);
-                    dot_cols<NP, NP, DP>(dk, qi, Tile::IMG, s0, f, lane);
+                    if constexpr (NP == 1) {
+                        RowFrags<NP, DP> qr, gr;
+                        ColFrags<NP, DP> gc, qc;
+                        PHASE();
+                        qr.read(qi, Tile::IMG, s0, lane);
+                        PHASE();
+                        gr.read(gi, Tile::IMG, s0, lane);
+                        qr.dot(s[0], kf);
+                        PHASE();
+                        gc.read(gi, Tile::IMG, s0, lane);
+                        gr.dot(dp[0], vf);
+                        weigh(s[0], s0);
+                        to_operand<NP>(f, s[0]);
+                        PHASE();
+                        qc.read(qi, Tile::IMG, s0, lane);
+                        gc.dot(dv, f);
+                        slope(dp[0], s[0], s0);
+                        to_operand<NP>(f, dp[0]);
+                        PHASE();
+                        qc.dot(dk, f);
+                    } else {
+                        dot_rows<NP, DP>(s[0], qi, Tile::IMG, s0, kf, lane);
+                        dot_rows<NP, DP>(dp[0], gi, Tile::IMG, s0, vf, lane);
+                        weigh(s[0], s0);
+                        to_operand<NP>(f, s[0]);
+                        dot_cols<NP, NP, DP>(dv, gi, Tile::IMG, s0, f, lane);
+                        slope(dp[0], s[0], s0);
+                        to_operand<NP>(f, dp[0]);
+                        dot_cols<NP, NP, DP>(dk, qi, Tile::IMG, s0, f, lane);
+                    }
                 }
             }
         }
