@@ -770,15 +770,23 @@ __global__ __launch_bounds__(256) void battn_kvsum_kernel(const float *__restric
 // The keys of a (utterance, key head) are cut into nsplit runs, one wave each; the G query heads of the group times the
 // queries are the tile's 32 columns, so the cache is read once.  A lane loads K as rows (16 bytes of its own key at a time,
 // the left operand as it lies) and V as whole lines for the wave's LDS image; the next 32 keys are in flight under the
-// current ones.  float32 and float16 caches are split into pieces in registers.  Bound: the cache's bytes.
+// current ones: K from where its registers are free, V from where it lies in LDS.  float32 and float16 caches are split into
+// pieces in registers.  Only a run that comes near its queries builds the table of buckets, over its own distances.
+// Bound: the cache's bytes.  16 caches of 4096 to 8192 frames, 16 heads on 2 of 128, bfloat16 (102 MB): 26 us, 3.9 TB/s.
+// Registers decide: what spills is reloaded behind the loads in flight and waits for them (36 us with the queries and the LDS
+// addresses kept in registers, an index product a load, and a check of D a word).  With one piece the queries therefore lie
+// in LDS and the addresses are formed in the loop.  K as whole lines through LDS, like V: 42 against 36 us.
 // battn_join_kernel joins the runs.
-template <int DT, int DP, bool VEC>
+template <int DT, int DP, int MODE>
 __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_kernel(AttnParams p) {
+    constexpr bool VEC = MODE > 0, FULL = MODE == 2;                                   // rows of 16-byte words; D = DP
+    constexpr bool QL = ElemOf<DT>::NP == 1;                                           // the queries are read from LDS
     constexpr int NP = ElemOf<DT>::NP, IMG = 32 * 2 * DP, CH = DP / 8, NC = DP / 16;
     typedef typename ElemOf<DT>::type E;
     constexpr int W = (int)sizeof(E) / 2;                                              // 16-byte words of eight elements
     extern __shared__ __attribute__((aligned(16))) unsigned char pool[];
-    float *tab = reinterpret_cast<float *>(pool + NP * IMG);                           // [nb][G] biases of the group's heads
+    unsigned char *qi = pool + NP * IMG;
+    float *tab = reinterpret_cast<float *>(qi + (QL ? IMG : 0));                         // [nb][G] biases of the group's heads
     uint8_t *slot = reinterpret_cast<uint8_t *>(tab + p.bk.nb * p.G);                  // bucket by distance, -R - PAD .. R + PAD
     __shared__ int16_t edge[MAX_EDGES];
     const int lane = threadIdx.x, half = lane >> 5, col = lane & 31;
@@ -795,7 +803,7 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
         Raw r;
         if constexpr (VEC) {
 #pragma unroll
-            for (int u = 0; u < W; ++u) r.w[u] = d < p.D ? reinterpret_cast<const u32x4p *>(a + d)[u] : u32x4p{0u, 0u, 0u, 0u};
+            for (int u = 0; u < W; ++u) r.w[u] = FULL || d < p.D ? reinterpret_cast<const u32x4p *>(a + d)[u] : u32x4p{0u, 0u, 0u, 0u};
         } else {
             E t[8];
 #pragma unroll
@@ -824,41 +832,61 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
     };
     const E *kb = (const E *)p.kraw + b * p.k.sb + (int64_t)hk * p.k.sh, *vb = (const E *)p.vraw + b * p.v.sb + (int64_t)hk * p.v.sh;
     Raw kr[NC], vr[NC];
-    bool vok[NC];
-    auto load = [&](int j0) {
+    unsigned vok = 0;                                                                  // by c, where a key of the 32 may be left out
+    auto load_k = [&](int j0) {
         const E *k = kb + (int64_t)min(j0 + col, je - 1) * p.k.st;
 #pragma unroll
         for (int c = 0; c < NC; ++c) kr[c] = raw8(k, 16 * c + 8 * half);
+    };
+    auto load_v = [&](int j0) {
+        if (64 % CH == 0 && j0 + 32 <= je && keep == nullptr) {                        // one product of indexes instead of one a load
+            const E *v = vb + (int64_t)(j0 + lane / CH) * p.v.st;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int f = lane + 64 * c, j = j0 + f / CH;
-            vok[c] = j < je && (keep == nullptr || keep[j]);
-            vr[c] = raw8(vb + (int64_t)min(j, je - 1) * p.v.st, f % CH * 8);
+            for (int c = 0; c < NC; ++c) vr[c] = raw8(v + c * (64 / CH) * p.v.st, lane % CH * 8);
+        } else {
+            vok = 0;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int f = lane + 64 * c, j = j0 + f / CH;
+                vok |= (j < je && (keep == nullptr || keep[j])) << c;
+                vr[c] = raw8(vb + (int64_t)min(j, je - 1) * p.v.st, f % CH * 8);
+            }
         }
     };
-    if (jb < je) load(jb);
-    bf16x8 qf[NP][NC];
+    if (jb < je) {
+        load_k(jb);
+        load_v(jb);
+    }
+    bf16x8 qf[QL ? 1 : NP][QL ? 1 : NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         bf16x8 w[NP];
         pieces8(raw8((const E *)p.qraw + b * p.q.sb + (int64_t)i * p.q.st + h * p.q.sh, 16 * c + 8 * half), w);
 #pragma unroll
-        for (int q = 0; q < NP; ++q) qf[q][c] = w[q];
+        for (int q = 0; q < NP; ++q)
+            if constexpr (QL) *reinterpret_cast<u32x4p *>(qi + q * IMG + img_at<DP>(col, 2 * c + half)) = __builtin_bit_cast(u32x4p, w[q]);
+            else qf[q][c] = w[q];
     }
+    wave_sync();
     const int pmin = off, pmax = off + p.Tq - 1;
     const bool near = !(je - 1 - pmin <= -R || jb - pmax >= R);                        // some key of the run within the last edge
-    for (int t = lane; t < p.bk.nb * p.G; t += 64) tab[t] = p.table ? p.table[(t / p.G) * p.H + hk * p.G + t % p.G] * LOG2E : 0.f;
-    for (int t = lane; t < p.bk.nedge; t += 64) edge[t] = p.bk.edge[t];
-    __syncthreads();
-    if (near)
-        for (int t = lane; t < 2 * (R + LUT_PAD) + 1; t += 64) slot[t] = (uint8_t)bucket_of(p.bk, edge, min(max(t - R - LUT_PAD, -R), R));
-    __syncthreads();
+    const float bl = p.table ? p.table[(p.bk.nd - 1) * p.H + h] * LOG2E : 0.f;
+    const float br = p.table ? p.table[(p.bk.causal ? 0 : p.bk.nb - 1) * p.H + h] * LOG2E : 0.f;
+    if (near) {
+        for (int t = lane; t < p.bk.nb * p.G; t += 64) tab[t] = p.table ? p.table[(t / p.G) * p.H + hk * p.G + t % p.G] * LOG2E : 0.f;
+        for (int t = lane; t < p.bk.nedge; t += 64) edge[t] = p.bk.edge[t];
+        __syncthreads();
+        const int lo = max(jb - pmax, -R), hi = min(je + 31 - pmin, R);                // the run's distances
+        for (int t = lo + lane; t <= hi; t += 64) slot[t + R + LUT_PAD] = (uint8_t)bucket_of(p.bk, edge, t);
+        __syncthreads();
+    }
     f32x16 o[DP / 32];
     zero16(o);
     float m = -INFINITY, ms = 0.f, l = 0.f;
     const float c = p.scale * LOG2E;
-    const float bl = tab[(p.bk.nd - 1) * p.G + g], br = tab[(p.bk.causal ? 0 : p.bk.nb - 1) * p.G + g];
     for (int j0 = jb; j0 < je; j0 += 32) {
+        int ln = lane;                                                                 // LDS addresses are formed in the loop: kept, they spill
+        asm volatile("" : "+v"(ln));
         f32x16 s[1];
         zero16(s);
 #pragma unroll
@@ -868,20 +896,30 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
 #pragma unroll
             for (int t = NP - 1; t >= 0; --t)
 #pragma unroll
-                for (int q = t; q >= 0; --q) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[q], qf[t - q][ks], s[0], 0, 0, 0);
+                for (int q = t; q >= 0; --q) {
+                    bf16x8 x;
+                    if constexpr (QL) x = frag_rows<DP>(qi + (t - q) * IMG, 0, ks, ln);
+                    else x = qf[t - q][ks];
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[q], x, s[0], 0, 0, 0);
+                }
         }
+        if (j0 + 32 < je) load_k(j0 + 32);
         wave_sync();
+        const bool whole = j0 + 32 <= je && keep == nullptr;
 #pragma unroll
         for (int ks = 0; ks < NC; ++ks) {
             bf16x8 w[NP];
             pieces8(vr[ks], w);
-            const int f = lane + 64 * ks;
+            const int f = ln + 64 * ks;
 #pragma unroll
             for (int q = 0; q < NP; ++q)
-                *reinterpret_cast<u32x4p *>(pool + q * IMG + img_at<DP>(f / CH, f % CH)) = vok[ks] ? __builtin_bit_cast(u32x4p, w[q]) : u32x4p{0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4p *>(pool + q * IMG + img_at<DP>(f / CH, f % CH)) =
+                    whole || (vok >> ks & 1) ? __builtin_bit_cast(u32x4p, w[q]) : u32x4p{0u, 0u, 0u, 0u};
         }
         wave_sync();
-        if (j0 + 32 < je) load(j0 + 32);
+        if (j0 + 32 < je) {
+            load_v(j0 + 32);
+        }
         if (j0 + 31 - pmin <= -R || j0 - pmax >= R) {
             const float bf = j0 - pmax >= R ? br : bl;
 #pragma unroll
@@ -920,18 +958,18 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
         }
         bf16x8 pf[NP][2];
         to_operand<NP>(pf, s[0]);
-        dot_cols<NP, NP, DP>(o, pool, IMG, 0, pf, lane);
+        dot_cols<NP, NP, DP>(o, pool, IMG, 0, pf, ln);
         wave_sync();
     }
     l += __shfl_xor(l, 32, 64);
     if (col >= rows) return;
     if (p.nsplit == 1) {
         const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        put_acc<E, DP>((E *)p.out + (((int64_t)b * p.Tq + i) * p.H + h) * p.D, o, f, p.D, half);
+        put_acc<E, DP>((E *)p.out + (((int64_t)b * p.Tq + i) * p.H + h) * p.D, o, f, FULL ? DP : p.D, half);
         return;
     }
     const int64_t at = ((int64_t)bhk * p.nsplit + sp) * rows + col;
-    put_acc<float, DP>(p.po + at * p.D, o, 1.f, p.D, half);
+    put_acc<float, DP>(p.po + at * p.D, o, 1.f, FULL ? DP : p.D, half);
     if (half == 0) {
         p.pml[2 * at] = m == -INFINITY ? -INFINITY : ms;
         p.pml[2 * at + 1] = l;
@@ -1167,10 +1205,10 @@ static int battn_fwd(const asr_bucket_attention_args *a, hipStream_t st) {
         const int64_t rows = (int64_t)p.G * p.Tq * a->B * a->Hk;
         p.po = (float *)a->ws;
         p.pml = p.po + rows * p.nsplit * a->D;
-        const size_t lds = NP * 32 * 2 * DP + sizeof(float) * p.bk.nb * p.G + (2 * (p.bk.R + LUT_PAD) + 1);
-        ASR_CHECK(vec ? battn_lds(battn_few_kernel<DT, DP, true>, lds, "bucket_attention_fwd") : battn_lds(battn_few_kernel<DT, DP, false>, lds, "bucket_attention_fwd"));
-        if (vec) hipLaunchKernelGGL((battn_few_kernel<DT, DP, true>), dim3(a->B * a->Hk, p.nsplit), dim3(64), lds, st, p);
-        else hipLaunchKernelGGL((battn_few_kernel<DT, DP, false>), dim3(a->B * a->Hk, p.nsplit), dim3(64), lds, st, p);
+        const size_t lds = (NP == 1 ? 2 : NP) * 32 * 2 * DP + sizeof(float) * p.bk.nb * p.G + (2 * (p.bk.R + LUT_PAD) + 1);
+        const auto few = !vec ? battn_few_kernel<DT, DP, 0> : a->D < DP ? battn_few_kernel<DT, DP, 1> : battn_few_kernel<DT, DP, 2>;
+        ASR_CHECK(battn_lds(few, lds, "bucket_attention_fwd"));
+        hipLaunchKernelGGL(few, dim3(a->B * a->Hk, p.nsplit), dim3(64), lds, st, p);
         if (p.nsplit > 1) hipLaunchKernelGGL((battn_join_kernel<DT>), dim3((unsigned)rows), dim3(128), 0, st, p);
         ASR_CHECK_LAUNCH("battn_few_kernel");
         return ASR_OK;
