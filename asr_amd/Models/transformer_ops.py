@@ -256,8 +256,8 @@ def bucket_attention(q, k, v, table=None, lengths=None, keep=None, offset=None, 
     ``causal`` a query reads only the keys up to its own position and all buckets are for the past, otherwise the second half
     of the buckets is for the keys behind the query.  Keys from ``lengths[b]`` on and keys with ``keep[b, j]`` false are left
     out, whatever they hold (infinities and NaN too); a query that no key is left for gets zeros, and passes no gradient.
-    D at most 128, num_buckets at most 256, max_distance at most 1024.  Without gradients, calls of at most 32 query
-    rows a key head (Tq H / Hk: one new frame against a cache) split the keys over the GPU."""
+    D at most 128, num_buckets at most 256, max_distance at most 1024.  Without gradients, calls with few queries
+    (one new frame against a cache, one utterance at a time) split the keys over the GPU."""
     who = "bucket_attention"
     _tensor(who, "q", q, 4)
     _tensor(who, "k", k, 4, like=q)

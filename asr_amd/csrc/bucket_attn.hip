@@ -766,12 +766,14 @@ __global__ __launch_bounds__(256) void battn_kvsum_kernel(const float *__restric
     }
 }
 
-// -------------------------------------------------------------------- a few queries against a long cache, forward --
-// The keys of a (utterance, key head) are cut into nsplit runs, one wave each; the G query heads of the group times the
-// queries are the tile's 32 columns, so the cache is read once.  A lane loads K as rows (16 bytes of its own key at a time,
+// ------------------------------------------------------------------------- few queries against many keys, forward --
+// The keys of a (utterance, key head) are cut into nsplit runs, one wave each for 32 of the queries; a query's G heads of the
+// group are neighbouring columns of the tile, so for single tokens the cache is read once.  A lane loads K as rows (16 bytes of its own key at a time,
 // the left operand as it lies) and V as whole lines for the wave's LDS image; the next 32 keys are in flight under the
 // current ones: K from where its registers are free, V from where it lies in LDS.  float32 and float16 caches are split into
 // pieces in registers.  Only a run that comes near its queries builds the table of buckets, over its own distances.
+// A tile's masked keys are one ballot (a byte of the mask a row and element waited for each other: 16 against 12 us for one
+// utterance of 150 frames, 4 heads of 40, float16; of these 5 go into the launch, the first loads and the bucket table).
 // Bound: the cache's bytes.  16 caches of 4096 to 8192 frames, 16 heads on 2 of 128, bfloat16 (102 MB): 26 us, 3.9 TB/s.
 // Registers decide: what spills is reloaded behind the loads in flight and waits for them (36 us with the queries and the LDS
 // addresses kept in registers, an index product a load, and a check of D a word).  With one piece the queries therefore lie
@@ -791,10 +793,11 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
     __shared__ int16_t edge[MAX_EDGES];
     const int lane = threadIdx.x, half = lane >> 5, col = lane & 31;
     const int bhk = blockIdx.x, b = bhk / p.Hk, hk = bhk - b * p.Hk, sp = blockIdx.y;
-    const int rows = p.G * p.Tq, R = p.bk.R, off = p.offset ? p.offset[b] : 0;
-    const int cc = min(col, rows - 1), g = cc % p.G, i = cc / p.G, h = hk * p.G + g, pos = off + i;
+    const int r0 = blockIdx.z * 32, r1 = min(r0 + 32, p.G * p.Tq) - 1, R = p.bk.R, off = p.offset ? p.offset[b] : 0;
+    const int row = min(r0 + col, r1), g = row % p.G, i = row / p.G, h = hk * p.G + g, pos = off + i;
+    const int pmin = off + r0 / p.G, pmax = off + r1 / p.G;
     int n = keys_of(p, b);
-    if (p.bk.causal) n = min(n, max(off + p.Tq, 0));
+    if (p.bk.causal) n = min(n, max(pmax + 1, 0));
     const int run = ((n + p.nsplit - 1) / p.nsplit + 31) / 32 * 32, jb = min(n, sp * run), je = min(n, jb + run);
     const uint8_t *keep = p.keep ? p.keep + (int64_t)b * p.Tk : nullptr;
     // eight elements of a row at d, raw; zeros past D
@@ -832,24 +835,23 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
     };
     const E *kb = (const E *)p.kraw + b * p.k.sb + (int64_t)hk * p.k.sh, *vb = (const E *)p.vraw + b * p.v.sb + (int64_t)hk * p.v.sh;
     Raw kr[NC], vr[NC];
-    unsigned vok = 0;                                                                  // by c, where a key of the 32 may be left out
+    bool kept = true;                                                                  // the lane's key of the tile is not masked
     auto load_k = [&](int j0) {
+        if (keep) kept = keep[min(j0 + col, je - 1)] != 0;
         const E *k = kb + (int64_t)min(j0 + col, je - 1) * p.k.st;
 #pragma unroll
         for (int c = 0; c < NC; ++c) kr[c] = raw8(k, 16 * c + 8 * half);
     };
     auto load_v = [&](int j0) {
-        if (64 % CH == 0 && j0 + 32 <= je && keep == nullptr) {                        // one product of indexes instead of one a load
+        if (64 % CH == 0 && j0 + 32 <= je) {                        // one product of indexes instead of one a load
             const E *v = vb + (int64_t)(j0 + lane / CH) * p.v.st;
 #pragma unroll
             for (int c = 0; c < NC; ++c) vr[c] = raw8(v + c * (64 / CH) * p.v.st, lane % CH * 8);
         } else {
-            vok = 0;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const int f = lane + 64 * c, j = j0 + f / CH;
-                vok |= (j < je && (keep == nullptr || keep[j])) << c;
-                vr[c] = raw8(vb + (int64_t)min(j, je - 1) * p.v.st, f % CH * 8);
+                const int f = lane + 64 * c;
+                vr[c] = raw8(vb + (int64_t)min(j0 + f / CH, je - 1) * p.v.st, f % CH * 8);
             }
         }
     };
@@ -868,7 +870,6 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
             else qf[q][c] = w[q];
     }
     wave_sync();
-    const int pmin = off, pmax = off + p.Tq - 1;
     const bool near = !(je - 1 - pmin <= -R || jb - pmax >= R);                        // some key of the run within the last edge
     const float bl = p.table ? p.table[(p.bk.nd - 1) * p.H + h] * LOG2E : 0.f;
     const float br = p.table ? p.table[(p.bk.causal ? 0 : p.bk.nb - 1) * p.H + h] * LOG2E : 0.f;
@@ -903,9 +904,9 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
                     s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[q], x, s[0], 0, 0, 0);
                 }
         }
+        const unsigned live = (unsigned)__ballot(j0 + col < je && kept);
         if (j0 + 32 < je) load_k(j0 + 32);
         wave_sync();
-        const bool whole = j0 + 32 <= je && keep == nullptr;
 #pragma unroll
         for (int ks = 0; ks < NC; ++ks) {
             bf16x8 w[NP];
@@ -914,7 +915,7 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
 #pragma unroll
             for (int q = 0; q < NP; ++q)
                 *reinterpret_cast<u32x4p *>(pool + q * IMG + img_at<DP>(f / CH, f % CH)) =
-                    whole || (vok >> ks & 1) ? __builtin_bit_cast(u32x4p, w[q]) : u32x4p{0u, 0u, 0u, 0u};
+                    live == 0xffffffffu || (live >> (f / CH) & 1) ? __builtin_bit_cast(u32x4p, w[q]) : u32x4p{0u, 0u, 0u, 0u};
         }
         wave_sync();
         if (j0 + 32 < je) {
@@ -929,13 +930,11 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
             for (int r = 0; r < 16; ++r)
                 s[0][r] = __builtin_fmaf(s[0][r], c, tab[slot[min(max(j0 + row_of(r, half) - pos, -R), R) + R + LUT_PAD] * p.G + g]);
         }
-        if (j0 + 32 > je || keep || (p.bk.causal && j0 + 31 > pmin)) {
+        if (live != 0xffffffffu || (p.bk.causal && j0 + 31 > pmin)) {
+            const int seen = p.bk.causal ? pos - j0 - 4 * half : 64;                   // register rows up to here are not after the query
+            const unsigned mine = live >> (4 * half);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int jj = j0 + row_of(r, half);
-                const bool ok = jj < je && (!p.bk.causal || jj <= pos) && (keep == nullptr || keep[min(jj, p.Tk - 1)]);
-                s[0][r] = ok ? s[0][r] : -INFINITY;
-            }
+            for (int r = 0; r < 16; ++r) s[0][r] = (mine >> row_of(r, 0) & 1) && row_of(r, 0) <= seen ? s[0][r] : -INFINITY;
         }
         float mx = s[0][0];
 #pragma unroll
@@ -962,13 +961,13 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
         wave_sync();
     }
     l += __shfl_xor(l, 32, 64);
-    if (col >= rows) return;
+    if (r0 + col > r1) return;
     if (p.nsplit == 1) {
         const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
         put_acc<E, DP>((E *)p.out + (((int64_t)b * p.Tq + i) * p.H + h) * p.D, o, f, FULL ? DP : p.D, half);
         return;
     }
-    const int64_t at = ((int64_t)bhk * p.nsplit + sp) * rows + col;
+    const int64_t at = ((int64_t)bhk * p.nsplit + sp) * p.G * p.Tq + row;
     put_acc<float, DP>(p.po + at * p.D, o, 1.f, FULL ? DP : p.D, half);
     if (half == 0) {
         p.pml[2 * at] = m == -INFINITY ? -INFINITY : ms;
@@ -1036,13 +1035,21 @@ __global__ __launch_bounds__(256) void battn_pack_kernel(AttnPack a) {
 // -------------------------------------------------------------------------------------------------------- host --
 static int64_t bup(int64_t v) { return (v + 255) / 256 * 256; }
 static int battn_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
-static bool battn_few(const asr_bucket_attention_args *a) { return !a->train && (a->H / a->Hk) * a->Tq <= 32; }
+static int battn_few_tiles(const asr_bucket_attention_args *a) { return (int)cdiv((int64_t)a->H / a->Hk * a->Tq, 32); }
+// Without gradients the keys are split where there are few queries: one tile of 32 rows a key head, or so few workgroups of
+// 128 queries for so many keys that splitting gains more than the smaller tiles cost.  us, split against not, at B x T, 4 heads
+// of 64: float32 1 x 374 18 / 33, 1 x 1500 57 / 104, 4 x 374 35 / 35, 8 x 374 47 / 38; bfloat16 1 x 374 13 / 15, 1 x 1500 30 / 42,
+// 1 x 150 11 / 9, 4 x 374 21 / 15.
+static bool battn_few(const asr_bucket_attention_args *a) {
+    const int64_t wgs = (int64_t)a->B * a->H * cdiv(a->Tq, 128);
+    return !a->train && (battn_few_tiles(a) == 1 || (wgs <= a->Tk / (a->dtype == ASR_T_BF16 ? 24 : 16) && battn_few_tiles(a) <= 65535));
+}
 
 // Runs of a split cache: about eight waves a compute unit, each run at least 64 keys long (a shorter one spends more on its
 // joined row than on its keys)
 static int battn_runs(const asr_bucket_attention_args *a) {
-    int64_t n = 2048 / ((int64_t)a->B * a->Hk);
-    if (n > a->Tk / 64) n = a->Tk / 64;
+    int64_t n = 2048 / ((int64_t)a->B * a->Hk * battn_few_tiles(a));
+    if (n > cdiv(a->Tk, 64)) n = cdiv(a->Tk, 64);
     if (n > 64) n = 64;
     return n < 1 ? 1 : (int)n;
 }
@@ -1208,7 +1215,7 @@ static int battn_fwd(const asr_bucket_attention_args *a, hipStream_t st) {
         const size_t lds = (NP == 1 ? 2 : NP) * 32 * 2 * DP + sizeof(float) * p.bk.nb * p.G + (2 * (p.bk.R + LUT_PAD) + 1);
         const auto few = !vec ? battn_few_kernel<DT, DP, 0> : a->D < DP ? battn_few_kernel<DT, DP, 1> : battn_few_kernel<DT, DP, 2>;
         ASR_CHECK(battn_lds(few, lds, "bucket_attention_fwd"));
-        hipLaunchKernelGGL(few, dim3(a->B * a->Hk, p.nsplit), dim3(64), lds, st, p);
+        hipLaunchKernelGGL(few, dim3(a->B * a->Hk, p.nsplit, battn_few_tiles(a)), dim3(64), lds, st, p);
         if (p.nsplit > 1) hipLaunchKernelGGL((battn_join_kernel<DT>), dim3((unsigned)rows), dim3(128), 0, st, p);
         ASR_CHECK_LAUNCH("battn_few_kernel");
         return ASR_OK;

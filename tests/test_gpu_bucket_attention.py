@@ -150,6 +150,22 @@ def test_few_queries_against_a_cache(B, Tq, Tk, H, Hk, D, causal, dtype):
     _check(q, k, v, up, t, lengths=n * 0, offset=n, causal=causal, train=False)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("causal", [False, True], ids=["both-sides", "causal"])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,D", [
+    (1, 150, 374, 4, 4, 40), (1, 129, 900, 6, 2, 64), (2, 33, 1000, 2, 1, 128),          # keys split, several tiles of rows
+    (3, 50, 256, 1, 1, 7), (1, 1, 1, 40, 1, 96), (5, 200, 400, 8, 2, 80), (2, 300, 300, 8, 8, 128)])    # the last two not split
+def test_recognition_of_few_and_of_many_utterances(B, Tq, Tk, H, Hk, D, causal, dtype):
+    q, k, v, up, t = _inputs(B, Tq, Tk, H, Hk, D, dtype)
+    n = torch.randint(0, Tk + 1, (B,), generator=torch.Generator().manual_seed(6)).to(DEV)
+    n[0] = Tk
+    off = torch.randint(-Tq, Tk + 1, (B,), generator=torch.Generator().manual_seed(7)).to(DEV)
+    _check(q, k, v, up, t, causal=causal, train=False)
+    _check(q, k, v, up, t, lengths=n, offset=off, causal=causal, train=False)
+    _check(q, k, v, up, t, offset=torch.full((B,), Tk - Tq, device=DEV), causal=causal, train=False, reach=40,
+           keep=torch.rand(B, Tk, generator=torch.Generator().manual_seed(8)).to(DEV) < 0.3)
+
+
 def test_chunks_of_a_stream_equal_the_whole():
     """A causal pass in one call, in chunks against the growing cache, and frame by frame: the same rows."""
     from asr_amd.Models.transformer_ops import bucket_attention
