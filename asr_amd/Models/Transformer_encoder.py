@@ -345,17 +345,18 @@ class _HeadNormAttnFunction(torch.autograd.Function):
 
     @staticmethod
     @_exact
-    def forward(ctx, x, nw, nb_, wq, bq, wk, bk, wv, bv, gq, gk, table, wo, bo, keep, H, rot, reach, p, training):
+    def forward(ctx, x, nw, nb_, wq, bq, wk, bk, wv, bv, gq, gk, table, wo, bo, keep, H, rot, reach, p, training, graph):
         B, T, d = x.shape
         x2 = _req(x).view(B * T, d)
         h, mean, rstd = _ln_fwd(x2, nw, nb_)
         q, k, v = (_linear(h, w, b).view(B, T, H, d // H) for w, b in ((wq, bq), (wk, bk), (wv, bv)))
-        qr, kr = tops._rope_fwd(q, k, gq, gk, None, rot, ROPE_BASE, LN_EPS)
+        ops, edges = _lib.native(), tops._edges(table, False, reach)
+        qr, kr = ops.rope_fwd(q, k, gq, gk, None, rot, ROPE_BASE, LN_EPS)
         scale = 1.0 / math.sqrt(d // H)
-        cx, lse, _ = tops._attn_fwd(qr, kr, v, table, None, keep, None, False, reach, scale, True)
+        cx, lse, _ = ops.attn_fwd(qr, kr, v, table, None, keep, None, edges, False, scale, graph)
         y, m_o, f_o = _residual_drop(x2, _linear(cx.view(B * T, d), wo, bo), 1.0, p, training, 1)
         ctx.save_for_backward(x2, nw, wq, wk, wv, gq, gk, table, wo, keep, mean, rstd, h, q, k, v, qr, kr, cx, lse)
-        ctx.aux = (rot, reach, scale, m_o, f_o)
+        ctx.aux = (rot, edges, scale, m_o, f_o)
         ctx.wparams = (wq, bq, wk, bk, wv, bv, wo, bo, nw, nb_)
         return y.view_as(x)
 
@@ -363,13 +364,14 @@ class _HeadNormAttnFunction(torch.autograd.Function):
     @_exact
     def backward(ctx, dy):
         (x2, nw, wq, wk, wv, gq, gk, table, wo, keep, mean, rstd, h, q, k, v, qr, kr, cx, lse) = ctx.saved_tensors
-        rot, reach, scale, m_o, f_o = ctx.aux
+        rot, edges, scale, m_o, f_o = ctx.aux
+        ops = _lib.native()
         dy2 = dy.contiguous().view_as(x2)
         d = x2.shape[1]
         do = _scale_mask(dy2, m_o, f_o)
         dcx = _linear_dx(do, wo)
-        dqr, dkr, dv, dtable = tops._attn_bwd(qr, kr, v, table, None, keep, None, lse, cx, False, reach, scale, dcx.view_as(cx))
-        dq, dk, dgq, dgk = tops._rope_bwd(q, k, gq, gk, None, rot, ROPE_BASE, LN_EPS, dqr, dkr)
+        dqr, dkr, dv, dtable = ops.attn_bwd(qr, kr, v, table, None, keep, None, lse, cx, edges, False, scale, dcx.view_as(cx))
+        dq, dk, dgq, dgk = ops.rope_bwd(q, k, gq, gk, None, rot, ROPE_BASE, LN_EPS, dqr, dkr)
         dq, dk, dv = (t.view_as(x2) for t in (dq, dk, dv))
         dh = _linear_dx(dq, wq)
         _linear_dx(dk, wk, dx_out=dh, accumulate=True)
@@ -380,7 +382,7 @@ class _HeadNormAttnFunction(torch.autograd.Function):
             (dWo, dWq, dWk, dWv), (dbo, dbq, dbk, dbv) = _linear_dw(
                 [(do, cx.view_as(x2), wo), (dq, h, wq), (dk, h, wk), (dv, h, wv)], [(do, d), (dq, d), (dk, d), (dv, d)])
         return (dx.view_as(dy), dg, dbeta, dWq, dbq, dWk, dbk, dWv, dbv, dgq, dgk, dtable, dWo, dbo, None, None, None, None,
-                None, None)
+                None, None, None)
 
 
 # ------------------------------------------------------------ gated feed-forward block --
@@ -393,7 +395,7 @@ class _GatedFFFunction(torch.autograd.Function):
     def forward(ctx, x, ln_w, ln_b, wg, wu, wd, scale, p, training, n_out_drop):
         x2 = _req(x).view(-1, x.shape[-1])
         h, mean, rstd = _ln_fwd(x2, ln_w, ln_b)
-        y, m_o, f = _residual_drop(x2, tops._ff_fwd(h, wg, wu, wd, tops.ACTIVATIONS["swish"]), scale, p, training, n_out_drop)
+        y, m_o, f = _residual_drop(x2, _lib.native().ff_fwd(h, wg, wu, wd, tops.ACTIVATIONS["swish"]), scale, p, training, n_out_drop)
         ctx.save_for_backward(x2, ln_w, wg, wu, wd, mean, rstd, h)
         ctx.aux = (m_o, f)
         return y.view_as(x)
@@ -404,7 +406,7 @@ class _GatedFFFunction(torch.autograd.Function):
         x2, ln_w, wg, wu, wd, mean, rstd, h = ctx.saved_tensors
         m_o, f = ctx.aux
         dy2 = dy.contiguous().view_as(x2)
-        dh, dwg, dwu, dwd = tops._ff_bwd(h, wg, wu, wd, tops.ACTIVATIONS["swish"], _scale_mask(dy2, m_o, f))
+        dh, dwg, dwu, dwd = _lib.native().ff_bwd(h, wg, wu, wd, tops.ACTIVATIONS["swish"], _scale_mask(dy2, m_o, f))
         dx, lnpart = _ln_bwd(dh, x2, ln_w, mean, rstd, dy2)
         dg, dbeta = _ln_bwd_sums(lnpart)
         return dx.view_as(dy), dg, dbeta, dwg, dwu, dwd, None, None, None, None
@@ -628,7 +630,7 @@ class HeadNormAttention(nn.Module):
         return _HeadNormAttnFunction.apply(
             x, norm.weight, norm.bias, self.q_linear.weight, self.q_linear.bias, self.k_linear.weight, self.k_linear.bias,
             self.v_linear.weight, self.v_linear.bias, self.q_norm, self.k_norm, self.distance_bias, self.out.weight, self.out.bias,
-            keep, self.h, self.d_k if self.distance_bias is None else 0, REACH, self.p, self.training)
+            keep, self.h, self.d_k if self.distance_bias is None else 0, REACH, self.p, self.training, torch.is_grad_enabled())
 
 
 class GatedFeedForwardConformer(nn.Module):

@@ -11,26 +11,14 @@ head, width); a head must be contiguous, the other strides are free (views of on
 Calls enqueue on the current stream of the tensors' device and return without synchronising; gradients are computed by
 kernels too, without atomics: the same call gives the same bits.
 """
-import contextlib
 import ctypes as C
 import functools
 
 import torch
 
 from .. import _lib
-from .._lib import check
 
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _stream(device):
-    """Handle of the device's current stream (a fifth of the host time of torch.cuda.current_stream's stream object)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _on(device):
-    """The tensors' device as the current one for the launches inside."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _tensor(who, name, t, dim, like=None, dtype=None):
@@ -47,64 +35,37 @@ def _tensor(who, name, t, dim, like=None, dtype=None):
         raise RuntimeError(f"asr_amd.{who}: {name} is on {t.device}, expected {like.device}")
 
 
+def _like(first, dim, *others):
+    """Whether `first` and `others` are tensors on one GPU, of one type that has kernels, with `dim` dimensions: the checks of
+    _tensor in a fifth of their time, for calls that pass them."""
+    try:
+        if not first.is_cuda or first.dtype not in _DTYPES or first.dim() != dim:
+            return False
+        for t in others:
+            if t.dtype != first.dtype or t.device != first.device or t.dim() != dim:
+                return False
+        return True
+    except AttributeError:
+        return False
+
+
+def _weights(first, dim, *others):
+    """The same for float32 parameters on the device of `first`."""
+    try:
+        for t in others:
+            if t.dtype != torch.float32 or t.device != first.device or t.dim() != dim:
+                return False
+        return True
+    except AttributeError:
+        return False
+
+
 def _heads(t):
     """t with contiguous heads: itself, or a copy."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 # ----------------------------------------------------------------------------------------- norm and rotation --
-_ROPE = _lib.packer(_lib.RopeArgs)
-
-
-def _rope_call(fn, q, k, wq, wk, pos, rot, base, eps, gq, gk, qo, ko, dwq, dwk, ws):
-    B, T, H, D = q.shape
-    qs, ks = q.stride(), k.stride()
-    if gq is None:
-        gqp = gkp = 0
-        gqs = gks = (0, 0, 0)
-    else:
-        gqp, gkp, gqs, gks = gq.data_ptr(), gk.data_ptr(), gq.stride(), gk.stride()
-    a = _ROPE.pack(q.data_ptr(), k.data_ptr(), gqp, gkp, wq.data_ptr(), wk.data_ptr(), 0 if pos is None else pos.data_ptr(),
-                   qo.data_ptr(), ko.data_ptr(), 0 if dwq is None else dwq.data_ptr(), 0 if dwk is None else dwk.data_ptr(),
-                   0 if ws is None else ws.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], gqs[0], gqs[1], gqs[2],
-                   gks[0], gks[1], gks[2], 0 if pos is None or pos.dim() == 1 else pos.stride(0), B, T, H, k.shape[2], D, rot,
-                   _DTYPES[q.dtype], eps, base)
-    device = q.device
-    with _on(device):
-        check(fn(a, _stream(device)))
-
-
-def _rope_fwd(q, k, wq, wk, pos, rot, base, eps):
-    qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
-    if qo.numel():
-        _rope_call(_lib.load().asr_qk_norm_rope_fwd, q, k, wq, wk, pos, rot, base, eps, None, None, qo, ko, None, None, None)
-    return qo, ko
-
-
-def _rope_bwd(q, k, wq, wk, pos, rot, base, eps, gq, gk):
-    """Gradients of q, k and the two weights."""
-    lib = _lib.load()
-    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
-    if not q.numel():
-        return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk)
-    dwq, dwk, ws = torch.empty_like(wq), torch.empty_like(wk), wq.new_empty(lib.asr_qk_norm_rope_ws_floats(q.shape[-1]))
-    _rope_call(lib.asr_qk_norm_rope_bwd, q, k, wq, wk, pos, rot, base, eps, _heads(gq), _heads(gk), dq, dk, dwq, dwk, ws)
-    return dq, dk, dwq, dwk
-
-
-class _QkNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, pos, rot, base, eps):
-        ctx.save_for_backward(q, k, wq, wk, pos)
-        ctx.aux = (rot, base, eps)
-        return _rope_fwd(q, k, wq, wk, pos, rot, base, eps)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        return (*_rope_bwd(*ctx.saved_tensors, *ctx.aux, gq, gk), None, None, None, None)
-
-
 def qk_norm_rope(q, k, q_weight, k_weight, positions=None, rot_dim=None, base=10000.0, eps=1e-6):
     """Root-mean-square norm of every head of q (B, T, H, D) and k (B, T, Hk, D), times q_weight / k_weight (D, float32),
     then the rotation by position in the same pass: elements p and p + rot_dim / 2 turn by
@@ -112,10 +73,11 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions=None, rot_dim=None, base=10
     numbers (T,) or (B, T) on the GPU, by default 0..T-1; for single new frames of long streams the stream's own (angles
     are reduced in float64).  D even, at most 128.  Returns contiguous (q, k), differentiable in all four tensors."""
     who = "qk_norm_rope"
-    _tensor(who, "q", q, 4)
-    _tensor(who, "k", k, 4, like=q)
-    _tensor(who, "q_weight", q_weight, 1, like=q, dtype=torch.float32)
-    _tensor(who, "k_weight", k_weight, 1, like=q, dtype=torch.float32)
+    if not (_like(q, 4, k) and _weights(q, 1, q_weight, k_weight)):
+        _tensor(who, "q", q, 4)
+        _tensor(who, "k", k, 4, like=q)
+        _tensor(who, "q_weight", q_weight, 1, like=q, dtype=torch.float32)
+        _tensor(who, "k_weight", k_weight, 1, like=q, dtype=torch.float32)
     B, T, H, D = q.shape
     if k.shape[0] != B or k.shape[1] != T or k.shape[3] != D:
         raise RuntimeError(f"asr_amd.{who}: q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
@@ -137,9 +99,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions=None, rot_dim=None, base=10
         if pos.dtype != torch.int64 or (T > 1 and pos.stride(-1) != 1):
             pos = pos.long().contiguous()
     q, k, q_weight, k_weight = _heads(q), _heads(k), q_weight.contiguous(), k_weight.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
-        return _QkNormRope.apply(q, k, q_weight, k_weight, pos, rot, float(base), float(eps))
-    return _rope_fwd(q, k, q_weight, k_weight, pos, rot, float(base), float(eps))
+    return _lib.native().rope(q, k, q_weight, k_weight, pos, rot, float(base), float(eps))
 
 
 # ------------------------------------------------------------------------- attention with a bucketed bias --
@@ -176,69 +136,9 @@ def _edges_host(num_buckets, max_distance, causal):
     return (C.c_int32 * max(1, len(e)))(*e)
 
 
-_ATTN = _lib.packer(_lib.BucketAttentionArgs)
-_ATTN_WS = [n for n, _ in _lib.BucketAttentionArgs._fields_].index("ws")
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _attn_call(backward, q, k, v, table, lengths, keep, offset, causal, reach, scale, train, g, out, out32, lse, dq, dk, dv, dt):
-    lib = _lib.load()
-    B, Tq, H, D = q.shape
-    nb = table.shape[0] if table is not None else 2 if causal else 4
-    qs, ks, vs, gs = q.stride(), k.stride(), v.stride(), (0, 0, 0) if g is None else g.stride()
-    a = [q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(g), _ptr(table), C.addressof(_edges_host(nb, reach, causal)), _ptr(lengths),
-         _ptr(offset), _ptr(keep), _ptr(out), _ptr(out32), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dt), 0, qs[0], qs[1],
-         qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], gs[0], gs[1], gs[2], B, Tq, k.shape[1], H, k.shape[2], D, nb, causal,
-         _DTYPES[q.dtype], train, scale]
-    device = q.device
-    with _on(device):
-        n = lib.asr_bucket_attention_ws_bytes(_ATTN.pack(*a), backward)
-        if n < 0:
-            check(-1)
-        if n:
-            ws = torch.empty(n, device=device, dtype=torch.uint8)
-            a[_ATTN_WS] = ws.data_ptr()
-        check((lib.asr_bucket_attention_bwd if backward else lib.asr_bucket_attention_fwd)(_ATTN.pack(*a), _stream(device)))
-
-
-def _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, train):
-    """out, and for training the row statistics and the output in float32 (out itself where it is)."""
-    out = q.new_empty(q.shape)
-    if not out.numel() or not k.shape[1]:
-        return out.zero_(), None, None
-    lse = out32 = None
-    if train:
-        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device, dtype=torch.float32)
-        out32 = out if q.dtype == torch.float32 else torch.empty(q.shape, device=q.device, dtype=torch.float32)
-    _attn_call(0, q, k, v, table, lengths, keep, offset, causal, reach, scale, train, None, out, out32, lse, None, None, None, None)
-    return out, lse, out32
-
-
-def _attn_bwd(q, k, v, table, lengths, keep, offset, lse, out32, causal, reach, scale, g):
-    """Gradients of q, k, v and the table (None without one)."""
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    dt = torch.empty_like(table) if table is not None else None
-    if not q.numel() or not k.shape[1]:
-        return tuple(t.zero_() if t is not None else None for t in (dq, dk, dv, dt))
-    _attn_call(1, q, k, v, table, lengths, keep, offset, causal, reach, scale, True, _heads(g), out32, out32, lse, dq, dk, dv, dt)
-    return dq, dk, dv, dt
-
-
-class _BucketAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, table, lengths, keep, offset, causal, reach, scale):
-        out, lse, out32 = _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, True)
-        ctx.save_for_backward(q, k, v, table, lengths, keep, offset, lse, out32)
-        ctx.aux = (causal, reach, scale)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        return (*_attn_bwd(*ctx.saved_tensors, *ctx.aux, g), None, None, None, None, None, None)
+def _edges(table, causal, reach):
+    """Address of the host's list of edges, which stays for the life of the program."""
+    return C.addressof(_edges_host(table.shape[0] if table is not None else 2 if causal else 4, reach, causal))
 
 
 def _per_utterance(who, name, t, B, q):
@@ -259,9 +159,10 @@ def bucket_attention(q, k, v, table=None, lengths=None, keep=None, offset=None, 
     D at most 128, num_buckets at most 256, max_distance at most 1024.  Without gradients, calls with few queries
     (one new frame against a cache, one utterance at a time) split the keys over the GPU."""
     who = "bucket_attention"
-    _tensor(who, "q", q, 4)
-    _tensor(who, "k", k, 4, like=q)
-    _tensor(who, "v", v, 4, like=q)
+    if not _like(q, 4, k, v):
+        _tensor(who, "q", q, 4)
+        _tensor(who, "k", k, 4, like=q)
+        _tensor(who, "v", v, 4, like=q)
     B, Tq, H, D = q.shape
     if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or H == 0 or k.shape[2] == 0 or H % k.shape[2]:
         raise RuntimeError(f"asr_amd.{who}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
@@ -290,63 +191,11 @@ def bucket_attention(q, k, v, table=None, lengths=None, keep=None, offset=None, 
         keep = keep.contiguous()
     scale = D ** -0.5 if scale is None else float(scale)
     q, k, v = _heads(q), _heads(k), _heads(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or (table is not None and table.requires_grad)):
-        return _BucketAttention.apply(q, k, v, table, lengths, keep, offset, causal, reach, scale)
-    return _attn_fwd(q, k, v, table, lengths, keep, offset, causal, reach, scale, False)[0]
+    return _lib.native().attention(q, k, v, table, lengths, keep, offset, _edges(table, causal, reach), causal, scale)
 
 
 # ---------------------------------------------------------------------------------------- gated feed-forward --
 ACTIVATIONS = {"swish": 0, "gelu": 1}
-
-
-_FF = _lib.packer(_lib.GatedFFArgs)
-
-
-def _ff_call(backward, x2, wg, wu, wd, act, dy, y, dx, dwg, dwu, dwd):
-    lib = _lib.load()
-    M, d = x2.shape
-    a = [x2.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), _ptr(dy), _ptr(y), _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd), 0,
-         M, d, wg.shape[0], wd.shape[0], _DTYPES[x2.dtype], act]
-    device = x2.device
-    with _on(device):
-        n = lib.asr_gated_ff_ws_bytes(_FF.pack(*a), backward)
-        if n < 0:
-            check(-1)
-        ws = torch.empty(n, device=device, dtype=torch.uint8)
-        a[10] = ws.data_ptr()
-        check((lib.asr_gated_ff_bwd if backward else lib.asr_gated_ff_fwd)(_FF.pack(*a), _stream(device)))
-
-
-def _ff_fwd(x2, wg, wu, wd, act):
-    y = x2.new_empty(x2.shape[0], wd.shape[0])
-    if y.shape[0]:
-        _ff_call(0, x2, wg, wu, wd, act, None, y, None, None, None, None)
-    return y
-
-
-def _ff_bwd(x2, wg, wu, wd, act, dy, need=(True, True, True, True)):
-    """Gradients of x2 and the three weights, None for what `need` leaves out (the two first weights come together)."""
-    if not x2.shape[0]:
-        return torch.zeros_like(x2), torch.zeros_like(wg), torch.zeros_like(wu), torch.zeros_like(wd)
-    dx = torch.empty_like(x2) if need[0] else None
-    dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need[1] or need[2] else (None, None)
-    dwd = torch.empty_like(wd) if need[3] else None
-    _ff_call(1, x2, wg, wu, wd, act, dy.contiguous(), None, dx, dwg, dwu, dwd)
-    return dx, dwg, dwu, dwd
-
-
-class _GatedFF(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x2, wg, wu, wd, act):
-        ctx.save_for_backward(x2, wg, wu, wd)
-        ctx.act = act
-        return _ff_fwd(x2, wg, wu, wd, act)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        return (*_ff_bwd(*ctx.saved_tensors, ctx.act, dy, ctx.needs_input_grad), None)
 
 
 def gated_feed_forward(x, w_gate, w_up, w_down, act="swish"):
@@ -357,9 +206,10 @@ def gated_feed_forward(x, w_gate, w_up, w_down, act="swish"):
     who = "gated_feed_forward"
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise RuntimeError(f"asr_amd.{who}: x must be a tensor of at least one dimension")
-    _tensor(who, "x", x, x.dim())
-    for n, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
-        _tensor(who, n, w, 2, like=x)
+    if not _like(x, x.dim()) or not (_like(w_gate, 2, w_up, w_down) and w_gate.dtype == x.dtype and w_gate.device == x.device):
+        _tensor(who, "x", x, x.dim())
+        for n, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
+            _tensor(who, n, w, 2, like=x)
     if w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[-1] or w_down.shape[1] != w_gate.shape[0]:
         raise RuntimeError(f"asr_amd.{who}: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} and "
                            f"w_down {tuple(w_down.shape)} do not match")
@@ -369,8 +219,5 @@ def gated_feed_forward(x, w_gate, w_up, w_down, act="swish"):
         raise RuntimeError(f"asr_amd.{who}: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
     x2 = x.reshape(-1, x.shape[-1]).contiguous()
     ws = [w.contiguous() for w in (w_gate, w_up, w_down)]
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
-        y = _GatedFF.apply(x2, *ws, ACTIVATIONS[act])
-    else:
-        y = _ff_fwd(x2, *ws, ACTIVATIONS[act])
+    y = _lib.native().ff(x2, *ws, ACTIVATIONS[act])
     return y.view(*x.shape[:-1], y.shape[-1])

@@ -5,11 +5,12 @@ module raises -- there is no CPU or eager-PyTorch fallback anywhere in
 ``asr_amd``.  Build it with ``make`` (or ``__graft_entry__.build()``).
 """
 import ctypes as C
+import importlib.util
 import os
-import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libasr_amd.so")
+NATIVE_PATH = os.path.join(_HERE, "lib", "_transformer_ops.so")
 
 c_f = C.c_void_p      # device pointers travel as integers (tensor.data_ptr())
 c_i64 = C.c_int64
@@ -76,15 +77,6 @@ class AttDecBwdArgs(C.Structure):
         ("ws", c_f),
         ("defer_tail", C.c_int),
     ]
-
-
-def packer(cls):
-    """struct.Struct that writes a ctypes structure's bytes from its values in order, for calls whose host time matters (a third
-    of setting the fields one by one); a function whose argument is declared as a pointer (c_void_p) takes the bytes."""
-    codes = {C.c_void_p: "P", C.c_int64: "q", C.c_int: "i", C.c_float: "f", C.c_double: "d"}
-    s = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
-    pad = C.sizeof(cls) - s.size                    # what the compiler leaves behind the last field
-    return s if pad == 0 else struct.Struct(s.format + "%dx" % pad)
 
 
 class RopeArgs(C.Structure):
@@ -218,6 +210,7 @@ SYMBOLS = {
 }
 
 _lib = None
+_native = None
 
 
 def load():
@@ -236,6 +229,21 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def native():
+    """The module of torch bindings (csrc/transformer_ops.cpp), loaded once; raises if it is missing."""
+    global _native
+    if _native is None:
+        load()
+        if not os.path.exists(NATIVE_PATH):
+            raise RuntimeError(f"asr_amd: {NATIVE_PATH} not found -- the native module is required (run `make` in the repo root); "
+                               "there is no fallback path")
+        spec = importlib.util.spec_from_file_location("_transformer_ops", NATIVE_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _native = module
+    return _native
 
 
 def check(rc):

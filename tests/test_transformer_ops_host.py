@@ -89,17 +89,6 @@ def test_c_abi_refusals():
         _refused("asr_gated_ff_bwd", ff(), **change)
 
 
-def test_packed_arguments_are_the_structures_bytes():
-    from asr_amd import _lib
-    for cls in (_lib.RopeArgs, _lib.BucketAttentionArgs, _lib.GatedFFArgs):
-        s = _lib.packer(cls)
-        values = [i + 1 for i, _ in enumerate(cls._fields_)]
-        a = cls()
-        for (n, _), v in zip(cls._fields_, values):
-            setattr(a, n, v)
-        assert s.pack(*values) == bytes(a)
-
-
 def test_encoder_options():
     from asr_amd.Models.AttModel import AttModel
     from asr_amd.Models.Transformer_encoder import TransformerEncoder
