@@ -879,6 +879,7 @@ static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, i
 // a product, 75 without loads and LDS writes).  Several pieces: three to six products an LDS byte, 128 x 128 with four waves.
 // Smaller tiles where larger ones would leave compute units without one.
 typedef GemmCfg<1, 64, 2, 2, 512, 2, 4> CfgBig;             // 256 x 256
+typedef GemmCfg<1, 32, 2, 2, 512, 2, 4> CfgGate;            // gate tiles of 256 x 128
 template <int NP> struct CfgMid { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 512, 4, 2> T; };             // 256 x 128
 template <int NP> struct CfgHalf { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 512, 1, 4, 2> T; };      // 96 x 128, two grids of waves
 template <int NP> struct CfgSmall { typedef GemmCfg<NP, NP == 1 ? 64 : 32, NP == 1 ? 2 : 1, NP == 1 ? 2 : 1, 256, 2, 2> T; };
@@ -926,7 +927,15 @@ static int gff_gate_go(GateParams &g, hipStream_t st) {
 template <int DT, bool BWD>
 static int gff_gate(GateParams &g, hipStream_t st) {
     constexpr int NP = ElemOf<DT>::NP;
-    if ((int64_t)cdiv(g.Mp, 256) * (g.fp / 64) >= 256) return gff_gate_go<typename CfgMid<NP>::T, 256, 64, BWD>(g, st);
+    const int64_t rows = cdiv(g.Mp, 256);
+    if constexpr (NP == 1) {
+        // One piece is bound by the LDS: a wave's 128 x 32 of each product reads 16 B per matrix instruction less than 64 x 32
+        // (8192 x 1024 x 4096: 298 -> 274 us with dh, 170 -> 163 us without; k-tiles of 64 would spill, 351 us).  A unit's
+        // rounds of these tiles against those of half their size:
+        const int64_t wide = (rows * (g.fp / 128) + 255) / 256, narrow = (rows * (g.fp / 64) + 255) / 256;
+        if (g.fp % 128 == 0 && 1.85 * (double)wide <= (double)narrow) return gff_gate_go<CfgGate, 256, 128, BWD>(g, st);
+    }
+    if (rows * (g.fp / 64) >= 256) return gff_gate_go<typename CfgMid<NP>::T, 256, 64, BWD>(g, st);
     return gff_gate_go<typename CfgSmall<NP>::T, 128, 64, BWD>(g, st);
 }
 

@@ -47,6 +47,13 @@ def test_gelu(dtype):
     _check(*_inputs(7, 64, 100, 64, dtype, scale=3.0), act="gelu")
 
 
+@pytest.mark.parametrize("M,d,f,n", [(2060, 40, 2041, 33), (4000, 64, 2048, 64), (4100, 40, 2041, 33)])
+def test_tiles_of_every_width(M, d, f, n):
+    """16-bit products of enough tiles for the widest, with ragged last ones."""
+    _check(*_inputs(M, d, f, n, torch.bfloat16))
+    _check(*_inputs(M, d, f, n, torch.float16))
+
+
 def test_many_tiles_and_split_sums():
     _check(*_inputs(3000, 128, 256, 128, torch.bfloat16))
     _check(*_inputs(2100, 64, 192, 96, torch.float32))
