@@ -10,9 +10,16 @@
 // pieces of pieces.h (bfloat16: one piece, 2^-8 relative half step, like the stored type itself; the others 2^-16 and
 // 2^-24) because the next product reads them as matrix operands.
 //
-// Bound: the matrix cores.  128 x 128 tiles (gate and up columns interleaved by 32, so that a wave holds a and b of the same
-// elements), 4 waves of 64 x 64 from v_mfma_f32_32x32x16_bf16, operands staged through registers into LDS one k-tile ahead:
-// two LDS images for one piece, one image (two workgroups a compute unit hide each other's barriers) for two and three.
+// Gate and up columns are interleaved by 32, so that a wave holds a and b of the same elements; products are
+// v_mfma_f32_32x32x16_bf16 over tiles of 256 rows and eight waves where there are enough of them (the tiles of each product
+// stand at its launch), operands staged through registers into two LDS images.
+// Bound: the LDS with one piece, whose reads take as long as the matrix work; the matrix cores with more, and in the gate
+// kernel the stores behind each tile.  Measured, rates in bf16 matrix operations (a library product of the size: 1.2 PFLOP/s):
+//   bfloat16 8192 x 1024 x 4096    gate 163 us (0.84 PFLOP/s), backward 275 (0.75), y and dx 108 each on average (0.95),
+//                                  weight gradients 124 each on average (0.83)
+//   float32 11968 x 256 x 2048     gate 178 (0.85), backward 329 (0.69; without its 441 MB of stores 261), y and dx 133 (0.85),
+//                                  weight gradients 107 (1.06)
+//   bfloat16 8 x 1024 x 4096       8.3 + 5.2 + 2.3 us in three launches: 25 MB of weights at 1.6 TB/s, three waits long
 // Rows and columns beyond the matrix are read from its last row (clamped) and masked in the epilogues; the arrays h, da, db
 // are padded to whole tiles with zeros, which is what the products over them read past the end.
 #include <type_traits>
