@@ -23,7 +23,7 @@
 // instead of 10, and no atomics: every sum has a fixed order.
 //
 // Measured, rates in bf16 matrix operations: bfloat16 2 x 4096 causal, 16 heads of 128 on 2: forward 332 us (0.41 PFLOP/s of
-// the formula, 0.83 with the two further pieces of P), dQ 302 (0.68), dK and dV 460 (0.60); float32 32 x 374, 4 heads of 64, half
+// the formula, 0.83 with the further pieces of P), dQ 349 (0.59; 0.79), dK and dV 460 (0.60); float32 32 x 374, 4 heads of 64, half
 // to whole lengths: 45, 64 and 86 us (0.6 to 0.7 of six products a product of the padded maps), packing 18 us a pass at 5.1 TB/s.
 #include "pieces.h"
 
@@ -466,6 +466,10 @@ __global__ __launch_bounds__(256) void battn_delta_kernel(const void *dout, int6
 // their sums down a little more often than up, and every other query's dP is formed negated (float32 at 32 x 374, error of
 // dtable against 64 bits: 5.4e-7, without it 2.2e-6).
 // Key tiles of 32 where 64 would spill (one piece, D = 128: 302 us against 311 at 2 x 4096 causal, 16 heads).
+// With one piece dS goes into dQ in two: a row's dS sum to zero, and what rounding leaves of the sum meets the keys' mean, so
+// dQ would be off by up to 1.56 of its own last rounding (2 x 2821 frames, a head of 16; with two 1.0; 349 against 302 us at
+// 2 x 4096).  dK and dV take P and dS in one: nothing cancels there, the two roundings add up to 1.41 of one; two pieces would
+// cost 562 us against 460.
 template <int DT, int DP>
 __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void battn_dq_kernel(AttnParams p) {
     constexpr int NP = ElemOf<DT>::NP, KT = NP * DP > 64 ? 32 : KeyTile<NP>::N;
@@ -573,9 +577,10 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
                 }
                 wave_sync();
             }
-            bf16x8 df[NP][2];
-            to_operand<NP>(df, s[0]);
-            dot_cols<NP, NP, DP>(dq, ki, Tile::IMG, s0, df, lane);
+            constexpr int W = NP == 1 ? 2 : NP;
+            bf16x8 df[W][2];
+            to_operand<W>(df, s[0]);
+            dot_cols<NP, W, DP>(dq, ki, Tile::IMG, s0, df, lane);
         }
     }
     farl = wave_sum(farl);
