@@ -144,6 +144,8 @@ def _edges(table, causal, reach):
 def _per_utterance(who, name, t, B, q):
     if not isinstance(t, torch.Tensor) or t.device != q.device or t.dtype not in (torch.int32, torch.int64) or t.shape != (B,):
         raise RuntimeError(f"asr_amd.{who}: {name} must be ({B},) whole numbers on {q.device}")
+    if t.dtype == torch.int64:                    # beyond 2^30 from the keys nothing changes any more
+        t = t.clamp(-2 ** 30, 2 ** 30)
     return t.to(torch.int32).contiguous()
 
 

@@ -328,6 +328,8 @@ __device__ __forceinline__ void put_acc(E *row, const f32x16 (&acc)[DP / 32], fl
 
 template <int NP> struct KeyTile { static constexpr int N = NP == 1 ? 64 : 32; };
 
+// beyond 2^30 from the keys (at most 2^24 of them) nothing changes any more, and sums with frames stay in 32 bits
+__device__ __forceinline__ int offset_of(const AttnParams &p, int b) { return p.offset ? min(max(p.offset[b], -(1 << 30)), 1 << 30) : 0; }
 __device__ __forceinline__ int keys_of(const AttnParams &p, int b) {
     const int n = p.lengths ? p.lengths[b] : p.Tk;
     return min(max(n, 0), p.Tk);
@@ -351,7 +353,7 @@ __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 128 ? 1 : 2) void battn_
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int bh = blockIdx.x % (p.B * p.H), b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
     const int q0 = (p.ntile - 1 - (int)(blockIdx.x / (p.B * p.H))) * 128;              // the longest causal rows first
-    const int off = p.offset ? p.offset[b] : 0;
+    const int off = offset_of(p, b);
     const int i = q0 + wave * 32 + (lane & 31);
     const int n = keys_of(p, b);
     const int last = off + min(q0 + 127, p.Tq - 1);
@@ -485,7 +487,7 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP * DP <= 192 ? 2 : 1)) void bat
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int bh = blockIdx.x % (p.B * p.H), b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
     const int qt = p.ntile - 1 - (int)(blockIdx.x / (p.B * p.H)), q0 = qt * 128;
-    const int off = p.offset ? p.offset[b] : 0;
+    const int off = offset_of(p, b);
     const int i = q0 + wave * 32 + (lane & 31);
     const bool on = i < p.Tq;
     const int n = keys_of(p, b);
@@ -640,7 +642,7 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 
     // id = (tile, group of heads, utterance and key head): causal, the first keys have most queries and start first
     const int bhk = blockIdx.x % (p.B * p.Hk), b = bhk / p.Hk, hk = bhk - b * p.Hk;
     const int gs = blockIdx.x / (p.B * p.Hk) % p.gsplit, k0 = (int)(blockIdx.x / (p.B * p.Hk) / p.gsplit) * 128;
-    const int off = p.offset ? p.offset[b] : 0;
+    const int off = offset_of(p, b);
     const int n = keys_of(p, b);
     const int R = p.bk.R;
     const int jw = k0 + wave * 32, j = jw + (lane & 31);
@@ -802,7 +804,7 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
     __shared__ int16_t edge[MAX_EDGES];
     const int lane = threadIdx.x, half = lane >> 5, col = lane & 31;
     const int bhk = blockIdx.x, b = bhk / p.Hk, hk = bhk - b * p.Hk, sp = blockIdx.y;
-    const int r0 = blockIdx.z * 32, r1 = min(r0 + 32, p.G * p.Tq) - 1, R = p.bk.R, off = p.offset ? p.offset[b] : 0;
+    const int r0 = blockIdx.z * 32, r1 = min(r0 + 32, p.G * p.Tq) - 1, R = p.bk.R, off = offset_of(p, b);
     const int row = min(r0 + col, r1), g = row % p.G, i = row / p.G, h = hk * p.G + g, pos = off + i;
     const int pmin = off + r0 / p.G, pmax = off + r1 / p.G;
     int n = keys_of(p, b);
@@ -1044,14 +1046,15 @@ __global__ __launch_bounds__(256) void battn_pack_kernel(AttnPack a) {
 // -------------------------------------------------------------------------------------------------------- host --
 static int64_t bup(int64_t v) { return (v + 255) / 256 * 256; }
 static int battn_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
-static int battn_few_tiles(const asr_bucket_attention_args *a) { return (int)cdiv((int64_t)a->H / a->Hk * a->Tq, 32); }
+static int64_t battn_few_tiles(const asr_bucket_attention_args *a) { return ((int64_t)a->H / a->Hk * a->Tq + 31) / 32; }
 // Without gradients the keys are split where there are few queries: one tile of 32 rows a key head, or so few workgroups of
 // 128 queries for so many keys that splitting gains more than the smaller tiles cost.  us, split against not, at B x T, 4 heads
 // of 64: float32 1 x 374 18 / 33, 1 x 1500 57 / 104, 4 x 374 35 / 35, 8 x 374 47 / 38; bfloat16 1 x 374 13 / 15, 1 x 1500 30 / 42,
-// 1 x 150 11 / 9, 4 x 374 21 / 15.
+// 1 x 150 11 / 9, 4 x 374 21 / 15.  (Several tiles: the biases of a group of at most 32 heads lie in LDS.)
 static bool battn_few(const asr_bucket_attention_args *a) {
     const int64_t wgs = (int64_t)a->B * a->H * cdiv(a->Tq, 128);
-    return !a->train && (battn_few_tiles(a) == 1 || (wgs <= a->Tk / (a->dtype == ASR_T_BF16 ? 24 : 16) && battn_few_tiles(a) <= 65535));
+    return !a->train && (battn_few_tiles(a) == 1 || (wgs <= a->Tk / (a->dtype == ASR_T_BF16 ? 24 : 16) && a->H / a->Hk <= 32 &&
+                                                 battn_few_tiles(a) <= 65535));
 }
 
 // Runs of a split cache: about eight waves a compute unit, each run at least 64 keys long (a shorter one spends more on its
@@ -1224,7 +1227,7 @@ static int battn_fwd(const asr_bucket_attention_args *a, hipStream_t st) {
         const size_t lds = (NP == 1 ? 2 : NP) * 32 * 2 * DP + sizeof(float) * p.bk.nb * p.G + (2 * (p.bk.R + LUT_PAD) + 1);
         const auto few = !vec ? battn_few_kernel<DT, DP, 0> : a->D < DP ? battn_few_kernel<DT, DP, 1> : battn_few_kernel<DT, DP, 2>;
         ASR_CHECK(battn_lds(few, lds, "bucket_attention_fwd"));
-        hipLaunchKernelGGL(few, dim3(a->B * a->Hk, p.nsplit, battn_few_tiles(a)), dim3(64), lds, st, p);
+        hipLaunchKernelGGL(few, dim3(a->B * a->Hk, p.nsplit, (unsigned)battn_few_tiles(a)), dim3(64), lds, st, p);
         if (p.nsplit > 1) hipLaunchKernelGGL((battn_join_kernel<DT>), dim3((unsigned)rows), dim3(128), 0, st, p);
         ASR_CHECK_LAUNCH("battn_few_kernel");
         return ASR_OK;

@@ -182,6 +182,33 @@ def test_chunks_of_a_stream_equal_the_whole():
             held(got, (want[0][:, a:b], want[1][:, a:b]))
 
 
+@pytest.mark.parametrize("Tq", [1, 40])
+@pytest.mark.parametrize("causal", [False, True], ids=["both-sides", "causal"])
+def test_offsets_and_lengths_of_64_bits(Tq, causal):
+    """Beyond the last bucket edge all places are alike: the same bits as from a place that a small number names."""
+    from asr_amd.Models.transformer_ops import bucket_attention
+    q, k, v, up, t = _inputs(4, Tq, 60, 2, 1, 32, torch.float32)
+
+    def run(train, **kw):
+        leaves = [x.clone().requires_grad_(train) for x in (q, k, v, t)]
+        y = bucket_attention(*leaves, causal=causal, **{n: torch.tensor(x, dtype=d, device=DEV) for n, (x, d) in kw.items()})
+        return (y, *torch.autograd.grad(y, leaves, up)) if train else (y,)
+    i32, i64 = torch.int32, torch.int64
+    for train in (False, True):
+        for a, b in ((dict(offset=([2 ** 40 + 3, -2 ** 40, 2 ** 32 - 5, 30 - 2 ** 32], i64)), dict(offset=([9000, -9000, 9000, -9000], i64))),
+                     (dict(offset=([2 ** 31 - 1, -2 ** 31, 2 ** 31 - 20, 30], i32)), dict(offset=([9000, -9000, 9000, 30], i32))),
+                     (dict(lengths=([2 ** 32 + 5, 5 - 2 ** 32, 2 ** 33, 7], i64)), dict(lengths=([60, 0, 60, 7], i32)))):
+            for x, y in zip(run(train, **a), run(train, **b)):
+                assert torch.equal(x, y), (train, a)
+
+
+def test_many_heads_on_one_key_head():
+    """More query heads in a group than the split form keeps biases of; 256 buckets."""
+    q, k, v, up, _ = _inputs(1, 20, 700, 130, 1, 8, torch.float32)
+    t = torch.randn(256, 130, generator=torch.Generator().manual_seed(2)).to(DEV)
+    _check(q, k, v, up, t, offset=torch.tensor([680], device=DEV), causal=True, reach=300)
+
+
 def test_offsets_before_and_beyond_the_keys():
     q, k, v, up, t = _inputs(3, 40, 60, 2, 1, 32, torch.float32)
     for off in ([-30, 500, 10], [-60, 2 ** 20, 0]):
