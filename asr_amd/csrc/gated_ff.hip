@@ -495,17 +495,20 @@ __global__ __launch_bounds__(C::NT, 2) void gff_nt_kernel(NtParams p) {
 // ------------------------------------------------------------- C = A^T B over the rows, split over workgroups --
 // Output row r < half goes to c0, r >= half to c1 (the gate's and the up projection's gradients lie half apart in [da db]);
 // rows from `valid` on of either are padding.  With splits > 1 every split writes float32 partials, gff_sum_kernel adds them in
-// order.
+// order.  Both kernels take up to two products: the first one's workgroups come first.
 struct TnParams {
     Planes a, b;
     void *c0, *c1;
     float *part;
-    int64_t half, valid, N, part_sz;
+    int64_t rows, half, valid, N, part_sz;
     int64_t kt, kt_split;
-    int ncol, ntiles, vec;
+    int ncol, ntiles, splits, vec;
 };
+struct TnPair { TnParams p[2]; int blk; };
 template <int DT, typename C, int BM, int BN>
-__global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnParams p) {
+__global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnPair pair) {
+    const TnParams &p = pair.p[(int)blockIdx.x >= pair.blk];
+    const int id = (int)blockIdx.x - ((int)blockIdx.x >= pair.blk ? pair.blk : 0), split = id / p.ntiles;
     constexpr int NP = C::NP, RM = BM / C::WM, RN = BN / C::WN, TM = RM / 32, TN = RN / 32;
     typedef typename ElemOf<DT>::type E;
     typedef TnTile<C, BM> TA;
@@ -514,7 +517,7 @@ __global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnParams p) {
     __shared__ __attribute__((aligned(16))) unsigned char pool[POOL > TURN ? POOL : TURN];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WN, wn = wave % C::WN;
     int tm, tn;
-    tile_of(blockIdx.x, p.ntiles, p.ncol, tm, tn);
+    tile_of(id - split * p.ntiles, p.ntiles, p.ncol, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
     f32x16 acc[TM][TN];
     zero_acc(acc);
@@ -522,7 +525,7 @@ __global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnParams p) {
     TB tb;
     ta.init(p.a, m0);
     tb.init(p.b, n0);
-    const int64_t k0 = blockIdx.y * p.kt_split;
+    const int64_t k0 = split * p.kt_split;
     main_loop<C>(acc, ta, tb, pool, k0, min(p.kt, k0 + p.kt_split),
                  [&](const unsigned char *img, int i, int ks) { return frag_tn<BM>(img, wm * RM + i * 32, ks, lane); },
                  [&](const unsigned char *img, int j, int ks) { return frag_tn<BN>(img, wn * RN + j * 32, ks, lane); });
@@ -538,7 +541,7 @@ __global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnParams p) {
                 row -= second ? p.half : 0;
                 if (row >= p.valid || (second && p.c1 == nullptr)) return;
                 if (p.part) {
-                    float *dst = p.part + blockIdx.y * p.part_sz + ((second ? p.valid : 0) + row) * p.N;
+                    float *dst = p.part + split * p.part_sz + ((second ? p.valid : 0) + row) * p.N;
                     put_row4<float>(dst, cb + c, p.N, p.vec, v);
                 } else {
                     put_row4<E>((E *)(second ? p.c1 : p.c0) + row * p.N, cb + c, p.N, p.vec, v);
@@ -547,17 +550,20 @@ __global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnParams p) {
         }
 }
 template <int DT, int V>
-__global__ __launch_bounds__(256) void gff_sum_kernel(const float *__restrict__ part, int64_t sz, int splits, int64_t n0, void *c0, void *c1) {
+__global__ __launch_bounds__(256) void gff_sum_kernel(TnPair pair) {
     typedef typename ElemOf<DT>::type E;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < sz; i += (int64_t)gridDim.x * 256 * V) {
+    const bool second = (int)blockIdx.x >= pair.blk;
+    const TnParams &p = pair.p[second];
+    const int64_t n0 = p.valid * p.N, nblk = second ? (int)gridDim.x - pair.blk : min((int)gridDim.x, pair.blk), blk = (int)blockIdx.x - (second ? pair.blk : 0);
+    for (int64_t i = (blk * 256 + threadIdx.x) * V; i < p.part_sz; i += nblk * 256 * V) {
         float v[V], t[V];
-        load_vec<float, V>(part + i, v);
-        for (int s = 1; s < splits; ++s) {
-            load_vec<float, V>(part + s * sz + i, t);
+        load_vec<float, V>(p.part + i, v);
+        for (int s = 1; s < p.splits; ++s) {
+            load_vec<float, V>(p.part + s * p.part_sz + i, t);
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] += t[e];
         }
-        store_vec<E, V>(i < n0 ? (E *)c0 + i : (E *)c1 + (i - n0), v);
+        store_vec<E, V>(i < n0 ? (E *)p.c0 + i : (E *)p.c1 + (i - n0), v);
     }
 }
 
@@ -760,6 +766,8 @@ static int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 // A weight gradient (rows x cols, summed over M): the tile, and in how many runs of M it is summed.  A run has at least 8
 // k-tiles, and there are runs until the launch has two workgroups of four waves (or one of eight) for each compute unit.
+// Where both gradients take the small tile they share their launches, which then neither fills the GPU alone (1003 x 200 x 683
+// float16: 14 + 14 us for the products and 4 + 4 for their sums become 17 and 4).
 struct TnPlan { int big, splits; };
 static TnPlan gff_tn_plan(int NP, int64_t rows, int64_t cols, int64_t M) {
     const int64_t kt = cdiv(M, NP == 1 ? 64 : 32);
@@ -782,7 +790,7 @@ struct GffPlan {
     TnPlan gu, wd;                       // the weight gradients of [gate; up] and down
     int64_t off[16], bytes;              // workspace: byte offsets
 };
-enum { O_X, O_WG, O_WU, O_WD, O_H, O_DY, O_WDT, O_WGUT, O_DAB, O_PART };
+enum { O_X, O_WG, O_WU, O_WD, O_H, O_DY, O_WDT, O_WGUT, O_DAB, O_PART, O_PART_WD };
 
 static bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
@@ -816,10 +824,8 @@ static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
         take(O_DAB, p.Mp * 2 * p.fp * e);
         p.gu = gff_tn_plan(p.NP, 2 * p.fp, a->d, a->M);
         p.wd = gff_tn_plan(p.NP, a->n, a->f, a->M);
-        int64_t part = 0;
-        if (p.gu.splits > 1) part = (int64_t)p.gu.splits * 2 * a->f * a->d;
-        if (p.wd.splits > 1 && (int64_t)p.wd.splits * a->n * a->f > part) part = (int64_t)p.wd.splits * a->n * a->f;
-        take(O_PART, part * 4);
+        take(O_PART, p.gu.splits > 1 ? (int64_t)p.gu.splits * 2 * a->f * a->d * 4 : 0);
+        take(O_PART_WD, p.wd.splits > 1 ? (int64_t)p.wd.splits * a->n * a->f * 4 : 0);
     }
     p.bytes = o;
 }
@@ -943,37 +949,49 @@ static int gff_gate(GateParams &g, hipStream_t st) {
         if (g.fp % 128 == 0 && 1.85 * (double)wide <= (double)narrow) return gff_gate_go<CfgGate, 256, 128, BWD>(g, st);
     }
     if (rows * (g.fp / 64) >= 256) return gff_gate_go<typename CfgMid<NP>::T, 256, 64, BWD>(g, st);
+    // (1003 x 200 x 683 float16, 88 tiles of 128 x 64: 25 and 17.5 us, in tiles of 64 x 64 16.3 and 11.9)
+    if ((int64_t)cdiv(g.Mp, 128) * (g.fp / 64) < 256) return gff_gate_go<typename CfgDeep<NP>::T, 64, 64, BWD>(g, st);
     return gff_gate_go<typename CfgSmall<NP>::T, 128, 64, BWD>(g, st);
 }
 
 template <int DT, typename C, int BM, int BN>
-static void gff_tn_go(TnParams &p, int64_t rows, int64_t M, int splits, hipStream_t st) {
-    p.ncol = cdiv(p.N, BN);
-    p.ntiles = cdiv(rows, BM) * p.ncol;
-    p.kt = cdiv(M, C::BK);
-    p.kt_split = (p.kt + splits - 1) / splits;
-    hipLaunchKernelGGL((gff_tn_kernel<DT, C, BM, BN>), dim3(p.ntiles, splits), dim3(C::NT), 0, st, p);
-}
-template <int DT>
-static int gff_tn(const Planes &a, const Planes &b, void *c0, void *c1, int64_t rows, int64_t half, int64_t valid, int64_t N, int64_t M,
-                  const TnPlan &pl, float *part, hipStream_t st) {
-    constexpr int NP = ElemOf<DT>::NP;
-    const int splits = pl.splits;
-    TnParams p{a, b, c0, c1, splits > 1 ? part : nullptr, half, valid, N, (c1 ? 2 : 1) * valid * N, 0, 0, 0, 0,
-               (int)(N % 4 == 0 && aligned16(c0) && aligned16(c1))};
-    if (pl.big) gff_tn_go<DT, typename CfgMid<NP>::T, 256, 128>(p, rows, M, splits, st);
-    else gff_tn_go<DT, typename CfgSmall<NP>::T, 128, 128>(p, rows, M, splits, st);
-    ASR_CHECK_LAUNCH("gff_tn_kernel");
-    if (splits > 1) {
-        const int64_t n0 = valid * N;
-        if (n0 % 4 == 0 && aligned16(c0) && aligned16(c1))
-            hipLaunchKernelGGL((gff_sum_kernel<DT, 4>), dim3((unsigned)(cdiv(p.part_sz, 1024) < 4096 ? cdiv(p.part_sz, 1024) : 4096)), dim3(256), 0, st, part,
-                               p.part_sz, splits, n0, c0, c1);
-        else
-            hipLaunchKernelGGL((gff_sum_kernel<DT, 1>), dim3((unsigned)(cdiv(p.part_sz, 256) < 4096 ? cdiv(p.part_sz, 256) : 4096)), dim3(256), 0, st, part,
-                               p.part_sz, splits, n0, c0, c1);
-        ASR_CHECK_LAUNCH("gff_sum_kernel");
+static void gff_tn_go(TnPair &pair, int n, int64_t M, hipStream_t st) {
+    int64_t blocks = 0;
+    for (int k = 0; k < n; ++k) {
+        TnParams &p = pair.p[k];
+        p.ncol = cdiv(p.N, BN);
+        p.ntiles = cdiv(p.rows, BM) * p.ncol;
+        p.kt = cdiv(M, C::BK);
+        p.kt_split = (p.kt + p.splits - 1) / p.splits;
+        blocks += (int64_t)p.ntiles * p.splits;
+        if (k == 0) pair.blk = (int)blocks;
     }
+    hipLaunchKernelGGL((gff_tn_kernel<DT, C, BM, BN>), dim3((unsigned)blocks), dim3(C::NT), 0, st, pair);
+}
+// n = 1 or 2 products with the same tile
+template <int DT>
+static int gff_tn(TnPair &pair, int n, int big, int64_t M, hipStream_t st) {
+    constexpr int NP = ElemOf<DT>::NP;
+    if (big) gff_tn_go<DT, typename CfgMid<NP>::T, 256, 128>(pair, n, M, st);
+    else gff_tn_go<DT, typename CfgSmall<NP>::T, 128, 128>(pair, n, M, st);
+    ASR_CHECK_LAUNCH("gff_tn_kernel");
+    TnPair sums{};
+    int m = 0, blocks = 0;
+    bool vec = true;
+    for (int k = 0; k < n; ++k)
+        if (pair.p[k].splits > 1) {
+            const TnParams &p = sums.p[m++] = pair.p[k];
+            vec = vec && p.valid * p.N % 4 == 0 && aligned16(p.c0) && aligned16(p.c1);
+        }
+    if (!m) return ASR_OK;
+    for (int k = 0; k < m; ++k) {
+        const int need = cdiv(sums.p[k].part_sz, vec ? 1024 : 256);
+        blocks += need < 4096 ? need : 4096;
+        if (k == 0) sums.blk = blocks;
+    }
+    if (vec) hipLaunchKernelGGL((gff_sum_kernel<DT, 4>), dim3(blocks), dim3(256), 0, st, sums);
+    else hipLaunchKernelGGL((gff_sum_kernel<DT, 1>), dim3(blocks), dim3(256), 0, st, sums);
+    ASR_CHECK_LAUNCH("gff_sum_kernel");
     return ASR_OK;
 }
 
@@ -1020,9 +1038,14 @@ static int gff_run(const asr_gated_ff_args *a, bool bwd, hipStream_t st) {
     }
     ASR_CHECK((gff_gate<DT, true>(g, st)));
     if (a->dx) ASR_CHECK(gff_nt<DT>(dab, wgut, a->dx, a->M, a->d, 2 * p.fp, st));
-    float *part = (float *)at(O_PART);
-    if (a->dwg) ASR_CHECK(gff_tn<DT>(dab, x, a->dwg, a->dwu, 2 * p.fp, p.fp, a->f, a->d, a->M, p.gu, part, st));
-    if (a->dwd) ASR_CHECK(gff_tn<DT>(dy, h, a->dwd, nullptr, a->n, up_to(a->n, 256), a->n, a->f, a->M, p.wd, part, st));
+    const TnParams gu{dab, x, a->dwg, a->dwu, p.gu.splits > 1 ? (float *)at(O_PART) : nullptr, 2 * p.fp, p.fp, a->f, a->d, 2ll * a->f * a->d, 0, 0, 0, 0,
+                      p.gu.splits, (int)(a->d % 4 == 0 && aligned16(a->dwg) && aligned16(a->dwu))};
+    const TnParams down{dy, h, a->dwd, nullptr, p.wd.splits > 1 ? (float *)at(O_PART_WD) : nullptr, a->n, up_to(a->n, 256), a->n, a->f, (int64_t)a->n * a->f,
+                        0, 0, 0, 0, p.wd.splits, (int)(a->f % 4 == 0 && aligned16(a->dwd))};
+    TnPair both{{gu, down}, 0}, one{{gu}, 0}, other{{down}, 0};
+    if (a->dwg && a->dwd && !p.gu.big && !p.wd.big) return gff_tn<DT>(both, 2, 0, a->M, st);
+    if (a->dwg) ASR_CHECK(gff_tn<DT>(one, 1, p.gu.big, a->M, st));
+    if (a->dwd) ASR_CHECK(gff_tn<DT>(other, 1, p.wd.big, a->M, st));
     return ASR_OK;
 }
 
