@@ -7,8 +7,8 @@
 //           3  dWg, dWu = [da db]^T x,  dWd = dy^T h                                           (gff_tn_kernel, split over M)
 // Nothing but x is kept for the backward: computing a and b again costs 4 M d f operations of 22 and saves writing and
 // reading two M x f arrays each way; it also keeps act' on unrounded a and b.  h, da and db are rounded once to the
-// pieces of pieces.h (bfloat16: one piece, 2^-8 relative half step, like the stored type itself; the others 2^-16 and
-// 2^-24) because the next product reads them as matrix operands.
+// stored type's own precision (bfloat16 2^-8, float16 2^-11 relative half step, float32 three pieces of pieces.h, 2^-24) because
+// the next product reads them as matrix operands.
 //
 // Gate and up columns are interleaved by 32, so that a wave holds a and b of the same elements; products are
 // v_mfma_f32_32x32x16_bf16 over tiles of 256 rows and eight waves where there are enough of them (the tiles of each product
@@ -26,10 +26,23 @@
 #include "pieces.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4g __attribute__((ext_vector_type(4)));
 typedef short s16x8g __attribute__((ext_vector_type(8)));
 
 enum { GFF_SWISH = 0, GFF_GELU = 1 };
+
+// float16 operands go into v_mfma_f32_32x32x16_f16 as they lie, one product like bfloat16
+template <int DT> struct FfElem : ElemOf<DT> {
+    static constexpr int NP = DT == ASR_T_F32 ? 3 : 1;
+    static constexpr bool F16 = DT == ASR_T_F16;
+};
+template <bool F16>
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+    if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
 
 // ------------------------------------------------------------------------------------------------- operands --
 // A matrix as NP planes of bf16, row-major; rows are clamped to [0, rows)
@@ -47,7 +60,7 @@ __device__ __forceinline__ float exp_acc(float x) {
     const float r = __builtin_amdgcn_exp2f(hi);
     return __builtin_fmaf(r, lo * 0.693147180559945309417f, r);
 }
-// FAST: for values that are rounded to bfloat16 right after, exp by one base-2 exponential (relative error 2^-24 |x|)
+// FAST: for values that are rounded to 16 bits right after, exp by one base-2 exponential (relative error 2^-24 |x|)
 template <bool FAST>
 __device__ __forceinline__ float exp_of(float x) { return FAST ? __builtin_amdgcn_exp2f(x * 1.44269504088896340736f) : exp_acc(x); }
 template <bool FAST>
@@ -70,9 +83,10 @@ __device__ __forceinline__ float act_fwd(int kind, float a) {
 
 // -------------------------------------------------------------------------------------------- LDS images --
 // A workgroup of the products: pieces, depth of a k-tile, LDS images of it, register sets on their way, threads, the waves'
-// grid WM x WN over the tile, and WK such grids that share out each k-tile's steps of 16 k
-template <int NP_, int BK_, int NBUF_, int NSET_, int NT_, int WM_, int WN_, int WK_ = 1>
+// grid WM x WN over the tile, WK such grids that share out each k-tile's steps of 16 k, and whether operands are float16
+template <int NP_, int BK_, int NBUF_, int NSET_, int NT_, int WM_, int WN_, int WK_ = 1, bool F16_ = false>
 struct GemmCfg {
+    static constexpr bool F16 = F16_;
     static constexpr int NP = NP_, BK = BK_, NBUF = NBUF_, NSET = NSET_, NT = NT_, WM = WM_, WN = WN_, WK = WK_;
     static_assert(NT == 64 * WM * WN * WK, "threads");
 };
@@ -185,7 +199,7 @@ __device__ __forceinline__ void store_all(const T &t, unsigned char *img) {
 }
 
 // acc += A B over one k-tile; fa / fb (piece, tile, ks) deliver fragments.  Smallest pieces first.
-template <int NP, int KS, int TM, int TN, typename FA, typename FB>
+template <int NP, bool F16, int KS, int TM, int TN, typename FA, typename FB>
 __device__ __forceinline__ void mma_tile(f32x16 (&acc)[TM][TN], FA fa, FB fb) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -205,7 +219,7 @@ __device__ __forceinline__ void mma_tile(f32x16 (&acc)[TM][TN], FA fa, FB fb) {
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
                     for (int j = 0; j < TN; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[q][i], b[s - q][j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = mma<F16>(a[q][i], b[s - q][j], acc[i][j]);
     }
 }
 
@@ -231,7 +245,7 @@ __device__ __forceinline__ void main_loop(f32x16 (&acc)[TM][TN], TA &ta, TB &tb,
                 load_all<0>(ta, (kt + 1) * C::BK);
                 load_all<0>(tb, (kt + 1) * C::BK);
             }
-            mma_tile<NP, C::BK / 16, TM, TN>(acc, [&](int q, int i, int ks) { return frag_a(lds + q * TA::IMG, i, ks); },
+            mma_tile<NP, C::F16, C::BK / 16, TM, TN>(acc, [&](int q, int i, int ks) { return frag_a(lds + q * TA::IMG, i, ks); },
                                              [&](int q, int j, int ks) { return frag_b(lds + IA + q * TB::IMG, j, ks); });
             __syncthreads();
         }
@@ -270,7 +284,7 @@ __device__ __forceinline__ void main_loop(f32x16 (&acc)[TM][TN], TA &ta, TB &tb,
                 for (int s = NP - 1; s >= 0; --s)
 #pragma unroll
                     for (int q = s; q >= 0; --q)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks % NFB][q][i], b[ks % NFB][s - q][j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = mma<C::F16>(a[ks % NFB][q][i], b[ks % NFB][s - q][j], acc[i][j]);
 #pragma unroll
                 for (int sl = c * NSL / NCH; sl < (c + 1) * NSL / NCH; ++sl) {
                     if (sl < TA::NS) {
@@ -321,8 +335,12 @@ __device__ __forceinline__ void turn_tile(const f32x16 &t, float *S, F put) {
     wave_sync();
 }
 
-template <int NP>
+template <int NP, bool F16>
 __device__ __forceinline__ void put_pieces(__bf16 *dst, int64_t ps, float4 v) {
+    if constexpr (F16) {
+        *reinterpret_cast<f16x4 *>(dst) = f16x4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+        return;
+    }
     unsigned lo[NP], hi[NP];
     split_pair<NP>(v.x, v.y, lo);
     split_pair<NP>(v.z, v.w, hi);
@@ -350,6 +368,45 @@ __device__ __forceinline__ void tile_of(int id, int ntiles, int ncol, int &row, 
     col = t - row * ncol;
 }
 
+// ------------------------------------------------------------------------- powers of two for float16 h, da, db --
+// h, da and db may leave the range of float16 where y and the gradients do not (and gradients may be tiny), so they are kept
+// times a power of two that brings a bound on them to 2^15: |a_ij| <= |x_i| |wg_j|, likewise b and dh, |act(a)| <= |a| and
+// |act'(a)| <= 1.13.  The bound is above a typical value by about sqrt(d) each, so that is 2^-14 and more: normal numbers down to
+// 2^-15 of it.  gff_norm_kernel leaves the largest squared row norms by workgroup, the products' waves finish them.  Rows that
+// hold infinities or NaN do not count: what they reach is infinite or NaN anyway.
+#define NORM_BLOCKS 64
+enum { N_X, N_WG, N_WU, N_DY, N_WDT, N_COUNT };
+struct NormJobs { Planes m[N_COUNT]; };
+__global__ __launch_bounds__(256) void gff_norm_kernel(NormJobs jobs, float *out) {
+    __shared__ float red[4];
+    const Planes &m = jobs.m[blockIdx.y];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const _Float16 *p = reinterpret_cast<const _Float16 *>(m.p);
+    float top = 0.f;
+    for (int64_t r = blockIdx.x * 4 + wave; r < m.rows; r += NORM_BLOCKS * 4) {
+        float s = 0.f;
+        for (int64_t k = lane * 8; k < m.ld; k += 512) {
+            const f16x8 v = *reinterpret_cast<const f16x8 *>(p + r * m.ld + k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += (float)v[e] * (float)v[e];
+        }
+        s = wave_sum(s);
+        if (s < INFINITY) top = fmaxf(top, s);
+    }
+    if (lane == 0) red[wave] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) out[blockIdx.y * NORM_BLOCKS + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+enum { S_NONE, S_H, S_DAB };
+// 2^(sign (15 - e)), e the exponent above the bound
+__device__ __forceinline__ float pow2_of(const float *n, int which, int sign) {
+    const int lane = threadIdx.x & 63;
+    auto top = [&](int k) { return wave_max(n[k * NORM_BLOCKS + lane]); };
+    const float x = top(N_X), g = top(N_WG), u = top(N_WU);
+    const float bound = which == S_H ? sqrtf(x * g) * sqrtf(x * u) : 1.13f * sqrtf(top(N_DY) * top(N_WDT)) * sqrtf(x * fmaxf(g, u));
+    return bound > 0.f ? ldexpf(1.f, sign * (15 - min(max(ilogbf(bound) + 1, -100), 100))) : 1.f;
+}
+
 // ------------------------------------------------------------------- a, b (and dh) of one tile, elementwise part --
 struct GateParams {
     Planes x, wg, wu;                    // x (M, dp), weights (f, dp)
@@ -358,6 +415,7 @@ struct GateParams {
     int64_t h_ps, dab_ps;
     int64_t M, Mp, fp;
     int f, dp, np, ncol, ntiles, act;
+    const float *norm;
 };
 
 // BM rows x BN columns of h: A tile of BM rows, B tile of 2 BN (gate and up rows interleaved), then of BN rows of Wd^T
@@ -398,6 +456,11 @@ __global__ __launch_bounds__(C::NT, 2) void gff_gate_kernel(GateParams p) {
     }
     float *S = reinterpret_cast<float *>(pool) + wave * 1024;
     const int64_t cb = n0 + wn * 32;
+    float sh = 1.f, sd = 1.f;
+    if constexpr (C::F16) {
+        sh = pow2_of(p.norm, S_H, 1);
+        if (BWD) sd = pow2_of(p.norm, S_DAB, 1);
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int64_t rb = m0 + wm * RM + i * 32;
@@ -411,6 +474,11 @@ __global__ __launch_bounds__(C::NT, 2) void gff_gate_kernel(GateParams p) {
             if (BWD) {
                 da[r] = dh[i][0][r] * ab[i][1][r] * dy;
                 db[r] = dh[i][0][r] * y;
+            }
+            if (C::F16) {
+                hh[r] *= sh;
+                da[r] *= sd;
+                db[r] *= sd;
             }
         }
         if (cb + 32 > p.f || rb + 32 > p.M) {                                      // what lies past the matrix is stored as zeros
@@ -426,10 +494,10 @@ __global__ __launch_bounds__(C::NT, 2) void gff_gate_kernel(GateParams p) {
         }
         __bf16 *h = p.h + rb * p.fp + cb, *d = BWD ? p.dab + rb * 2 * p.fp + cb : nullptr;
         const int fp = (int)p.fp;
-        turn_tile(hh, S, [&](int r, int c, float4 v) { put_pieces<NP>(h + (r * fp + c), p.h_ps, v); });
+        turn_tile(hh, S, [&](int r, int c, float4 v) { put_pieces<NP, C::F16>(h + (r * fp + c), p.h_ps, v); });
         if (BWD) {
-            turn_tile(da, S, [&](int r, int c, float4 v) { put_pieces<NP>(d + (r * 2 * fp + c), p.dab_ps, v); });
-            turn_tile(db, S, [&](int r, int c, float4 v) { put_pieces<NP>(d + (r * 2 * fp + fp + c), p.dab_ps, v); });
+            turn_tile(da, S, [&](int r, int c, float4 v) { put_pieces<NP, C::F16>(d + (r * 2 * fp + c), p.dab_ps, v); });
+            turn_tile(db, S, [&](int r, int c, float4 v) { put_pieces<NP, C::F16>(d + (r * 2 * fp + fp + c), p.dab_ps, v); });
         }
     }
 }
@@ -439,12 +507,13 @@ struct NtParams {
     Planes a, b;
     void *c;
     int64_t ldc, M, N, K;
-    int ncol, ntiles, vec;
+    int ncol, ntiles, vec, which;
+    const float *norm;
 };
 template <int DT, typename C, int BM, int BN>
 __global__ __launch_bounds__(C::NT, 2) void gff_nt_kernel(NtParams p) {
     constexpr int NP = C::NP, RM = BM / C::WM, RN = BN / C::WN, TM = RM / 32, TN = RN / 32, GRID = C::WM * C::WN;
-    typedef typename ElemOf<DT>::type E;
+    typedef typename FfElem<DT>::type E;
     typedef NtTile<C, BM> TA;
     typedef NtTile<C, BN> TB;
     constexpr int POOL = C::NBUF * NP * (TA::IMG + TB::IMG), TURN = GRID * (4096 + (C::WK - 1) * TM * TN * 4096);
@@ -481,12 +550,14 @@ __global__ __launch_bounds__(C::NT, 2) void gff_nt_kernel(NtParams p) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] += J[((i * TN + j) * 16 + r) * 64 + lane];
     }
+    const float back = C::F16 ? pow2_of(p.norm, p.which, -1) : 1.f;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int64_t rb = m0 + wm * RM + i * 32, cb = n0 + wn * RN + j * 32;
             turn_tile(acc[i][j], S, [&](int r, int c, float4 v) {
+                if (C::F16) v = make_float4(v.x * back, v.y * back, v.z * back, v.w * back);
                 if (rb + r < p.M) put_row4<E>((E *)p.c + (rb + r) * p.ldc, cb + c, p.N, p.vec, v);
             });
         }
@@ -502,7 +573,8 @@ struct TnParams {
     float *part;
     int64_t rows, half, valid, N, part_sz;
     int64_t kt, kt_split;
-    int ncol, ntiles, splits, vec;
+    int ncol, ntiles, splits, vec, which;
+    const float *norm;
 };
 struct TnPair { TnParams p[2]; int blk; };
 template <int DT, typename C, int BM, int BN>
@@ -530,12 +602,14 @@ __global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnPair pair) {
                  [&](const unsigned char *img, int i, int ks) { return frag_tn<BM>(img, wm * RM + i * 32, ks, lane); },
                  [&](const unsigned char *img, int j, int ks) { return frag_tn<BN>(img, wn * RN + j * 32, ks, lane); });
     float *S = reinterpret_cast<float *>(pool) + wave * 1024;
+    const float back = C::F16 ? pow2_of(p.norm, p.which, -1) : 1.f;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int64_t rb = m0 + wm * RM + i * 32, cb = n0 + wn * RN + j * 32;
             turn_tile(acc[i][j], S, [&](int r, int c, float4 v) {
+                if (C::F16) v = make_float4(v.x * back, v.y * back, v.z * back, v.w * back);
                 int64_t row = rb + r;
                 const bool second = row >= p.half;
                 row -= second ? p.half : 0;
@@ -582,8 +656,9 @@ struct PackJobs { PackJob j[8]; int n; };
 
 template <int DT>
 __global__ __launch_bounds__(256) void gff_pack_kernel(PackJobs jobs) {
-    typedef typename ElemOf<DT>::type E;
-    constexpr int NP = ElemOf<DT>::NP;
+    typedef typename FfElem<DT>::type E;
+    constexpr int NP = FfElem<DT>::NP;
+    constexpr bool F16 = FfElem<DT>::F16;
     __shared__ float tile[64][65];
     int k = 0;
     while (k + 1 < jobs.n && (int)blockIdx.x >= jobs.j[k + 1].blk0) ++k;
@@ -611,7 +686,7 @@ __global__ __launch_bounds__(256) void gff_pack_kernel(PackJobs jobs) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (r0 + 16 * i < J.R && c0 < J.wide)
-                put_pieces<NP>(J.dst + (int64_t)(r0 + 16 * i) * J.ldd + c0, J.ps, make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
+                put_pieces<NP, F16>(J.dst + (int64_t)(r0 + 16 * i) * J.ldd + c0, J.ps, make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
         return;
     }
 #pragma unroll
@@ -623,7 +698,7 @@ __global__ __launch_bounds__(256) void gff_pack_kernel(PackJobs jobs) {
     for (int i = 0; i < 4; ++i) {
         const int c = bx * 64 + tr + 16 * i, r = by * 64 + tc;                 // row and column of the result
         if (c < J.C && r < J.wide)
-            put_pieces<NP>(J.dst + (int64_t)c * J.ldd + r, J.ps,
+            put_pieces<NP, F16>(J.dst + (int64_t)c * J.ldd + r, J.ps,
                            make_float4(tile[tc][tr + 16 * i], tile[tc + 1][tr + 16 * i], tile[tc + 2][tr + 16 * i], tile[tc + 3][tr + 16 * i]));
     }
 }
@@ -790,13 +865,13 @@ struct GffPlan {
     TnPlan gu, wd;                       // the weight gradients of [gate; up] and down
     int64_t off[16], bytes;              // workspace: byte offsets
 };
-enum { O_X, O_WG, O_WU, O_WD, O_H, O_DY, O_WDT, O_WGUT, O_DAB, O_PART, O_PART_WD };
+enum { O_X, O_WG, O_WU, O_WD, O_H, O_DY, O_WDT, O_WGUT, O_DAB, O_PART, O_PART_WD, O_NORM };
 
 static bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
-// A bfloat16 matrix whose k is whole k-tiles is an operand as it lies; every other one is packed into the workspace.
+// A 16-bit matrix whose k is whole k-tiles is an operand as it lies; every other one is packed into the workspace.
 static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
-    p.NP = a->dtype == ASR_T_F32 ? 3 : a->dtype == ASR_T_F16 ? 2 : 1;
+    p.NP = a->dtype == ASR_T_F32 ? 3 : 1;
     p.dp = up_to(a->d, 64);
     p.np = up_to(a->n, 64);
     p.fp = up_to(a->f, 64);
@@ -816,6 +891,7 @@ static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
     take(O_WG, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * e);
     take(O_WU, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * e);
     take(O_H, p.Mp * p.fp * e);
+    take(O_NORM, a->dtype == ASR_T_F16 ? N_COUNT * NORM_BLOCKS * 4 : 0);
     take(O_WD, p.direct_wd || bwd ? 0 : (int64_t)a->n * p.fp * e);
     if (bwd) {
         take(O_DY, p.direct_dy ? 0 : a->M * p.np * e);
@@ -891,12 +967,16 @@ static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, i
 // and 128 x 128 the LDS was the bound, its writes and reads as long as the matrix work (8192 x 1024 x 4096 bfloat16: 133 us
 // a product, 75 without loads and LDS writes).  Several pieces: three to six products an LDS byte, 128 x 128 with four waves.
 // Smaller tiles where larger ones would leave compute units without one.
-typedef GemmCfg<1, 64, 2, 2, 512, 2, 4> CfgBig;             // 256 x 256
-typedef GemmCfg<1, 32, 2, 2, 512, 2, 4> CfgGate;            // gate tiles of 256 x 128
-template <int NP> struct CfgMid { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 512, 4, 2> T; };             // 256 x 128
-template <int NP> struct CfgHalf { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 512, 1, 4, 2> T; };      // 96 x 128, two grids of waves
-template <int NP> struct CfgSmall { typedef GemmCfg<NP, NP == 1 ? 64 : 32, NP == 1 ? 2 : 1, NP == 1 ? 2 : 1, 256, 2, 2> T; };
-template <int NP> struct CfgDeep { typedef GemmCfg<NP, NP == 1 ? 64 : 32, 2, 2, 256, 2, 2> T; };
+template <int DT> struct Cfg {
+    static constexpr int NP = FfElem<DT>::NP, BK = NP == 1 ? 64 : 32;
+    static constexpr bool F16 = FfElem<DT>::F16;
+    typedef GemmCfg<1, 64, 2, 2, 512, 2, 4, 1, F16> Big;                            // 256 x 256, one piece
+    typedef GemmCfg<1, 32, 2, 2, 512, 2, 4, 1, F16> Gate;                           // gate tiles of 256 x 128, one piece
+    typedef GemmCfg<NP, BK, 2, 2, 512, 4, 2, 1, F16> Mid;                           // 256 x 128
+    typedef GemmCfg<NP, BK, 2, 2, 512, 1, 4, 2, F16> Half;                          // 96 x 128, two grids of waves
+    typedef GemmCfg<NP, BK, NP == 1 ? 2 : 1, NP == 1 ? 2 : 1, 256, 2, 2, 1, F16> Small;
+    typedef GemmCfg<NP, BK, 2, 2, 256, 2, 2, 1, F16> Deep;
+};
 
 template <int DT, typename C, int BM, int BN>
 static int gff_nt_go(NtParams &p, hipStream_t st) {
@@ -907,9 +987,9 @@ static int gff_nt_go(NtParams &p, hipStream_t st) {
     return ASR_OK;
 }
 template <int DT>
-static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t N, int64_t K, hipStream_t st) {
-    constexpr int NP = ElemOf<DT>::NP;
-    NtParams p{a, b, c, N, M, N, K, 0, 0, (int)(N % 4 == 0 && aligned16(c))};
+static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t N, int64_t K, int which, const float *norm, hipStream_t st) {
+    constexpr int NP = FfElem<DT>::NP;
+    NtParams p{a, b, c, N, M, N, K, 0, 0, (int)(N % 4 == 0 && aligned16(c)), which, norm};
     // The tile that is done first: the compute unit with most tiles has ceil(tiles / 256) of them; `rate` is the matrix work a
     // unit does in a time, `one` the share of it that a lone workgroup reaches where two or three are meant to share the unit
     // (from float32 products of 11968 x 256, k 2048 and 4096, bfloat16 ones of 8192 x 1024: 256 x 128 reaches 1.4 PFLOP/s
@@ -922,11 +1002,11 @@ static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t 
                  t128 = time(128, 64, 0.6, 0.7), t64 = time(64, 64, 0.55, 0.9);
     const double best = fmin(fmin(fmin(t256, tmid), fmin(t96, t128)), t64);
     if constexpr (NP == 1)
-        if (t256 == best) return gff_nt_go<DT, CfgBig, 256, 256>(p, st);
-    if (tmid == best) return gff_nt_go<DT, typename CfgMid<NP>::T, 256, 128>(p, st);
-    if (t96 == best) return gff_nt_go<DT, typename CfgHalf<NP>::T, 96, 128>(p, st);
-    if (t128 == best) return gff_nt_go<DT, typename CfgDeep<NP>::T, 128, 64>(p, st);
-    return gff_nt_go<DT, typename CfgDeep<NP>::T, 64, 64>(p, st);
+        if (t256 == best) return gff_nt_go<DT, typename Cfg<DT>::Big, 256, 256>(p, st);
+    if (tmid == best) return gff_nt_go<DT, typename Cfg<DT>::Mid, 256, 128>(p, st);
+    if (t96 == best) return gff_nt_go<DT, typename Cfg<DT>::Half, 96, 128>(p, st);
+    if (t128 == best) return gff_nt_go<DT, typename Cfg<DT>::Deep, 128, 64>(p, st);
+    return gff_nt_go<DT, typename Cfg<DT>::Deep, 64, 64>(p, st);
 }
 
 template <typename C, int BM, int BN, bool BWD>
@@ -939,19 +1019,19 @@ static int gff_gate_go(GateParams &g, hipStream_t st) {
 }
 template <int DT, bool BWD>
 static int gff_gate(GateParams &g, hipStream_t st) {
-    constexpr int NP = ElemOf<DT>::NP;
+    constexpr int NP = FfElem<DT>::NP;
     const int64_t rows = cdiv(g.Mp, 256);
     if constexpr (NP == 1) {
         // One piece is bound by the LDS: a wave's 128 x 32 of each product reads 16 B per matrix instruction less than 64 x 32
         // (8192 x 1024 x 4096: 298 -> 274 us with dh, 170 -> 163 us without; k-tiles of 64 would spill, 351 us).  A unit's
         // rounds of these tiles against those of half their size:
         const int64_t wide = (rows * (g.fp / 128) + 255) / 256, narrow = (rows * (g.fp / 64) + 255) / 256;
-        if (g.fp % 128 == 0 && 1.85 * (double)wide <= (double)narrow) return gff_gate_go<CfgGate, 256, 128, BWD>(g, st);
+        if (g.fp % 128 == 0 && 1.85 * (double)wide <= (double)narrow) return gff_gate_go<typename Cfg<DT>::Gate, 256, 128, BWD>(g, st);
     }
-    if (rows * (g.fp / 64) >= 256) return gff_gate_go<typename CfgMid<NP>::T, 256, 64, BWD>(g, st);
+    if (rows * (g.fp / 64) >= 256) return gff_gate_go<typename Cfg<DT>::Mid, 256, 64, BWD>(g, st);
     // (1003 x 200 x 683 float16, 88 tiles of 128 x 64: 25 and 17.5 us, in tiles of 64 x 64 16.3 and 11.9)
-    if ((int64_t)cdiv(g.Mp, 128) * (g.fp / 64) < 256) return gff_gate_go<typename CfgDeep<NP>::T, 64, 64, BWD>(g, st);
-    return gff_gate_go<typename CfgSmall<NP>::T, 128, 64, BWD>(g, st);
+    if ((int64_t)cdiv(g.Mp, 128) * (g.fp / 64) < 256) return gff_gate_go<typename Cfg<DT>::Deep, 64, 64, BWD>(g, st);
+    return gff_gate_go<typename Cfg<DT>::Small, 128, 64, BWD>(g, st);
 }
 
 template <int DT, typename C, int BM, int BN>
@@ -971,9 +1051,8 @@ static void gff_tn_go(TnPair &pair, int n, int64_t M, hipStream_t st) {
 // n = 1 or 2 products with the same tile
 template <int DT>
 static int gff_tn(TnPair &pair, int n, int big, int64_t M, hipStream_t st) {
-    constexpr int NP = ElemOf<DT>::NP;
-    if (big) gff_tn_go<DT, typename CfgMid<NP>::T, 256, 128>(pair, n, M, st);
-    else gff_tn_go<DT, typename CfgSmall<NP>::T, 128, 128>(pair, n, M, st);
+    if (big) gff_tn_go<DT, typename Cfg<DT>::Mid, 256, 128>(pair, n, M, st);
+    else gff_tn_go<DT, typename Cfg<DT>::Small, 128, 128>(pair, n, M, st);
     ASR_CHECK_LAUNCH("gff_tn_kernel");
     TnPair sums{};
     int m = 0, blocks = 0;
@@ -1031,17 +1110,22 @@ static int gff_run(const asr_gated_ff_args *a, bool bwd, hipStream_t st) {
         hipLaunchKernelGGL((gff_pack_kernel<DT>), dim3((unsigned)blocks), dim3(256), 0, st, jobs);
         ASR_CHECK_LAUNCH("gff_pack_kernel");
     }
-    GateParams g{x, wg, wu, dy, wdt, (__bf16 *)h.p, (__bf16 *)dab.p, h.ps, dab.ps, a->M, p.Mp, p.fp, a->f, (int)p.dp, (int)p.np, 0, 0, a->act};
+    float *norm = (float *)at(O_NORM);
+    if constexpr (DT == ASR_T_F16) {
+        hipLaunchKernelGGL(gff_norm_kernel, dim3(NORM_BLOCKS, bwd ? N_COUNT : N_DY), dim3(256), 0, st, NormJobs{{x, wg, wu, dy, wdt}}, norm);
+        ASR_CHECK_LAUNCH("gff_norm_kernel");
+    }
+    GateParams g{x, wg, wu, dy, wdt, (__bf16 *)h.p, (__bf16 *)dab.p, h.ps, dab.ps, a->M, p.Mp, p.fp, a->f, (int)p.dp, (int)p.np, 0, 0, a->act, norm};
     if (!bwd) {
         ASR_CHECK((gff_gate<DT, false>(g, st)));
-        return gff_nt<DT>(h, wd, a->y, a->M, a->n, p.fp, st);
+        return gff_nt<DT>(h, wd, a->y, a->M, a->n, p.fp, S_H, norm, st);
     }
     ASR_CHECK((gff_gate<DT, true>(g, st)));
-    if (a->dx) ASR_CHECK(gff_nt<DT>(dab, wgut, a->dx, a->M, a->d, 2 * p.fp, st));
+    if (a->dx) ASR_CHECK(gff_nt<DT>(dab, wgut, a->dx, a->M, a->d, 2 * p.fp, S_DAB, norm, st));
     const TnParams gu{dab, x, a->dwg, a->dwu, p.gu.splits > 1 ? (float *)at(O_PART) : nullptr, 2 * p.fp, p.fp, a->f, a->d, 2ll * a->f * a->d, 0, 0, 0, 0,
-                      p.gu.splits, (int)(a->d % 4 == 0 && aligned16(a->dwg) && aligned16(a->dwu))};
+                      p.gu.splits, (int)(a->d % 4 == 0 && aligned16(a->dwg) && aligned16(a->dwu)), S_DAB, norm};
     const TnParams down{dy, h, a->dwd, nullptr, p.wd.splits > 1 ? (float *)at(O_PART_WD) : nullptr, a->n, up_to(a->n, 256), a->n, a->f, (int64_t)a->n * a->f,
-                        0, 0, 0, 0, p.wd.splits, (int)(a->f % 4 == 0 && aligned16(a->dwd))};
+                        0, 0, 0, 0, p.wd.splits, (int)(a->f % 4 == 0 && aligned16(a->dwd)), S_H, norm};
     TnPair both{{gu, down}, 0}, one{{gu}, 0}, other{{down}, 0};
     if (a->dwg && a->dwd && !p.gu.big && !p.wd.big) return gff_tn<DT>(both, 2, 0, a->M, st);
     if (a->dwg) ASR_CHECK(gff_tn<DT>(one, 1, p.gu.big, a->M, st));

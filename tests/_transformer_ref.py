@@ -46,29 +46,33 @@ def gated_ff64(x, wg, wu, wd, dy, kind, dtype):
     """Float64 block and gradients with their tolerances: a list of (value, tolerance).
 
     u_h: half step of what h, da and db are kept in between the products; drop: what the products leave out of a term
-    (pieces.h: 2^-24 for each of two dropped products and for the rest behind three pieces, one dropped product of two
-    halves of at most 2^-8 for two pieces); every sum of n terms in float32 is off by at most n u of the sum of its terms'
-    sizes."""
+    (pieces.h: 2^-24 for each of two dropped products and for the rest behind three pieces; up to 64 rows without gradients
+    float16 has two pieces, one dropped product of two halves of at most 2^-8); every sum of n terms in float32 is off by at
+    most n u of the sum of its terms' sizes.  float16 h, da and db are kept times a power of two that brings a bound on them
+    above 2^14: a value below the normal numbers is off by half of 2^-24, 2^-39 of the bound."""
     u = U[dtype]
     u_h, drop = {torch.float32: (2.0 ** -24, 3 * 2.0 ** -24), torch.bfloat16: (2.0 ** -8, 0.0),
-                 torch.float16: (2.0 ** -16, 2.0 ** -16)}[dtype]
+                 torch.float16: (2.0 ** -11, 2.0 ** -16)}[dtype]
     d, f, n, M = x.shape[1], wg.shape[0], wd.shape[0], x.shape[0]
     a, b = x @ wg.t(), x @ wu.t()
     ea, eb = ((d * U32 + drop) * (x.abs() @ w.abs().t()) for w in (wg, wu))
     act, slope = act64(a, kind)
     h = act * b
+    low = 2.0 ** -39 if dtype == torch.float16 else 0.0
+    norm_x, norm_g, norm_u = (t.norm(dim=1).max() for t in (x, wg, wu))
     own = 16 * U32                                        # exp, reciprocal or erf and the products around them
     slope_max = 1.13                                      # the largest slope of either activation; of the slope, 1.0
     eact, eslope = slope_max * ea + own * (act.abs() + a.abs() * slope.abs()), ea + own * (1 + a.abs())
-    eh = eact * b.abs() + act.abs() * eb + eact * eb + (u_h + U32) * h.abs()
+    eh = eact * b.abs() + act.abs() * eb + eact * eb + (u_h + U32) * h.abs() + low * norm_x ** 2 * norm_g * norm_u
     y = h @ wd.t()
     out = [(y, eh @ wd.abs().t() + (f * U32 + drop) * (h.abs() @ wd.abs().t()))]
     if dy is not None:
         dh = dy @ wd
         edh = (n * U32 + drop) * (dy.abs() @ wd.abs())
         da, db = dh * b * slope, dh * act
-        eda = (edh * (b * slope).abs() + eb * (dh * slope).abs() + eslope * (dh * b).abs()) * 1.01 + (u_h + 4 * U32) * da.abs()
-        edb = (edh * act.abs() + eact * dh.abs()) * 1.01 + (u_h + 2 * U32) * db.abs()
+        low = low * 1.13 * dy.norm(dim=1).max() * wd.norm(dim=0).max() * norm_x * torch.maximum(norm_g, norm_u)
+        eda = (edh * (b * slope).abs() + eb * (dh * slope).abs() + eslope * (dh * b).abs()) * 1.01 + (u_h + 4 * U32) * da.abs() + low
+        edb = (edh * act.abs() + eact * dh.abs()) * 1.01 + (u_h + 2 * U32) * db.abs() + low
         s = M * U32 + drop
         out.append((da @ wg + db @ wu, eda @ wg.abs() + edb @ wu.abs()
                     + (2 * f * U32 + drop) * (da.abs() @ wg.abs() + db.abs() @ wu.abs())))

@@ -54,6 +54,28 @@ def test_tiles_of_every_width(M, d, f, n):
     _check(*_inputs(M, d, f, n, torch.float16))
 
 
+@pytest.mark.parametrize("M", [70, 300])
+@pytest.mark.parametrize("xs,ws,ds,gs", [(60.0, 1.0, 1e-3, 1.0), (200.0, 4.0, 1e-4, 1e-4), (1e-6, 1.0, 1.0, 1e-6), (1.0, 1e-3, 1.0, 3e-7), (0.0, 1.0, 1.0, 1.0),
+                                         (1.0, 1.0, 0.0, 1.0), (1.0, 1.0, 1.0, 0.0), (1.0, 100.0, 1e-3, 50.0)])
+def test_float16_hidden_values_out_of_its_range(M, xs, ws, ds, gs):
+    """h, da and db far above the largest float16 and below its normal numbers, where y and gradients may be neither."""
+    x, wg, wu, wd, dy = _inputs(M, 64, 96, 40, torch.float32)
+    _check(*[(t.float() * s).to(torch.float16) for t, s in ((x, xs), (wg, ws), (wu, ws), (wd, ds), (dy, gs))])
+
+
+def test_float16_rows_with_infinities_leave_the_others():
+    from asr_amd.Models.transformer_ops import gated_feed_forward
+    x, wg, wu, wd, _ = _inputs(130, 64, 96, 40, torch.float16)
+    want = gated_feed_forward(x, wg, wu, wd)
+    bad = x.clone()
+    bad[3, 5], bad[77, 0], bad[129, 63] = float("inf"), float("nan"), -float("inf")
+    got = gated_feed_forward(bad, wg, wu, wd)
+    rest = torch.ones(130, dtype=torch.bool, device=x.device)
+    rest[[3, 77, 129]] = False
+    close = (got[rest].float() - want[rest].float()).abs() <= 2.0 ** -10 * want[rest].float().abs() + 2.0 ** -9 * float(want.abs().max())
+    assert bool(close.all()) and not got[~rest].isfinite().any()
+
+
 def test_many_tiles_and_split_sums():
     _check(*_inputs(3000, 128, 256, 128, torch.bfloat16))
     _check(*_inputs(2100, 64, 192, 96, torch.float32))
