@@ -19,6 +19,7 @@
 //                                  weight gradients 124 each on average (0.83)
 //   float32 11968 x 256 x 2048     gate 178 (0.85), backward 329 (0.69; without its 441 MB of stores 261), y and dx 133 (0.85),
 //                                  weight gradients 107 (1.06)
+//   float16 3000 x 1024 x 4096     a training call 431 us, bfloat16 392 (float16 as two bf16 pieces, three products: 918)
 //   bfloat16 8 x 1024 x 4096       8.3 + 5.2 + 2.3 us in three launches: 25 MB of weights at 1.6 TB/s, three waits long
 // Rows and columns beyond the matrix are read from its last row (clamped) and masked in the epilogues; the arrays h, da, db
 // are padded to whole tiles with zeros, which is what the products over them read past the end.

@@ -118,7 +118,7 @@ def attention64(q, k, v, table, g, dtype, *, lengths, keep, offset, causal, reac
     """Float64 attention and gradients with tolerances: [(value, tolerance)] for out, dq, dk, dv, dtable.
 
     drop / u_p: what the products leave out of a term and the half step of the probabilities and score gradients between two
-    products, by type (pieces.h; bfloat16 probabilities carry 16 bits in training).  A score's absolute error es (its product,
+    products, by type (pieces.h; bfloat16 probabilities carry at least 16 bits in training's forward).  A score's absolute error es (its product,
     the bias and scale in base 2) makes a relative error es of its probability; one exponential, the sum's roundings and
     the quotient add `own`."""
     B, Tq, H, D = q.shape
