@@ -235,6 +235,7 @@ def native():
     """The module of torch bindings (csrc/transformer_ops.cpp), loaded once; raises if it is missing."""
     global _native
     if _native is None:
+        import torch  # noqa: F401  (its libraries first: the module needs them)
         load()
         if not os.path.exists(NATIVE_PATH):
             raise RuntimeError(f"asr_amd: {NATIVE_PATH} not found -- the native module is required (run `make` in the repo root); "
