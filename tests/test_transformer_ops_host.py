@@ -89,6 +89,13 @@ def test_c_abi_refusals():
         _refused("asr_gated_ff_bwd", ff(), **change)
 
 
+def test_native_module_loads_by_itself():
+    import subprocess
+    import sys
+    code = "from asr_amd import _lib; m = _lib.native(); assert m.rope and m.attention and m.ff"
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
 def test_encoder_options():
     from asr_amd.Models.AttModel import AttModel
     from asr_amd.Models.Transformer_encoder import TransformerEncoder
