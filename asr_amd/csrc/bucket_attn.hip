@@ -24,7 +24,7 @@
 //
 // Measured, rates in bf16 matrix operations: bfloat16 2 x 4096 causal, 16 heads of 128 on 2: forward 332 us (0.41 PFLOP/s of
 // the formula, 0.83 with the further pieces of P), dQ 349 (0.59; 0.79), dK and dV 460 (0.60); float32 32 x 374, 4 heads of 64, half
-// to whole lengths: 45, 64 and 86 us (0.6 to 0.7 of six products a product of the padded maps), packing 18 us a pass at 5.1 TB/s.
+// to whole lengths: 44, 64 and 67 us (0.63 to 0.82 PFLOP/s of six products a product over padded maps), packing 18 us a pass at 5.1 TB/s.
 #include "pieces.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -341,7 +341,7 @@ __device__ __forceinline__ int keys_of(const AttnParams &p, int b) {
 // 3.8e-6 in dtable instead of 6e-7.  The returned O is
 // rounded to 16 bits once.
 template <int DT, int DP, bool TRAIN>
-__global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 128 ? 1 : 2) void battn_fwd_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 192 ? 1 : 2) void battn_fwd_kernel(AttnParams p) {
     constexpr int NP = ElemOf<DT>::NP, W = NP == 1 && TRAIN ? 3 : NP, KT = KeyTile<NP>::N;
     typedef typename ElemOf<DT>::type E;
     typedef RowTile<NP, DP, KT> Tile;
@@ -628,8 +628,12 @@ __global__ __launch_bounds__(64) void battn_table_kernel(const float *__restrict
 }
 
 // ---------------------------------------------------------------------------------------------------- dK and dV --
+// Two workgroups a compute unit where 256 registers do: with several pieces that takes loading each tile when it is due (the
+// other workgroup hides the wait) and dP behind dV instead of beside S (float32 at 32 x 374, 4 heads of 64: 87 us with one
+// workgroup and tiles loaded ahead, 77 with two that spill them, 67).  One piece of D = 128 would still spill (465 -> 660 us).
+template <int NP, int DP> struct DkvTwo { static constexpr bool V = NP == 1 ? DP <= 64 : NP * DP <= 192; };
 template <int DT, int DP>
-__global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 2 : 1) void battn_dkv_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, (DkvTwo<ElemOf<DT>::NP, DP>::V ? 2 : 1)) void battn_dkv_kernel(AttnParams p) {
     constexpr int NP = ElemOf<DT>::NP, QT = KeyTile<NP>::N;
     typedef typename ElemOf<DT>::type E;
     typedef RowTile<NP, DP, QT> Tile;
@@ -670,18 +674,24 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 
                 const int i = t0 + (threadIdx.x & (QT - 1));
                 if (threadIdx.x < 2 * QT) st = i >= p.Tq ? (threadIdx.x < QT ? INFINITY : 0.f) : (threadIdx.x < QT ? lse : del)[i];
             };
-            if (i0 < p.Tq) {
+            constexpr bool AHEAD = NP == 1 || !DkvTwo<NP, DP>::V;
+            if (AHEAD && i0 < p.Tq) {
                 qt.load(i0, p.Tq, p.D, nullptr);
                 gt.load(i0, p.Tq, p.D, nullptr);
                 load_stat(i0);
             }
             for (int t0 = i0; t0 < p.Tq; t0 += QT) {
+                if (!AHEAD) {
+                    qt.load(t0, p.Tq, p.D, nullptr);
+                    gt.load(t0, p.Tq, p.D, nullptr);
+                    load_stat(t0);
+                }
                 __syncthreads();
                 qt.store(qi);
                 gt.store(gi);
                 if (threadIdx.x < 2 * QT) stat[threadIdx.x] = st;
                 __syncthreads();
-                if (t0 + QT < p.Tq) {
+                if (AHEAD && t0 + QT < p.Tq) {
                     qt.load(t0 + QT, p.Tq, p.D, nullptr);
                     gt.load(t0 + QT, p.Tq, p.D, nullptr);
                     load_stat(t0 + QT);
@@ -740,10 +750,10 @@ __global__ __launch_bounds__(256, (ElemOf<DT>::NP == 1 ? DP <= 64 : DP <= 32) ? 
                         qc.dot(dk, f);
                     } else {
                         dot_rows<NP, DP>(s[0], qi, Tile::IMG, s0, kf, lane);
-                        dot_rows<NP, DP>(dp[0], gi, Tile::IMG, s0, vf, lane);
                         weigh(s[0], s0);
                         to_operand<NP>(f, s[0]);
                         dot_cols<NP, NP, DP>(dv, gi, Tile::IMG, s0, f, lane);
+                        dot_rows<NP, DP>(dp[0], gi, Tile::IMG, s0, vf, lane);
                         slope(dp[0], s[0], s0);
                         to_operand<NP>(f, dp[0]);
                         dot_cols<NP, NP, DP>(dk, qi, Tile::IMG, s0, f, lane);
