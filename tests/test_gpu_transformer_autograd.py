@@ -1,5 +1,5 @@
 """GPU: the encoder-layer operators as autograd nodes: leaves that need no gradient, outputs nobody uses, graphs of gradients,
-backward passes from two threads' engines, tensors changed or freed in between, other devices' refusals."""
+leaves changed before the backward, checkpoints, backward passes from several threads."""
 import pytest
 import torch
 
