@@ -203,7 +203,7 @@ ACTIVATIONS = {"swish": 0, "gelu": 1}
 def gated_feed_forward(x, w_gate, w_up, w_down, act="swish"):
     """(act(x w_gate^T) * (x w_up^T)) w_down^T over the last axis of x: w_gate and w_up (f, d), w_down (n, f), no biases; act
     "swish" or "gelu" (the exact one).  All four of one type.  The hidden values are formed in float32 and rounded once for
-    the second product (to 8 bits for bfloat16, 11 for float16, 24 for float32, never out of range).  The backward keeps only the inputs and
+    the second product (to 8 bits for bfloat16, at least 11 for float16, 24 for float32, never out of range).  The backward keeps only the inputs and
     forms the hidden values again.  Up to 64 rows without gradients take a form that reads the weights once."""
     who = "gated_feed_forward"
     if not isinstance(x, torch.Tensor) or x.dim() < 1:

@@ -7,8 +7,8 @@
 //           3  dWg, dWu = [da db]^T x,  dWd = dy^T h                                           (gff_tn_kernel, split over M)
 // Nothing but x is kept for the backward: computing a and b again costs 4 M d f operations of 22 and saves writing and
 // reading two M x f arrays each way; it also keeps act' on unrounded a and b.  h, da and db are rounded once to the
-// stored type's own precision (bfloat16 2^-8, float16 2^-11 relative half step, float32 three pieces of pieces.h, 2^-24) because
-// the next product reads them as matrix operands.
+// stored type's own precision (bfloat16 2^-8, float16 2^-11 or, as pieces, 2^-16 relative half step, float32 three pieces of pieces.h,
+// 2^-24) because the next product reads them as matrix operands.
 //
 // Gate and up columns are interleaved by 32, so that a wave holds a and b of the same elements; products are
 // v_mfma_f32_32x32x16_bf16 over tiles of 256 rows and eight waves where there are enough of them (the tiles of each product
@@ -34,10 +34,14 @@ typedef short s16x8g __attribute__((ext_vector_type(8)));
 
 enum { GFF_SWISH = 0, GFF_GELU = 1 };
 
-// float16 operands go into v_mfma_f32_32x32x16_f16 as they lie, one product like bfloat16
-template <int DT> struct FfElem : ElemOf<DT> {
-    static constexpr int NP = DT == ASR_T_F32 ? 3 : 1;
-    static constexpr bool F16 = DT == ASR_T_F16;
+// float16 operands go into v_mfma_f32_32x32x16_f16 as they lie, one product like bfloat16 (F16_AS_IS), or as two pieces of
+// bfloat16, three products; gff_native says which
+#define F16_AS_IS 3
+template <int DT> struct FfElem : ElemOf<DT> { static constexpr bool F16 = false; };
+template <> struct FfElem<F16_AS_IS> {
+    typedef _Float16 type;
+    static constexpr int NP = 1;
+    static constexpr bool F16 = true;
 };
 template <bool F16>
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
@@ -583,7 +587,7 @@ __global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnPair pair) {
     const TnParams &p = pair.p[(int)blockIdx.x >= pair.blk];
     const int id = (int)blockIdx.x - ((int)blockIdx.x >= pair.blk ? pair.blk : 0), split = id / p.ntiles;
     constexpr int NP = C::NP, RM = BM / C::WM, RN = BN / C::WN, TM = RM / 32, TN = RN / 32;
-    typedef typename ElemOf<DT>::type E;
+    typedef typename FfElem<DT>::type E;
     typedef TnTile<C, BM> TA;
     typedef TnTile<C, BN> TB;
     constexpr int POOL = C::NBUF * NP * (TA::IMG + TB::IMG), TURN = C::NT / 64 * 4096;
@@ -626,7 +630,7 @@ __global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnPair pair) {
 }
 template <int DT, int V>
 __global__ __launch_bounds__(256) void gff_sum_kernel(TnPair pair) {
-    typedef typename ElemOf<DT>::type E;
+    typedef typename FfElem<DT>::type E;
     const bool second = (int)blockIdx.x >= pair.blk;
     const TnParams &p = pair.p[second];
     const int64_t n0 = p.valid * p.N, nblk = second ? (int)gridDim.x - pair.blk : min((int)gridDim.x, pair.blk), blk = (int)blockIdx.x - (second ? pair.blk : 0);
@@ -870,9 +874,16 @@ enum { O_X, O_WG, O_WU, O_WD, O_H, O_DY, O_WDT, O_WGUT, O_DAB, O_PART, O_PART_WD
 
 static bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
+// float16 as it lies rounds h, da and db to 11 bits and needs their scale; as pieces they keep 16 bits.  The forward takes it
+// always (3000 x 1024 x 4096: 110 us against 238; 374 x 256 x 2048: 22 against 42): y is off by 1.4 of its own rounding.  In
+// the backward two roundings that partly cancel make that up to 1.5, so it pays there only from some size on (a training call at
+// 1003 x 200 x 683: 106 us, in pieces 97; 4000 x 256 x 2048 160 and 250; 3000 x 1024 x 4096 431 and 918).
+static bool gff_native(const asr_gated_ff_args *a, bool bwd) {
+    return a->dtype == ASR_T_F16 && (!bwd || (double)a->M * a->d * a->f >= (double)(1 << 29));
+}
 // A 16-bit matrix whose k is whole k-tiles is an operand as it lies; every other one is packed into the workspace.
 static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
-    p.NP = a->dtype == ASR_T_F32 ? 3 : 1;
+    p.NP = a->dtype == ASR_T_F32 ? 3 : a->dtype == ASR_T_F16 && !gff_native(a, bwd) ? 2 : 1;
     p.dp = up_to(a->d, 64);
     p.np = up_to(a->n, 64);
     p.fp = up_to(a->f, 64);
@@ -892,7 +903,7 @@ static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
     take(O_WG, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * e);
     take(O_WU, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * e);
     take(O_H, p.Mp * p.fp * e);
-    take(O_NORM, a->dtype == ASR_T_F16 ? N_COUNT * NORM_BLOCKS * 4 : 0);
+    take(O_NORM, gff_native(a, bwd) ? N_COUNT * NORM_BLOCKS * 4 : 0);
     take(O_WD, p.direct_wd || bwd ? 0 : (int64_t)a->n * p.fp * e);
     if (bwd) {
         take(O_DY, p.direct_dy ? 0 : a->M * p.np * e);
@@ -1112,15 +1123,16 @@ static int gff_run(const asr_gated_ff_args *a, bool bwd, hipStream_t st) {
         ASR_CHECK_LAUNCH("gff_pack_kernel");
     }
     float *norm = (float *)at(O_NORM);
-    if constexpr (DT == ASR_T_F16) {
+    if constexpr (FfElem<DT>::F16) {
         hipLaunchKernelGGL(gff_norm_kernel, dim3(NORM_BLOCKS, bwd ? N_COUNT : N_DY), dim3(256), 0, st, NormJobs{{x, wg, wu, dy, wdt}}, norm);
         ASR_CHECK_LAUNCH("gff_norm_kernel");
     }
     GateParams g{x, wg, wu, dy, wdt, (__bf16 *)h.p, (__bf16 *)dab.p, h.ps, dab.ps, a->M, p.Mp, p.fp, a->f, (int)p.dp, (int)p.np, 0, 0, a->act, norm};
-    if (!bwd) {
-        ASR_CHECK((gff_gate<DT, false>(g, st)));
-        return gff_nt<DT>(h, wd, a->y, a->M, a->n, p.fp, S_H, norm, st);
-    }
+    if constexpr (DT != ASR_T_F16)                                                     // (as pieces only in the backward)
+        if (!bwd) {
+            ASR_CHECK((gff_gate<DT, false>(g, st)));
+            return gff_nt<DT>(h, wd, a->y, a->M, a->n, p.fp, S_H, norm, st);
+        }
     ASR_CHECK((gff_gate<DT, true>(g, st)));
     if (a->dx) ASR_CHECK(gff_nt<DT>(dab, wgut, a->dx, a->M, a->d, 2 * p.fp, S_DAB, norm, st));
     const TnParams gu{dab, x, a->dwg, a->dwu, p.gu.splits > 1 ? (float *)at(O_PART) : nullptr, 2 * p.fp, p.fp, a->f, a->d, 2ll * a->f * a->d, 0, 0, 0, 0,
@@ -1162,7 +1174,7 @@ extern "C" int asr_gated_ff_fwd(const asr_gated_ff_args *a, void *stream) {
     switch (a->dtype) {
         case ASR_T_F32: return few ? gff_few_pick<ASR_T_F32>(a, st) : gff_run<ASR_T_F32>(a, false, st);
         case ASR_T_BF16: return few ? gff_few_pick<ASR_T_BF16>(a, st) : gff_run<ASR_T_BF16>(a, false, st);
-        default: return few ? gff_few_pick<ASR_T_F16>(a, st) : gff_run<ASR_T_F16>(a, false, st);
+        default: return few ? gff_few_pick<ASR_T_F16>(a, st) : gff_run<F16_AS_IS>(a, false, st);
     }
 }
 
@@ -1174,6 +1186,6 @@ extern "C" int asr_gated_ff_bwd(const asr_gated_ff_args *a, void *stream) {
     switch (a->dtype) {
         case ASR_T_F32: return gff_run<ASR_T_F32>(a, true, st);
         case ASR_T_BF16: return gff_run<ASR_T_BF16>(a, true, st);
-        default: return gff_run<ASR_T_F16>(a, true, st);
+        default: return gff_native(a, true) ? gff_run<F16_AS_IS>(a, true, st) : gff_run<ASR_T_F16>(a, true, st);
     }
 }

@@ -6,6 +6,7 @@
 // x1 = bf16(x - x0), x2 = bf16(x - x0 - x1):
 //   bfloat16 : NP = 1, exact                       one product
 //   float16  : NP = 2, exact (11 bits = 8 + 3)     x0 y0 + x0 y1 + x1 y0: what is dropped is 2^-16 of a term
+//                                                  (attention's scores: all four, exact)
 //   float32  : NP = 3, exact (24 bits = 8 + 8 + 8) the six products x_i y_j with i + j <= 2: dropped 2^-24 of a term
 // bf16 has the exponent range of float32, so nothing over- or underflows on the way (float16 gradients in particular),
 // and six bf16 products cost 6/16 of the time of one exact fp32 product (v_mfma_f32_32x32x2_f32 runs at 1/16 of the bf16

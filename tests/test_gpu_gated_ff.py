@@ -47,19 +47,19 @@ def test_gelu(dtype):
     _check(*_inputs(7, 64, 100, 64, dtype, scale=3.0), act="gelu")
 
 
-@pytest.mark.parametrize("M,d,f,n", [(2060, 40, 2041, 33), (4000, 64, 2048, 64), (4100, 40, 2041, 33)])
+@pytest.mark.parametrize("M,d,f,n", [(2060, 40, 2041, 33), (4000, 64, 2048, 64), (4100, 40, 2041, 33), (2100, 200, 1500, 72), (8200, 64, 1030, 64)])
 def test_tiles_of_every_width(M, d, f, n):
     """16-bit products of enough tiles for the widest, with ragged last ones."""
     _check(*_inputs(M, d, f, n, torch.bfloat16))
     _check(*_inputs(M, d, f, n, torch.float16))
 
 
-@pytest.mark.parametrize("M", [70, 300])
+@pytest.mark.parametrize("M,d,f", [(70, 64, 96), (300, 64, 96), (2100, 256, 1024)])         # the last one as it lies in the backward too
 @pytest.mark.parametrize("xs,ws,ds,gs", [(60.0, 1.0, 1e-3, 1.0), (200.0, 4.0, 1e-4, 1e-4), (1e-6, 1.0, 1.0, 1e-6), (1.0, 1e-3, 1.0, 3e-7), (0.0, 1.0, 1.0, 1.0),
                                          (1.0, 1.0, 0.0, 1.0), (1.0, 1.0, 1.0, 0.0), (1.0, 100.0, 1e-3, 50.0)])
-def test_float16_hidden_values_out_of_its_range(M, xs, ws, ds, gs):
+def test_float16_hidden_values_out_of_its_range(M, d, f, xs, ws, ds, gs):
     """h, da and db far above the largest float16 and below its normal numbers, where y and gradients may be neither."""
-    x, wg, wu, wd, dy = _inputs(M, 64, 96, 40, torch.float32)
+    x, wg, wu, wd, dy = _inputs(M, d, f, 40, torch.float32)
     _check(*[(t.float() * s).to(torch.float16) for t, s in ((x, xs), (wg, ws), (wu, ws), (wd, ds), (dy, gs))])
 
 
