@@ -944,7 +944,8 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
         if (j0 + 32 < je) {
             load_v(j0 + 32);
         }
-        if (j0 + 31 - pmin <= -R || j0 - pmax >= R) {
+        // (by the tile's last real key, as `near` goes by the run's: a run without a table of buckets has no tile that reads it)
+        if (min(j0 + 31, je - 1) - pmin <= -R || j0 - pmax >= R) {
             const float bf = j0 - pmax >= R ? br : bl;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[0][r] = __builtin_fmaf(s[0][r], c, bf);
