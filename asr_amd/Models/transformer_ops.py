@@ -203,8 +203,9 @@ ACTIVATIONS = {"swish": 0, "gelu": 1}
 def gated_feed_forward(x, w_gate, w_up, w_down, act="swish"):
     """(act(x w_gate^T) * (x w_up^T)) w_down^T over the last axis of x: w_gate and w_up (f, d), w_down (n, f), no biases; act
     "swish" or "gelu" (the exact one).  All four of one type.  The hidden values are formed in float32 and rounded once for
-    the second product (to 8 bits for bfloat16, at least 11 for float16, 24 for float32, never out of range).  The backward keeps only the inputs and
-    forms the hidden values again.  Up to 64 rows without gradients take a form that reads the weights once."""
+    the second product, each by itself (to 8 bits for bfloat16, 16 for float16, 24 for float32; never out of range), and so are
+    their gradients.  The backward keeps only the inputs and forms the hidden values again.  Up to 64 rows the forward takes a
+    form that reads the weights once and keeps the hidden values to 16 bits for both 16-bit types, to 24 for float32."""
     who = "gated_feed_forward"
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise RuntimeError(f"asr_amd.{who}: x must be a tensor of at least one dimension")

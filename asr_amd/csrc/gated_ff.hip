@@ -6,9 +6,9 @@
 //           2  dx = [da db] [Wg; Wu]                                                           (gff_nt_kernel)
 //           3  dWg, dWu = [da db]^T x,  dWd = dy^T h                                           (gff_tn_kernel, split over M)
 // Nothing but x is kept for the backward: computing a and b again costs 4 M d f operations of 22 and saves writing and
-// reading two M x f arrays each way; it also keeps act' on unrounded a and b.  h, da and db are rounded once to the
-// stored type's own precision (bfloat16 2^-8, float16 2^-11 or, as pieces, 2^-16 relative half step, float32 three pieces of pieces.h,
-// 2^-24) because the next product reads them as matrix operands.
+// reading two M x f arrays each way; it also keeps act' on unrounded a and b.  h, da and db are rounded once, each by
+// itself, because the next product reads them as matrix operands (half a step relative to the value: bfloat16 2^-8, one piece of
+// pieces.h, which makes the outputs' error 1.4 of their own rounding; float16 2^-16, two; float32 2^-24, three).
 //
 // Gate and up columns are interleaved by 32, so that a wave holds a and b of the same elements; products are
 // v_mfma_f32_32x32x16_bf16 over tiles of 256 rows and eight waves where there are enough of them (the tiles of each product
@@ -19,7 +19,8 @@
 //                                  weight gradients 124 each on average (0.83)
 //   float32 11968 x 256 x 2048     gate 178 (0.85), backward 329 (0.69; without its 441 MB of stores 261), y and dx 133 (0.85),
 //                                  weight gradients 107 (1.06)
-//   float16 3000 x 1024 x 4096     a training call 431 us, bfloat16 392 (float16 as two bf16 pieces, three products: 918)
+//   float16 3000 x 1024 x 4096     a training call 739 us, without gradients 173 (bfloat16: training 392); with operands of
+//                                  the gate kernel in pieces too 918 and 238
 //   bfloat16 8 x 1024 x 4096       8.3 + 5.2 + 2.3 us in three launches: 25 MB of weights at 1.6 TB/s, three waits long
 // Rows and columns beyond the matrix are read from its last row (clamped) and masked in the epilogues; the arrays h, da, db
 // are padded to whole tiles with zeros, which is what the products over them read past the end.
@@ -34,8 +35,11 @@ typedef short s16x8g __attribute__((ext_vector_type(8)));
 
 enum { GFF_SWISH = 0, GFF_GELU = 1 };
 
-// float16 operands go into v_mfma_f32_32x32x16_f16 as they lie, one product like bfloat16 (F16_AS_IS), or as two pieces of
-// bfloat16, three products; gff_native says which
+// float16 operands of the gate kernel (x, Wg, Wu, dy, Wd) go into v_mfma_f32_32x32x16_f16 as they lie: one exact product, like
+// bfloat16 (F16_AS_IS).  What it forms from them, h, da and db, may leave the range of float16 where y and the gradients do not,
+// and one large row of x or dy must not cost the others bits, so the products over those take two bf16 pieces a value, three
+// products: 16 bits of every value by itself, over the range of float32.  (One power of two for a whole h, from the largest
+// row norms, would keep single products, but rows 8000 times smaller than the largest would lose 11 % of their y.)
 #define F16_AS_IS 3
 template <int DT> struct FfElem : ElemOf<DT> { static constexpr bool F16 = false; };
 template <> struct FfElem<F16_AS_IS> {
@@ -43,6 +47,7 @@ template <> struct FfElem<F16_AS_IS> {
     static constexpr int NP = 1;
     static constexpr bool F16 = true;
 };
+template <int DT> struct GateOperands { static constexpr int V = DT == ASR_T_F16 ? F16_AS_IS : DT; };
 template <bool F16>
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
     if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -373,45 +378,6 @@ __device__ __forceinline__ void tile_of(int id, int ntiles, int ncol, int &row, 
     col = t - row * ncol;
 }
 
-// ------------------------------------------------------------------------- powers of two for float16 h, da, db --
-// h, da and db may leave the range of float16 where y and the gradients do not (and gradients may be tiny), so they are kept
-// times a power of two that brings a bound on them to 2^15: |a_ij| <= |x_i| |wg_j|, likewise b and dh, |act(a)| <= |a| and
-// |act'(a)| <= 1.13.  The bound is above a typical value by about sqrt(d) each, so that is 2^-14 and more: normal numbers down to
-// 2^-15 of it.  gff_norm_kernel leaves the largest squared row norms by workgroup, the products' waves finish them.  Rows that
-// hold infinities or NaN do not count: what they reach is infinite or NaN anyway.
-#define NORM_BLOCKS 64
-enum { N_X, N_WG, N_WU, N_DY, N_WDT, N_COUNT };
-struct NormJobs { Planes m[N_COUNT]; };
-__global__ __launch_bounds__(256) void gff_norm_kernel(NormJobs jobs, float *out) {
-    __shared__ float red[4];
-    const Planes &m = jobs.m[blockIdx.y];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const _Float16 *p = reinterpret_cast<const _Float16 *>(m.p);
-    float top = 0.f;
-    for (int64_t r = blockIdx.x * 4 + wave; r < m.rows; r += NORM_BLOCKS * 4) {
-        float s = 0.f;
-        for (int64_t k = lane * 8; k < m.ld; k += 512) {
-            const f16x8 v = *reinterpret_cast<const f16x8 *>(p + r * m.ld + k);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s += (float)v[e] * (float)v[e];
-        }
-        s = wave_sum(s);
-        if (s < INFINITY) top = fmaxf(top, s);
-    }
-    if (lane == 0) red[wave] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) out[blockIdx.y * NORM_BLOCKS + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
-enum { S_NONE, S_H, S_DAB };
-// 2^(sign (15 - e)), e the exponent above the bound
-__device__ __forceinline__ float pow2_of(const float *n, int which, int sign) {
-    const int lane = threadIdx.x & 63;
-    auto top = [&](int k) { return wave_max(n[k * NORM_BLOCKS + lane]); };
-    const float x = top(N_X), g = top(N_WG), u = top(N_WU);
-    const float bound = which == S_H ? sqrtf(x * g) * sqrtf(x * u) : 1.13f * sqrtf(top(N_DY) * top(N_WDT)) * sqrtf(x * fmaxf(g, u));
-    return bound > 0.f ? ldexpf(1.f, sign * (15 - min(max(ilogbf(bound) + 1, -100), 100))) : 1.f;
-}
-
 // ------------------------------------------------------------------- a, b (and dh) of one tile, elementwise part --
 struct GateParams {
     Planes x, wg, wu;                    // x (M, dp), weights (f, dp)
@@ -420,11 +386,10 @@ struct GateParams {
     int64_t h_ps, dab_ps;
     int64_t M, Mp, fp;
     int f, dp, np, ncol, ntiles, act;
-    const float *norm;
 };
 
-// BM rows x BN columns of h: A tile of BM rows, B tile of 2 BN (gate and up rows interleaved), then of BN rows of Wd^T
-template <typename C, int BM, int BN, bool BWD>
+// BM rows x BN columns of h, in OP pieces: A tile of BM rows, B tile of 2 BN (gate and up rows interleaved), then of BN rows of Wd^T
+template <typename C, int OP, int BM, int BN, bool BWD>
 __global__ __launch_bounds__(C::NT, 2) void gff_gate_kernel(GateParams p) {
     constexpr int NP = C::NP, TM = BM / C::WM / 32, RM = BM / C::WM;
     static_assert(BN / C::WN == 32, "a wave has the gate and the up values of 32 columns");
@@ -461,11 +426,6 @@ __global__ __launch_bounds__(C::NT, 2) void gff_gate_kernel(GateParams p) {
     }
     float *S = reinterpret_cast<float *>(pool) + wave * 1024;
     const int64_t cb = n0 + wn * 32;
-    float sh = 1.f, sd = 1.f;
-    if constexpr (C::F16) {
-        sh = pow2_of(p.norm, S_H, 1);
-        if (BWD) sd = pow2_of(p.norm, S_DAB, 1);
-    }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int64_t rb = m0 + wm * RM + i * 32;
@@ -474,16 +434,11 @@ __global__ __launch_bounds__(C::NT, 2) void gff_gate_kernel(GateParams p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float y, dy;
-            act_both<NP == 1>(p.act, ab[i][0][r], y, dy);
+            act_both<OP == 1>(p.act, ab[i][0][r], y, dy);
             hh[r] = y * ab[i][1][r];
             if (BWD) {
                 da[r] = dh[i][0][r] * ab[i][1][r] * dy;
                 db[r] = dh[i][0][r] * y;
-            }
-            if (C::F16) {
-                hh[r] *= sh;
-                da[r] *= sd;
-                db[r] *= sd;
             }
         }
         if (cb + 32 > p.f || rb + 32 > p.M) {                                      // what lies past the matrix is stored as zeros
@@ -499,10 +454,10 @@ __global__ __launch_bounds__(C::NT, 2) void gff_gate_kernel(GateParams p) {
         }
         __bf16 *h = p.h + rb * p.fp + cb, *d = BWD ? p.dab + rb * 2 * p.fp + cb : nullptr;
         const int fp = (int)p.fp;
-        turn_tile(hh, S, [&](int r, int c, float4 v) { put_pieces<NP, C::F16>(h + (r * fp + c), p.h_ps, v); });
+        turn_tile(hh, S, [&](int r, int c, float4 v) { put_pieces<OP, false>(h + (r * fp + c), p.h_ps, v); });
         if (BWD) {
-            turn_tile(da, S, [&](int r, int c, float4 v) { put_pieces<NP, C::F16>(d + (r * 2 * fp + c), p.dab_ps, v); });
-            turn_tile(db, S, [&](int r, int c, float4 v) { put_pieces<NP, C::F16>(d + (r * 2 * fp + fp + c), p.dab_ps, v); });
+            turn_tile(da, S, [&](int r, int c, float4 v) { put_pieces<OP, false>(d + (r * 2 * fp + c), p.dab_ps, v); });
+            turn_tile(db, S, [&](int r, int c, float4 v) { put_pieces<OP, false>(d + (r * 2 * fp + fp + c), p.dab_ps, v); });
         }
     }
 }
@@ -512,8 +467,7 @@ struct NtParams {
     Planes a, b;
     void *c;
     int64_t ldc, M, N, K;
-    int ncol, ntiles, vec, which;
-    const float *norm;
+    int ncol, ntiles, vec;
 };
 template <int DT, typename C, int BM, int BN>
 __global__ __launch_bounds__(C::NT, 2) void gff_nt_kernel(NtParams p) {
@@ -555,14 +509,12 @@ __global__ __launch_bounds__(C::NT, 2) void gff_nt_kernel(NtParams p) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] += J[((i * TN + j) * 16 + r) * 64 + lane];
     }
-    const float back = C::F16 ? pow2_of(p.norm, p.which, -1) : 1.f;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int64_t rb = m0 + wm * RM + i * 32, cb = n0 + wn * RN + j * 32;
             turn_tile(acc[i][j], S, [&](int r, int c, float4 v) {
-                if (C::F16) v = make_float4(v.x * back, v.y * back, v.z * back, v.w * back);
                 if (rb + r < p.M) put_row4<E>((E *)p.c + (rb + r) * p.ldc, cb + c, p.N, p.vec, v);
             });
         }
@@ -578,8 +530,7 @@ struct TnParams {
     float *part;
     int64_t rows, half, valid, N, part_sz;
     int64_t kt, kt_split;
-    int ncol, ntiles, splits, vec, which;
-    const float *norm;
+    int ncol, ntiles, splits, vec;
 };
 struct TnPair { TnParams p[2]; int blk; };
 template <int DT, typename C, int BM, int BN>
@@ -607,14 +558,12 @@ __global__ __launch_bounds__(C::NT, 2) void gff_tn_kernel(TnPair pair) {
                  [&](const unsigned char *img, int i, int ks) { return frag_tn<BM>(img, wm * RM + i * 32, ks, lane); },
                  [&](const unsigned char *img, int j, int ks) { return frag_tn<BN>(img, wn * RN + j * 32, ks, lane); });
     float *S = reinterpret_cast<float *>(pool) + wave * 1024;
-    const float back = C::F16 ? pow2_of(p.norm, p.which, -1) : 1.f;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int64_t rb = m0 + wm * RM + i * 32, cb = n0 + wn * RN + j * 32;
             turn_tile(acc[i][j], S, [&](int r, int c, float4 v) {
-                if (C::F16) v = make_float4(v.x * back, v.y * back, v.z * back, v.w * back);
                 int64_t row = rb + r;
                 const bool second = row >= p.half;
                 row -= second ? p.half : 0;
@@ -647,27 +596,30 @@ __global__ __launch_bounds__(256) void gff_sum_kernel(TnPair pair) {
 }
 
 // ---------------------------------------------------------------------------------------- packing into planes --
-// Up to 8 matrices in one launch: src (R, C) row-major with pitch lds -> pieces, straight (R, >= C, pitch ldd) or transposed
+// Up to 9 matrices in one launch: src (R, C) row-major with pitch lds -> pieces, straight (R, >= C, pitch ldd) or transposed
 // (C, >= R); columns of the result from the matrix' end to `wide` are zeros.
 struct PackJob {
     const void *src;
     __bf16 *dst;
     int64_t lds, ldd, ps;
-    int R, C, wide, trans, vec;
+    int R, C, wide, trans, vec, as_is;   // as_is: float16 as it lies instead of as pieces
     int blk0;                            // first workgroup of the job
     int nx;                              // workgroups along the source's columns
 };
-struct PackJobs { PackJob j[8]; int n; };
+struct PackJobs { PackJob j[9]; int n; };
 
 template <int DT>
 __global__ __launch_bounds__(256) void gff_pack_kernel(PackJobs jobs) {
     typedef typename FfElem<DT>::type E;
     constexpr int NP = FfElem<DT>::NP;
-    constexpr bool F16 = FfElem<DT>::F16;
     __shared__ float tile[64][65];
     int k = 0;
     while (k + 1 < jobs.n && (int)blockIdx.x >= jobs.j[k + 1].blk0) ++k;
     const PackJob &J = jobs.j[k];
+    auto put = [&](__bf16 *dst, float4 v) {
+        if (DT == ASR_T_F16 && J.as_is) put_pieces<1, true>(dst, 0, v);
+        else put_pieces<NP, false>(dst, J.ps, v);
+    };
     const int b = (int)blockIdx.x - J.blk0, by = b / J.nx, bx = b - by * J.nx;
     const E *src = (const E *)J.src;
     // a 64 x 64 block; source columns (or, transposed, rows) past the end read as zero.  All loads of a thread go out together.
@@ -691,7 +643,7 @@ __global__ __launch_bounds__(256) void gff_pack_kernel(PackJobs jobs) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (r0 + 16 * i < J.R && c0 < J.wide)
-                put_pieces<NP, F16>(J.dst + (int64_t)(r0 + 16 * i) * J.ldd + c0, J.ps, make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
+                put(J.dst + (int64_t)(r0 + 16 * i) * J.ldd + c0, make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
         return;
     }
 #pragma unroll
@@ -703,8 +655,8 @@ __global__ __launch_bounds__(256) void gff_pack_kernel(PackJobs jobs) {
     for (int i = 0; i < 4; ++i) {
         const int c = bx * 64 + tr + 16 * i, r = by * 64 + tc;                 // row and column of the result
         if (c < J.C && r < J.wide)
-            put_pieces<NP, F16>(J.dst + (int64_t)c * J.ldd + r, J.ps,
-                           make_float4(tile[tc][tr + 16 * i], tile[tc + 1][tr + 16 * i], tile[tc + 2][tr + 16 * i], tile[tc + 3][tr + 16 * i]));
+            put(J.dst + (int64_t)c * J.ldd + r,
+                make_float4(tile[tc][tr + 16 * i], tile[tc + 1][tr + 16 * i], tile[tc + 2][tr + 16 * i], tile[tc + 3][tr + 16 * i]));
     }
 }
 
@@ -864,52 +816,48 @@ static TnPlan gff_tn_plan(int NP, int64_t rows, int64_t cols, int64_t M) {
 }
 
 struct GffPlan {
-    int NP;
+    int NP, NG;                          // pieces of h, da, db and what they are multiplied by; of the gate kernel's operands
     int64_t dp, np, fp, Mp;              // padded widths of x / dy / h and rows of h, [da db]
     bool direct_x, direct_wgu, direct_wd, direct_dy;
     TnPlan gu, wd;                       // the weight gradients of [gate; up] and down
     int64_t off[16], bytes;              // workspace: byte offsets
 };
-enum { O_X, O_WG, O_WU, O_WD, O_H, O_DY, O_WDT, O_WGUT, O_DAB, O_PART, O_PART_WD, O_NORM };
+enum { O_X, O_WG, O_WU, O_WD, O_H, O_DY, O_WDT, O_WGUT, O_DAB, O_PART, O_PART_WD, O_XP, O_DYP };
 
 static bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
-// float16 as it lies rounds h, da and db to 11 bits and needs their scale; as pieces they keep 16 bits.  The forward takes it
-// always (3000 x 1024 x 4096: 110 us against 238; 374 x 256 x 2048: 22 against 42): y is off by 1.4 of its own rounding.  In
-// the backward two roundings that partly cancel make that up to 1.5, so it pays there only from some size on (a training call at
-// 1003 x 200 x 683: 106 us, in pieces 97; 4000 x 256 x 2048 160 and 250; 3000 x 1024 x 4096 431 and 918).
-static bool gff_native(const asr_gated_ff_args *a, bool bwd) {
-    return a->dtype == ASR_T_F16 && (!bwd || (double)a->M * a->d * a->f >= (double)(1 << 29));
-}
-// A 16-bit matrix whose k is whole k-tiles is an operand as it lies; every other one is packed into the workspace.
+// A 16-bit matrix whose k is whole k-tiles is an operand as it lies; every other one is packed into the workspace, float16 x and
+// dy once for the gate kernel and once, as pieces, for the weight gradients.
 static void gff_plan(const asr_gated_ff_args *a, bool bwd, GffPlan &p) {
-    p.NP = a->dtype == ASR_T_F32 ? 3 : a->dtype == ASR_T_F16 && !gff_native(a, bwd) ? 2 : 1;
+    p.NP = a->dtype == ASR_T_F32 ? 3 : a->dtype == ASR_T_F16 ? 2 : 1;
+    p.NG = a->dtype == ASR_T_F32 ? 3 : 1;
     p.dp = up_to(a->d, 64);
     p.np = up_to(a->n, 64);
     p.fp = up_to(a->f, 64);
     p.Mp = up_to(a->M, 128);
-    const bool one = p.NP == 1;
+    const bool one = p.NG == 1;
     p.direct_x = one && p.dp == a->d && aligned16(a->x);
     p.direct_wgu = one && p.dp == a->d && aligned16(a->wg) && aligned16(a->wu);
-    p.direct_wd = one && p.fp == a->f && aligned16(a->wd);
+    p.direct_wd = p.NP == 1 && p.fp == a->f && aligned16(a->wd);
     p.direct_dy = one && p.np == a->n && aligned16(a->dy);
     int64_t o = 0;
     auto take = [&](int k, int64_t bytes) {
         p.off[k] = o;
         o += up_to(bytes, 256);
     };
-    const int64_t e = 2 * p.NP;
-    take(O_X, p.direct_x ? 0 : a->M * p.dp * e);
-    take(O_WG, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * e);
-    take(O_WU, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * e);
+    const int64_t e = 2 * p.NP, eg = 2 * p.NG;
+    take(O_X, p.direct_x ? 0 : a->M * p.dp * eg);
+    take(O_WG, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * eg);
+    take(O_WU, p.direct_wgu ? 0 : (int64_t)a->f * p.dp * eg);
     take(O_H, p.Mp * p.fp * e);
-    take(O_NORM, gff_native(a, bwd) ? N_COUNT * NORM_BLOCKS * 4 : 0);
     take(O_WD, p.direct_wd || bwd ? 0 : (int64_t)a->n * p.fp * e);
     if (bwd) {
-        take(O_DY, p.direct_dy ? 0 : a->M * p.np * e);
-        take(O_WDT, (int64_t)a->f * p.np * e);
+        take(O_DY, p.direct_dy ? 0 : a->M * p.np * eg);
+        take(O_WDT, (int64_t)a->f * p.np * eg);
         take(O_WGUT, (int64_t)a->d * 2 * p.fp * e);
         take(O_DAB, p.Mp * 2 * p.fp * e);
+        take(O_XP, p.NP == p.NG ? 0 : a->M * p.dp * e);
+        take(O_DYP, p.NP == p.NG ? 0 : a->M * p.np * e);
         p.gu = gff_tn_plan(p.NP, 2 * p.fp, a->d, a->M);
         p.wd = gff_tn_plan(p.NP, a->n, a->f, a->M);
         take(O_PART, p.gu.splits > 1 ? (int64_t)p.gu.splits * 2 * a->f * a->d * 4 : 0);
@@ -957,7 +905,7 @@ extern "C" int64_t asr_gated_ff_ws_bytes(const asr_gated_ff_args *a, int backwar
     return p.bytes;
 }
 
-static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, int64_t R, int64_t C, int64_t ldd, int64_t ps, int64_t wide, int trans) {
+static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, int64_t R, int64_t C, int64_t ldd, int64_t ps, int64_t wide, int trans, bool as_is) {
     PackJob &k = j.j[j.n++];
     k.src = src;
     k.dst = (__bf16 *)dst;
@@ -968,6 +916,7 @@ static void pack_add(PackJobs &j, int64_t &blocks, const void *src, void *dst, i
     k.C = (int)C;
     k.wide = (int)wide;
     k.trans = trans;
+    k.as_is = as_is;
     k.vec = C % 4 == 0 && (uintptr_t)src % 16 == 0;
     k.blk0 = (int)blocks;
     // straight: the padding columns belong to the last blocks of a row; transposed: to the last blocks of a column
@@ -999,9 +948,9 @@ static int gff_nt_go(NtParams &p, hipStream_t st) {
     return ASR_OK;
 }
 template <int DT>
-static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t N, int64_t K, int which, const float *norm, hipStream_t st) {
+static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t N, int64_t K, hipStream_t st) {
     constexpr int NP = FfElem<DT>::NP;
-    NtParams p{a, b, c, N, M, N, K, 0, 0, (int)(N % 4 == 0 && aligned16(c)), which, norm};
+    NtParams p{a, b, c, N, M, N, K, 0, 0, (int)(N % 4 == 0 && aligned16(c))};
     // The tile that is done first: the compute unit with most tiles has ceil(tiles / 256) of them; `rate` is the matrix work a
     // unit does in a time, `one` the share of it that a lone workgroup reaches where two or three are meant to share the unit
     // (from float32 products of 11968 x 256, k 2048 and 4096, bfloat16 ones of 8192 x 1024: 256 x 128 reaches 1.4 PFLOP/s
@@ -1021,29 +970,30 @@ static int gff_nt(const Planes &a, const Planes &b, void *c, int64_t M, int64_t 
     return gff_nt_go<DT, typename Cfg<DT>::Deep, 64, 64>(p, st);
 }
 
-template <typename C, int BM, int BN, bool BWD>
+template <typename C, int OP, int BM, int BN, bool BWD>
 static int gff_gate_go(GateParams &g, hipStream_t st) {
     g.ncol = cdiv(g.fp, BN);
     g.ntiles = cdiv(g.Mp, BM) * g.ncol;
-    hipLaunchKernelGGL((gff_gate_kernel<C, BM, BN, BWD>), dim3(g.ntiles), dim3(C::NT), 0, st, g);
+    hipLaunchKernelGGL((gff_gate_kernel<C, OP, BM, BN, BWD>), dim3(g.ntiles), dim3(C::NT), 0, st, g);
     ASR_CHECK_LAUNCH("gff_gate_kernel");
     return ASR_OK;
 }
 template <int DT, bool BWD>
 static int gff_gate(GateParams &g, hipStream_t st) {
-    constexpr int NP = FfElem<DT>::NP;
+    typedef Cfg<GateOperands<DT>::V> G;
+    constexpr int NP = G::NP, OP = FfElem<DT>::NP;
     const int64_t rows = cdiv(g.Mp, 256);
     if constexpr (NP == 1) {
         // One piece is bound by the LDS: a wave's 128 x 32 of each product reads 16 B per matrix instruction less than 64 x 32
         // (8192 x 1024 x 4096: 298 -> 274 us with dh, 170 -> 163 us without; k-tiles of 64 would spill, 351 us).  A unit's
         // rounds of these tiles against those of half their size:
         const int64_t wide = (rows * (g.fp / 128) + 255) / 256, narrow = (rows * (g.fp / 64) + 255) / 256;
-        if (g.fp % 128 == 0 && 1.85 * (double)wide <= (double)narrow) return gff_gate_go<typename Cfg<DT>::Gate, 256, 128, BWD>(g, st);
+        if (g.fp % 128 == 0 && 1.85 * (double)wide <= (double)narrow) return gff_gate_go<typename G::Gate, OP, 256, 128, BWD>(g, st);
     }
-    if (rows * (g.fp / 64) >= 256) return gff_gate_go<typename Cfg<DT>::Mid, 256, 64, BWD>(g, st);
+    if (rows * (g.fp / 64) >= 256) return gff_gate_go<typename G::Mid, OP, 256, 64, BWD>(g, st);
     // (1003 x 200 x 683 float16, 88 tiles of 128 x 64: 25 and 17.5 us, in tiles of 64 x 64 16.3 and 11.9)
-    if ((int64_t)cdiv(g.Mp, 128) * (g.fp / 64) < 256) return gff_gate_go<typename Cfg<DT>::Deep, 64, 64, BWD>(g, st);
-    return gff_gate_go<typename Cfg<DT>::Small, 128, 64, BWD>(g, st);
+    if ((int64_t)cdiv(g.Mp, 128) * (g.fp / 64) < 256) return gff_gate_go<typename G::Deep, OP, 64, 64, BWD>(g, st);
+    return gff_gate_go<typename G::Small, OP, 128, 64, BWD>(g, st);
 }
 
 template <int DT, typename C, int BM, int BN>
@@ -1088,6 +1038,7 @@ static int gff_tn(TnPair &pair, int n, int big, int64_t M, hipStream_t st) {
 
 template <int DT>
 static int gff_run(const asr_gated_ff_args *a, bool bwd, hipStream_t st) {
+    constexpr bool TWICE = DT == ASR_T_F16;            // x and dy as they lie for the gate kernel and as pieces for the weight gradients
     GffPlan p;
     gff_plan(a, bwd, p);
     char *ws = (char *)a->ws;
@@ -1097,48 +1048,46 @@ static int gff_run(const asr_gated_ff_args *a, bool bwd, hipStream_t st) {
     Planes wu{p.direct_wgu ? (const __bf16 *)a->wu : at(O_WU), p.dp, (int64_t)a->f * p.dp, a->f};
     Planes wd{p.direct_wd ? (const __bf16 *)a->wd : at(O_WD), p.fp, (int64_t)a->n * p.fp, a->n};
     Planes h{at(O_H), p.fp, p.Mp * p.fp, p.Mp};
-    Planes dy{}, wdt{}, wgut{}, dab{};
+    Planes dy{}, wdt{}, wgut{}, dab{}, xp{}, dyp{};
     PackJobs jobs;
     jobs.n = 0;
     int64_t blocks = 0;
-    if (!p.direct_x) pack_add(jobs, blocks, a->x, at(O_X), a->M, a->d, p.dp, x.ps, p.dp, 0);
+    if (!p.direct_x) pack_add(jobs, blocks, a->x, at(O_X), a->M, a->d, p.dp, x.ps, p.dp, 0, TWICE);
     if (!p.direct_wgu) {
-        pack_add(jobs, blocks, a->wg, at(O_WG), a->f, a->d, p.dp, wg.ps, p.dp, 0);
-        pack_add(jobs, blocks, a->wu, at(O_WU), a->f, a->d, p.dp, wu.ps, p.dp, 0);
+        pack_add(jobs, blocks, a->wg, at(O_WG), a->f, a->d, p.dp, wg.ps, p.dp, 0, TWICE);
+        pack_add(jobs, blocks, a->wu, at(O_WU), a->f, a->d, p.dp, wu.ps, p.dp, 0, TWICE);
     }
-    if (!bwd && !p.direct_wd) pack_add(jobs, blocks, a->wd, at(O_WD), a->n, a->f, p.fp, wd.ps, p.fp, 0);
+    if (!bwd && !p.direct_wd) pack_add(jobs, blocks, a->wd, at(O_WD), a->n, a->f, p.fp, wd.ps, p.fp, 0, false);
     if (bwd) {
         dy = Planes{p.direct_dy ? (const __bf16 *)a->dy : at(O_DY), p.np, a->M * p.np, a->M};
         wdt = Planes{at(O_WDT), p.np, (int64_t)a->f * p.np, a->f};
         wgut = Planes{at(O_WGUT), 2 * p.fp, (int64_t)a->d * 2 * p.fp, a->d};
         dab = Planes{at(O_DAB), 2 * p.fp, p.Mp * 2 * p.fp, p.Mp};
-        if (!p.direct_dy) pack_add(jobs, blocks, a->dy, at(O_DY), a->M, a->n, p.np, dy.ps, p.np, 0);
-        pack_add(jobs, blocks, a->wd, at(O_WDT), a->n, a->f, p.np, wdt.ps, p.np, 1);
-        pack_add(jobs, blocks, a->wg, at(O_WGUT), a->f, a->d, 2 * p.fp, wgut.ps, p.fp, 1);
-        pack_add(jobs, blocks, a->wu, at(O_WGUT) + p.fp, a->f, a->d, 2 * p.fp, wgut.ps, p.fp, 1);
+        xp = TWICE ? Planes{at(O_XP), p.dp, a->M * p.dp, a->M} : x;
+        dyp = TWICE ? Planes{at(O_DYP), p.np, a->M * p.np, a->M} : dy;
+        if (!p.direct_dy) pack_add(jobs, blocks, a->dy, at(O_DY), a->M, a->n, p.np, dy.ps, p.np, 0, TWICE);
+        pack_add(jobs, blocks, a->wd, at(O_WDT), a->n, a->f, p.np, wdt.ps, p.np, 1, TWICE);
+        pack_add(jobs, blocks, a->wg, at(O_WGUT), a->f, a->d, 2 * p.fp, wgut.ps, p.fp, 1, false);
+        pack_add(jobs, blocks, a->wu, at(O_WGUT) + p.fp, a->f, a->d, 2 * p.fp, wgut.ps, p.fp, 1, false);
+        if (TWICE && a->dwg) pack_add(jobs, blocks, a->x, at(O_XP), a->M, a->d, p.dp, xp.ps, p.dp, 0, false);
+        if (TWICE && a->dwd) pack_add(jobs, blocks, a->dy, at(O_DYP), a->M, a->n, p.np, dyp.ps, p.np, 0, false);
     }
     if (jobs.n) {
         ASR_CHECK_ARG(blocks < (1ll << 31), "gated_ff: too many rows");
         hipLaunchKernelGGL((gff_pack_kernel<DT>), dim3((unsigned)blocks), dim3(256), 0, st, jobs);
         ASR_CHECK_LAUNCH("gff_pack_kernel");
     }
-    float *norm = (float *)at(O_NORM);
-    if constexpr (FfElem<DT>::F16) {
-        hipLaunchKernelGGL(gff_norm_kernel, dim3(NORM_BLOCKS, bwd ? N_COUNT : N_DY), dim3(256), 0, st, NormJobs{{x, wg, wu, dy, wdt}}, norm);
-        ASR_CHECK_LAUNCH("gff_norm_kernel");
+    GateParams g{x, wg, wu, dy, wdt, (__bf16 *)h.p, (__bf16 *)dab.p, h.ps, dab.ps, a->M, p.Mp, p.fp, a->f, (int)p.dp, (int)p.np, 0, 0, a->act};
+    if (!bwd) {
+        ASR_CHECK((gff_gate<DT, false>(g, st)));
+        return gff_nt<DT>(h, wd, a->y, a->M, a->n, p.fp, st);
     }
-    GateParams g{x, wg, wu, dy, wdt, (__bf16 *)h.p, (__bf16 *)dab.p, h.ps, dab.ps, a->M, p.Mp, p.fp, a->f, (int)p.dp, (int)p.np, 0, 0, a->act, norm};
-    if constexpr (DT != ASR_T_F16)                                                     // (as pieces only in the backward)
-        if (!bwd) {
-            ASR_CHECK((gff_gate<DT, false>(g, st)));
-            return gff_nt<DT>(h, wd, a->y, a->M, a->n, p.fp, S_H, norm, st);
-        }
     ASR_CHECK((gff_gate<DT, true>(g, st)));
-    if (a->dx) ASR_CHECK(gff_nt<DT>(dab, wgut, a->dx, a->M, a->d, 2 * p.fp, S_DAB, norm, st));
-    const TnParams gu{dab, x, a->dwg, a->dwu, p.gu.splits > 1 ? (float *)at(O_PART) : nullptr, 2 * p.fp, p.fp, a->f, a->d, 2ll * a->f * a->d, 0, 0, 0, 0,
-                      p.gu.splits, (int)(a->d % 4 == 0 && aligned16(a->dwg) && aligned16(a->dwu)), S_DAB, norm};
-    const TnParams down{dy, h, a->dwd, nullptr, p.wd.splits > 1 ? (float *)at(O_PART_WD) : nullptr, a->n, up_to(a->n, 256), a->n, a->f, (int64_t)a->n * a->f,
-                        0, 0, 0, 0, p.wd.splits, (int)(a->f % 4 == 0 && aligned16(a->dwd)), S_H, norm};
+    if (a->dx) ASR_CHECK(gff_nt<DT>(dab, wgut, a->dx, a->M, a->d, 2 * p.fp, st));
+    const TnParams gu{dab, xp, a->dwg, a->dwu, p.gu.splits > 1 ? (float *)at(O_PART) : nullptr, 2 * p.fp, p.fp, a->f, a->d, 2ll * a->f * a->d, 0, 0, 0, 0,
+                      p.gu.splits, (int)(a->d % 4 == 0 && aligned16(a->dwg) && aligned16(a->dwu))};
+    const TnParams down{dyp, h, a->dwd, nullptr, p.wd.splits > 1 ? (float *)at(O_PART_WD) : nullptr, a->n, up_to(a->n, 256), a->n, a->f, (int64_t)a->n * a->f,
+                        0, 0, 0, 0, p.wd.splits, (int)(a->f % 4 == 0 && aligned16(a->dwd))};
     TnPair both{{gu, down}, 0}, one{{gu}, 0}, other{{down}, 0};
     if (a->dwg && a->dwd && !p.gu.big && !p.wd.big) return gff_tn<DT>(both, 2, 0, a->M, st);
     if (a->dwg) ASR_CHECK(gff_tn<DT>(one, 1, p.gu.big, a->M, st));
@@ -1174,7 +1123,7 @@ extern "C" int asr_gated_ff_fwd(const asr_gated_ff_args *a, void *stream) {
     switch (a->dtype) {
         case ASR_T_F32: return few ? gff_few_pick<ASR_T_F32>(a, st) : gff_run<ASR_T_F32>(a, false, st);
         case ASR_T_BF16: return few ? gff_few_pick<ASR_T_BF16>(a, st) : gff_run<ASR_T_BF16>(a, false, st);
-        default: return few ? gff_few_pick<ASR_T_F16>(a, st) : gff_run<F16_AS_IS>(a, false, st);
+        default: return few ? gff_few_pick<ASR_T_F16>(a, st) : gff_run<ASR_T_F16>(a, false, st);
     }
 }
 
@@ -1186,6 +1135,6 @@ extern "C" int asr_gated_ff_bwd(const asr_gated_ff_args *a, void *stream) {
     switch (a->dtype) {
         case ASR_T_F32: return gff_run<ASR_T_F32>(a, true, st);
         case ASR_T_BF16: return gff_run<ASR_T_BF16>(a, true, st);
-        default: return gff_native(a, true) ? gff_run<F16_AS_IS>(a, true, st) : gff_run<ASR_T_F16>(a, true, st);
+        default: return gff_run<ASR_T_F16>(a, true, st);
     }
 }

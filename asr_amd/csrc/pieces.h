@@ -1,9 +1,8 @@
 // Element types of the encoder-layer operators (rope.hip, gated_ff.hip, bucket_attn.hip) and the "pieces" their matrix
 // products are made of.
 //
-// Products run on v_mfma_f32_*_bf16 (but for the float16 ones of gated_ff.hip beyond 64 rows, which have their own way with
-// the range).  A value is held as NP bf16 pieces, x = x0 + x1 + x2 with x0 = bf16(x),
-// x1 = bf16(x - x0), x2 = bf16(x - x0 - x1):
+// Products run on v_mfma_f32_*_bf16 (but for those of float16 inputs in gated_ff.hip beyond 64 rows).  A value is held as NP
+// bf16 pieces, x = x0 + x1 + x2 with x0 = bf16(x), x1 = bf16(x - x0), x2 = bf16(x - x0 - x1):
 //   bfloat16 : NP = 1, exact                       one product
 //   float16  : NP = 2, exact (11 bits = 8 + 3)     x0 y0 + x0 y1 + x1 y0: what is dropped is 2^-16 of a term
 //                                                  (attention's scores: all four, exact)

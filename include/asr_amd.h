@@ -589,7 +589,7 @@ int asr_attdec_bwd_tail(const asr_attdec_bwd_args *a, void *stream);
  * Not in the reference: forms of the same sub-layers that its Conformer encoder (Models/Transformer_encoder.py:55-137,
  * 191-209) computes with sinusoidal positions and a plain Swish block.  Element types: dtype 0 = float32, 1 = bfloat16,
  * 2 = float16; products of all three run on the bf16 matrix cores with 3, 1 and 2 bf16 pieces a value (asr_gated_ff beyond
- * 64 rows: float16 as itself, hidden values times a power of two), sums, norms and softmax statistics are float32. */
+ * 64 rows: float16 inputs as themselves, hidden values in pieces), sums, norms and softmax statistics are float32. */
 
 /* RMS norm of each head of q (B,T,H,D) and k (B,T,Hk,D), times wq / wk (D floats), rotated: pairs (p, p + rot/2) by
  * position * base^(-2p/rot); elements from rot on are not rotated.  Any strides with contiguous heads (strides in
