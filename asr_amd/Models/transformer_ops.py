@@ -79,7 +79,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions=None, rot_dim=None, base=10
         _tensor(who, "q_weight", q_weight, 1, like=q, dtype=torch.float32)
         _tensor(who, "k_weight", k_weight, 1, like=q, dtype=torch.float32)
     B, T, H, D = q.shape
-    if k.shape[0] != B or k.shape[1] != T or k.shape[3] != D:
+    if k.shape[0] != B or k.shape[1] != T or k.shape[3] != D or (H == 0) != (k.shape[2] == 0):
         raise RuntimeError(f"asr_amd.{who}: q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
     if q_weight.shape[0] != D or k_weight.shape[0] != D:
         raise RuntimeError(f"asr_amd.{who}: the weights must hold one value for each of a head's {D} elements")

@@ -74,6 +74,7 @@ variable_list first_order(const variable_list &grads, F compute) {
 // ------------------------------------------------------------------------------------------ norm and rotation --
 asr_rope_args rope_args(const Tensor &q, const Tensor &k, const Tensor &wq, const Tensor &wk, const Tensor &pos, int64_t rot, double base, double eps) {
     asr_rope_args a{};
+    TORCH_CHECK(q.size(2) && k.size(2), "asr_amd.qk_norm_rope: ", q.size(2), " query heads and ", k.size(2), " key heads: both or none");
     a.q = q.data_ptr();
     a.k = k.data_ptr();
     a.wq = ptr<float>(wq);
@@ -92,7 +93,7 @@ asr_rope_args rope_args(const Tensor &q, const Tensor &k, const Tensor &wq, cons
 std::tuple<Tensor, Tensor> rope_fwd(const Tensor &q, const Tensor &k, const Tensor &wq, const Tensor &wk, const optional<Tensor> &pos, int64_t rot,
                                     double base, double eps) {
     Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
-    if (qo.numel()) {
+    if (qo.numel() || ko.numel()) {
         asr_rope_args a = rope_args(q, k, wq, wk, or_none(pos), rot, base, eps);
         a.q_out = qo.data_ptr();
         a.k_out = ko.data_ptr();
@@ -104,7 +105,7 @@ std::tuple<Tensor, Tensor> rope_fwd(const Tensor &q, const Tensor &k, const Tens
 std::tuple<Tensor, Tensor, Tensor, Tensor> rope_bwd(const Tensor &q, const Tensor &k, const Tensor &wq, const Tensor &wk, const optional<Tensor> &pos,
                                                     int64_t rot, double base, double eps, const Tensor &gq0, const Tensor &gk0) {
     Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
-    if (!q.numel()) return {dq, dk, at::zeros_like(wq), at::zeros_like(wk)};
+    if (!q.numel() && !k.numel()) return {dq, dk, at::zeros_like(wq), at::zeros_like(wk)};
     const Tensor gq = heads(gq0), gk = heads(gk0), dwq = floats(wq, wq.sizes()), dwk = floats(wk, wk.sizes());
     const Tensor ws = floats(wq, {asr_qk_norm_rope_ws_floats(size(q, 3))});
     asr_rope_args a = rope_args(q, k, wq, wk, or_none(pos), rot, base, eps);
