@@ -39,7 +39,12 @@ T *ptr(const Tensor &t) { return t.defined() ? static_cast<T *>(t.data_ptr()) : 
 Tensor floats(const Tensor &like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 Tensor bytes(const Tensor &like, int64_t n) { return at::empty({n}, like.options().dtype(at::kByte)); }
 Tensor heads(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+// Whether a call is a node of a graph.  Tangents raise with and without one: past the node they would be dropped in silence.
 bool wanted(std::initializer_list<const Tensor *> ts) {
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        for (const Tensor *t : ts)
+            TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                                        "asr_amd: the encoder-layer operators have no forward-mode derivatives");
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor *t : ts)
         if (t->defined() && t->requires_grad()) return true;

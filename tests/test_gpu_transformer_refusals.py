@@ -23,3 +23,31 @@ def test_norm_and_rotation_of_nothing():
         y = qk_norm_rope(q, k, w, w)
         assert all(o.shape == q.shape for o in y)
         assert not torch.autograd.grad(y, w, [torch.ones_like(o) for o in y])[0].any()
+
+
+def _calls():
+    from asr_amd.Models.transformer_ops import bucket_attention, gated_feed_forward, qk_norm_rope
+    g = torch.Generator().manual_seed(3)
+
+    def n(*shape):
+        return torch.randn(*shape, generator=g).to(DEV)
+    return {"rope": (lambda q, k, a, b: qk_norm_rope(q, k, a, b, rot_dim=16), [n(2, 50, 4, 32), n(2, 50, 2, 32), n(32), n(32)]),
+            "attention": (lambda q, k, v, t: (bucket_attention(q, k, v, t),), [n(2, 50, 4, 32), n(2, 50, 2, 32), n(2, 50, 2, 32), n(32, 4)]),
+            "ff": (lambda x, a, b, c: (gated_feed_forward(x, a, b, c),), [n(2, 35, 24), n(40, 24), n(40, 24), n(24, 40)])}
+
+
+@pytest.mark.parametrize("name", ["rope", "attention", "ff"])
+@pytest.mark.parametrize("leaf", range(4))
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_raise(name, leaf, grad):
+    import torch.autograd.forward_ad as fwd
+    fn, args = _calls()[name]
+    args = [t.requires_grad_(grad) for t in args]
+    with fwd.dual_level():
+        duals = list(args)
+        duals[leaf] = fwd.make_dual(args[leaf], torch.ones_like(args[leaf]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fn(*duals)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            fn(*duals)
+        fn(*args)                                             # no tangent among them

@@ -25,3 +25,27 @@ def test_norm_and_rotation_of_nothing(shape):
         assert out.shape == q.shape
     dq, dk, dwq, dwk = _native().rope_bwd(q, q, w, w, None, 8, 1e4, 1e-6, q, q)
     assert dq.shape == dk.shape == q.shape and not dwq.any() and not dwk.any()
+
+
+def _calls():
+    """The three operators as their Python functions call them, on tensors that no GPU holds."""
+    m, n = _native(), torch.randn
+    return {"rope": (lambda q, k, a, b: m.rope(q, k, a, b, None, 8, 1e4, 1e-6), [n(1, 3, 2, 8), n(1, 3, 1, 8), n(8), n(8)]),
+            "attention": (lambda q, k, v, t: m.attention(q, k, v, t, None, None, None, 0, True, 1.0), [n(1, 3, 2, 8), n(1, 3, 1, 8), n(1, 3, 1, 8), n(2, 2)]),
+            "ff": (lambda x, a, b, c: m.ff(x, a, b, c, 0), [n(3, 8), n(4, 8), n(4, 8), n(8, 4)])}
+
+
+@pytest.mark.parametrize("name", ["rope", "attention", "ff"])
+@pytest.mark.parametrize("leaf", range(4))
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_raise(name, leaf, grad):
+    """A tangent that no kernel carries on must not vanish, whether or not the call is a node of a graph."""
+    import torch.autograd.forward_ad as fwd
+    fn, args = _calls()[name]
+    args = [t.requires_grad_(grad) for t in args]
+    with fwd.dual_level():
+        args[leaf] = fwd.make_dual(args[leaf], torch.ones_like(args[leaf]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fn(*args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            fn(*args)
