@@ -4,6 +4,7 @@
 // been checked by the Python functions; what the C entry points refuse raises with their message.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/asr_amd.h"
@@ -39,8 +40,10 @@ T *ptr(const Tensor &t) { return t.defined() ? static_cast<T *>(t.data_ptr()) : 
 Tensor floats(const Tensor &like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 Tensor bytes(const Tensor &like, int64_t n) { return at::empty({n}, like.options().dtype(at::kByte)); }
 Tensor heads(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
-// Whether a call is a node of a graph.  Tangents raise with and without one: past the node they would be dropped in silence.
+// Whether a call is a node of a graph.  Tangents raise with and without one: past the node they would be dropped in silence.  So
+// does a trace, which would record the allocations and not the kernels.
 bool wanted(std::initializer_list<const Tensor *> ts) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), "asr_amd: the encoder-layer operators cannot be traced: a trace holds torch's own operations only");
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
         for (const Tensor *t : ts)
             TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),

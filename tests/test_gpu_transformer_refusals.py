@@ -51,3 +51,13 @@ def test_tangents_raise(name, leaf, grad):
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             fn(*duals)
         fn(*args)                                             # no tangent among them
+
+
+@pytest.mark.parametrize("name", ["rope", "attention", "ff"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_traces_raise(name, grad):
+    fn, args = _calls()[name]
+    args = tuple(t.requires_grad_(grad) for t in args)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(fn, args, check_trace=False)
+    fn(*args)

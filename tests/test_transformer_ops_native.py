@@ -49,3 +49,13 @@ def test_tangents_raise(name, leaf, grad):
             fn(*args)
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             fn(*args)
+
+
+@pytest.mark.parametrize("name", ["rope", "attention", "ff"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_traces_raise(name, grad):
+    """A trace would hold the outputs' allocation and no kernel."""
+    fn, args = _calls()[name]
+    args = tuple(t.requires_grad_(grad) for t in args)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(fn, args, check_trace=False)
