@@ -3,7 +3,8 @@
 // a few hundred frames keeps the GPU busy for 20 to 40 us, and nodes in Python took 70 to 140 us of host time.  Arguments have
 // been checked by the Python functions; what the C entry points refuse raises with their message.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
@@ -56,26 +57,32 @@ bool wanted(std::initializer_list<const Tensor *> ts) {
 Tensor or_none(const optional<Tensor> &t) { return t ? *t : Tensor(); }
 optional<Tensor> or_null(const Tensor &t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
 
-// A backward pass outside of autograd: where a graph of the gradients is asked for, going through it raises.
+// The operators have first derivatives only.  Where a graph of the gradients is asked for, they come with this node behind
+// them: it depends on all that they depend on, and says so when somebody goes through it.
+struct SecondDerivative : torch::autograd::Node {
+    variable_list apply(variable_list &&) override {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, "asr_amd: an encoder-layer operator was differentiated twice; it has first derivatives only");
+    }
+};
+// `compute` without a graph of its own; grads: the upstream gradients; the first four of `saved` are the inputs
 template <typename F>
-variable_list first_order(const variable_list &grads, F compute) {
+variable_list first_order(const variable_list &grads, const variable_list &saved, F compute) {
     variable_list out;
     {
         at::AutoGradMode off(false);
         out = compute();
     }
     if (!at::GradMode::is_enabled()) return out;
-    bool any = false;
-    for (const Tensor &g : grads) any = any || (g.defined() && g.requires_grad());
-    if (!any) return out;
-    variable_list fresh;
+    torch::autograd::edge_list from;
+    auto add = [&](const Tensor &t) {
+        if (t.defined() && t.requires_grad()) from.push_back(torch::autograd::impl::gradient_edge(t));
+    };
+    for (const Tensor &g : grads) add(g);
+    for (int i = 0; i < 4; ++i) add(saved[i]);
+    std::shared_ptr<SecondDerivative> node(new SecondDerivative(), torch::autograd::deleteNode);
+    node->set_next_edges(std::move(from));
     for (Tensor &t : out)
-        if (t.defined()) fresh.push_back(t.detach().requires_grad_());
-    torch::autograd::DelayedError node("trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)fresh.size());
-    variable_list marked = node.apply(std::move(fresh));
-    size_t k = 0;
-    for (Tensor &t : out)
-        if (t.defined()) t = marked[k++];
+        if (t.defined()) torch::autograd::set_history(t, node);
     return out;
 }
 
@@ -141,8 +148,8 @@ struct Rope : torch::autograd::Function<Rope> {
         return {qo, ko};
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &g) {
-        return first_order(g, [&]() -> variable_list {
-            const variable_list s = ctx->get_saved_variables();
+        const variable_list s = ctx->get_saved_variables();
+        return first_order(g, s, [&]() -> variable_list {
             auto [dq, dk, dwq, dwk] = rope_bwd(s[0], s[1], s[2], s[3], or_null(s[4]), ctx->saved_data["rot"].toInt(), ctx->saved_data["base"].toDouble(),
                                                ctx->saved_data["eps"].toDouble(), g[0], g[1]);
             return {dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor()};
@@ -244,8 +251,8 @@ struct Attention : torch::autograd::Function<Attention> {
         return {o[0]};
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &g) {
-        return first_order(g, [&] {
-            const variable_list s = ctx->get_saved_variables();
+        const variable_list s = ctx->get_saved_variables();
+        return first_order(g, s, [&] {
             variable_list d = attn_bwd_(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8],
                                         {ctx->saved_data["edges"].toInt(), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble()}, g[0]);
             d.resize(10);
@@ -322,8 +329,8 @@ struct GatedFF : torch::autograd::Function<GatedFF> {
         return ff_fwd(x, wg, wu, wd, act);
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &g) {
-        return first_order(g, [&] {
-            const variable_list s = ctx->get_saved_variables();
+        const variable_list s = ctx->get_saved_variables();
+        return first_order(g, s, [&] {
             variable_list d = ff_bwd_(s[0], s[1], s[2], s[3], ctx->saved_data["act"].toInt(), g[0],
                                       {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3)});
             d.resize(5);

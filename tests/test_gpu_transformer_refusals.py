@@ -61,3 +61,27 @@ def test_traces_raise(name, grad):
     with pytest.raises(RuntimeError, match="cannot be traced"):
         torch.jit.trace(fn, args, check_trace=False)
     fn(*args)
+
+
+@pytest.mark.parametrize("name", ["rope", "attention", "ff"])
+def test_a_second_derivative_raises_and_is_never_left_out(name):
+    """Also where the upstream gradient is a constant: the gradients depend on the inputs all the same."""
+    fn, args = _calls()[name]
+    leaves = [t.requires_grad_() for t in args]
+    out = fn(*leaves)
+    grads = torch.autograd.grad(out, leaves, [torch.ones_like(o) for o in out], create_graph=True)
+    assert all(g.requires_grad for g in grads)
+    for i in range(4):
+        with pytest.raises(RuntimeError, match="twice"):
+            torch.autograd.grad((grads[i] ** 2).sum() + (leaves[0] ** 2).sum(), leaves, retain_graph=True, allow_unused=True)
+        for leaf in leaves:                                   # with respect to one input, through any
+            with pytest.raises(RuntimeError, match="twice"):
+                torch.autograd.grad((grads[i] ** 2).sum() + (leaf ** 2).sum(), leaf, retain_graph=True)
+    # as numbers they are the gradients, and what does not go through them has its second derivatives
+    plain = torch.autograd.grad(fn(*leaves), leaves, [torch.ones_like(o) for o in out])
+    assert all(torch.equal(a, b) and not b.requires_grad for a, b in zip(grads, plain))
+    total = sum((o * o).sum() for o in fn(*leaves)) + (leaves[0] ** 3).sum()
+    total.backward(create_graph=True)
+    assert all(t.grad is not None for t in leaves)
+    for t in leaves:
+        t.grad = None
