@@ -750,6 +750,10 @@ class ConformerEncoder(nn.Module):
 
     def forward(self, src, keep):
         T = src.shape[1]
+        # the attention kernels read a byte for every frame
+        if keep.shape != src.shape[:2] or keep.device != src.device or keep.dtype not in (torch.uint8, torch.bool) or not keep.is_contiguous():
+            raise RuntimeError(f"asr_amd ConformerEncoder: keep must be {tuple(src.shape[:2])} contiguous truth values on {src.device}, got "
+                               f"{tuple(keep.shape)} of {keep.dtype} on {keep.device}")
         x, pe = src, None
         if self.attention == "relative":
             if T > 1024:
