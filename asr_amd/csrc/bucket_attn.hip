@@ -340,8 +340,10 @@ __device__ __forceinline__ int keys_of(const AttnParams &p, int b) {
 // ------------------------------------------------------------------------------------------------- forward --
 // With 16-bit tensors a training forward takes P in three pieces: delta, and with it the sum of a row of dS, is
 // as good as O.  Two bfloat16 pieces take 280 us instead of 332 at 2 x 4096 causal, 16 heads of 128, and leave an error of
-// 3.8e-6 in dtable instead of 6e-7.  The returned O is
-// rounded to 16 bits once.
+// 3.8e-6 in dtable instead of 6e-7.  The returned O is rounded to 16 bits once.
+// Without gradients bfloat16 takes P in one piece, 8 bits: O is off by 1.33 of its last rounding, training's by 1.0, and two
+// pieces would take 256 us instead of 203 at 2 x 4096 causal, 16 heads of 128, 21.6 instead of 18.9 at 32 x 374, 4 heads of 64.
+// (Split keys take two: battn_few_kernel.)
 template <int DT, int DP, bool TRAIN>
 __global__ __launch_bounds__(256, ElemOf<DT>::NP * DP > 192 ? 1 : 2) void battn_fwd_kernel(AttnParams p) {
     constexpr int NP = ElemOf<DT>::NP, W = NP < 3 && TRAIN ? 3 : NP, KT = KeyTile<NP>::N;
@@ -801,12 +803,14 @@ __global__ __launch_bounds__(256) void battn_kvsum_kernel(const float *__restric
 // Registers decide: what spills is reloaded behind the loads in flight and waits for them (36 us with the queries and the LDS
 // addresses kept in registers, an index product a load, and a check of D a word).  With one piece the queries therefore lie
 // in LDS and the addresses are formed in the loop.  K as whole lines through LDS, like V: 42 against 36 us.
+// bfloat16 P goes in as two pieces, 16 bits, so that O is off by its last rounding alone (with one piece by 1.2 to 1.3 of it): the
+// matrix cores wait for memory here, and the calls take 0.3 to 0.8 us more (16 caches of 8192: 33.6 against 32.8 us with the join).
 // battn_join_kernel joins the runs.
 template <int DT, int DP, int MODE>
 __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_kernel(AttnParams p) {
     constexpr bool VEC = MODE > 0, FULL = MODE == 2;                                   // rows of 16-byte words; D = DP
     constexpr bool QL = ElemOf<DT>::NP == 1;                                           // the queries are read from LDS
-    constexpr int NP = ElemOf<DT>::NP, IMG = 32 * 2 * DP, CH = DP / 8, NC = DP / 16;
+    constexpr int NP = ElemOf<DT>::NP, PP = NP == 1 ? 2 : NP, IMG = 32 * 2 * DP, CH = DP / 8, NC = DP / 16;
     typedef typename ElemOf<DT>::type E;
     constexpr int W = (int)sizeof(E) / 2;                                              // 16-byte words of eight elements
     extern __shared__ __attribute__((aligned(16))) unsigned char pool[];
@@ -979,9 +983,9 @@ __global__ __launch_bounds__(64, ElemOf<DT>::NP == 1 ? 2 : 1) void battn_few_ker
             s[0][r] = __builtin_amdgcn_exp2f(s[0][r] - ms);
             l += s[0][r];
         }
-        bf16x8 pf[NP][2];
-        to_operand<NP>(pf, s[0]);
-        dot_cols<NP, NP, DP>(o, pool, IMG, 0, pf, ln);
+        bf16x8 pf[PP][2];
+        to_operand<PP>(pf, s[0]);
+        dot_cols<NP, PP, DP>(o, pool, IMG, 0, pf, ln);
         wave_sync();
     }
     l += __shfl_xor(l, 32, 64);

@@ -69,3 +69,17 @@ def test_every_remainder_of_a_tile():
     for more in (0, 1, 15, 30):
         q, k, v, t = _inputs(B, 1, 100, 8, 1, 64, torch.bfloat16, nb=16, seed=more)
         _check(q, k, v, t, lengths=n, offset=n - 1 + reach + more, causal=True, reach=reach)
+
+
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,D,causal", [(3, 1, 700, 8, 2, 64, True), (1, 1, 3000, 4, 4, 128, True), (2, 5, 333, 6, 3, 40, False),
+                                                   (1, 150, 374, 4, 4, 40, False), (2, 33, 1000, 2, 1, 128, True), (1, 100, 500, 2, 2, 96, False)])
+def test_bfloat16_probabilities_keep_16_bits(B, Tq, Tk, H, Hk, D, causal):
+    """Split keys: held to the tolerance of training's forward, whose probabilities have at least 16 bits."""
+    from asr_amd.Models.transformer_ops import bucket_attention
+    g = torch.Generator().manual_seed(11)
+    q, k, v = (torch.randn(B, T, h, D, generator=g).to(torch.bfloat16).to(DEV) for T, h in ((Tq, H), (Tk, Hk), (Tk, Hk)))
+    t = torch.randn(32, H, generator=g).to(DEV)
+    off = torch.full((B,), Tk - Tq, device=DEV, dtype=torch.int32)
+    got = bucket_attention(q, k, v, t, offset=off, causal=causal)
+    held(got, attention64(*(x.double() for x in (q, k, v, t)), None, torch.bfloat16, lengths=None, keep=None, offset=off, causal=causal,
+                          reach=128, scale=D ** -0.5, train=True)[0])
