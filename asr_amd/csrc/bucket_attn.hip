@@ -1065,12 +1065,15 @@ static int64_t bup(int64_t v) { return (v + 255) / 256 * 256; }
 static int battn_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 static int64_t battn_few_tiles(const asr_bucket_attention_args *a) { return ((int64_t)a->H / a->Hk * a->Tq + 31) / 32; }
 // Without gradients the keys are split where there are few queries: one tile of 32 rows a key head, or so few workgroups of
-// 128 queries for so many keys that splitting gains more than the smaller tiles cost.  us, split against not, at B x T, 4 heads
-// of 64: float32 1 x 374 18 / 33, 1 x 1500 57 / 104, 4 x 374 35 / 35, 8 x 374 47 / 38; bfloat16 1 x 374 13 / 15, 1 x 1500 30 / 42,
-// 1 x 150 11 / 9, 4 x 374 21 / 15.  (Several tiles: the biases of a group of at most 32 heads lie in LDS.)
+// 128 queries for so many keys that splitting gains more than the smaller tiles cost, and not one for every compute unit: past
+// that nothing is left to split, and every 32 queries read all keys for themselves.  us, split against not, at B x T, 4 heads
+// of 64: float32 1 x 374 18 / 31, 1 x 1500 57 / 97, 1 x 4096 216 / 246, 1 x 8192 783 / 509, 1 x 16384 2985 / 1543; 4 x 374 35 / 35,
+// 8 x 374 47 / 38; bfloat16 1 x 374 13 / 15, 1 x 1500 31 / 43, 1 x 4096 85 / 107, 1 x 8192 274 / 217, 1 x 16384 750 / 532; 1 x 150
+// 11 / 9, 4 x 374 21 / 15; one head of 64, 1 x 8192 (64 workgroups) float32 213 / 465.
+// (Several tiles: the biases of a group of at most 32 heads lie in LDS.)
 static bool battn_few(const asr_bucket_attention_args *a) {
     const int64_t wgs = (int64_t)a->B * a->H * cdiv(a->Tq, 128);
-    return !a->train && (battn_few_tiles(a) == 1 || (wgs <= a->Tk / (a->dtype == ASR_T_BF16 ? 24 : 16) && a->H / a->Hk <= 32 &&
+    return !a->train && (battn_few_tiles(a) == 1 || (wgs <= a->Tk / (a->dtype == ASR_T_BF16 ? 24 : 16) && wgs < 256 && a->H / a->Hk <= 32 &&
                                                  battn_few_tiles(a) <= 65535));
 }
 

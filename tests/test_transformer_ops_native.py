@@ -59,3 +59,23 @@ def test_traces_raise(name, grad):
     args = tuple(t.requires_grad_(grad) for t in args)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         torch.jit.trace(fn, args, check_trace=False)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_long_utterances_do_not_take_the_form_for_few_queries(dtype):
+    """Told by the workspace: float32 partial rows of the split form, or the planes of the other one."""
+    import ctypes as C
+    from asr_amd import _lib
+    edges = (C.c_int32 * 7)(12, 16, 23, 32, 46, 64, 91)
+
+    def few(T, H):
+        a = _lib.BucketAttentionArgs()
+        a.edges_host = C.addressof(edges)
+        a.B, a.Tq, a.Tk, a.H, a.Hk, a.D, a.nb, a.dtype, a.scale = 1, T, T, H, H, 64, 32, dtype, 1.0
+        # (the pointers' addresses are on the 16-byte grid, strides zero: bfloat16 is an operand as it lies)
+        n = _lib.load().asr_bucket_attention_ws_bytes(C.byref(a), 0)
+        planes = {0: 3, 1: 0, 2: 2}[dtype] * 2 * 64 * 3 * H * T
+        return n != planes
+    assert few(374, 4) and few(1500, 4) and few(4096, 4) and few(8192, 1)
+    for T, H in ((8192, 4), (16384, 4), (32768, 4), (32768, 1), (16384, 2), (1 << 20, 1)):
+        assert not few(T, H), (T, H)
