@@ -101,3 +101,21 @@ def test_one_large_hidden_unit_that_the_output_leaves_out(M, d, f, n):
     # the same sum without the unit: its own products are zeros
     rest = torch.arange(f, device=DEV) != 5
     held(got, gated_ff64(*[t.double() for t in (ts[0], ts[1][rest], ts[2][rest], ts[3][:, rest])], None, "swish", torch.float16)[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("M", [20, 130, 600])
+def test_rows_with_infinities_leave_the_others_as_they_were(M, dtype):
+    from asr_amd.Models.transformer_ops import gated_feed_forward
+    x, wg, wu, wd, dy = (t.to(dtype).to(DEV) for t in _inputs(M, 64, 96, 40))
+    bad_x, bad_dy = x.clone(), dy.clone()
+    bad_x[3, 5], bad_x[7, 0], bad_x[M - 1, 63], bad_dy[11, 2] = float("inf"), float("nan"), -float("inf"), float("nan")
+    rest = torch.ones(M, dtype=torch.bool, device=DEV)
+    rest[[3, 7, 11, M - 1]] = False
+
+    def run(a, g):
+        a = a.detach().requires_grad_()
+        y = gated_feed_forward(a, wg, wu, wd)
+        return y.detach(), torch.autograd.grad(y, a, g)[0]
+    for want, got in zip(run(x, dy), run(bad_x, bad_dy)):
+        assert torch.equal(got[rest], want[rest])
