@@ -9,7 +9,9 @@ Not in the reference, which has sinusoidal relative positions and a plain Swish 
 bfloat16 or float16 on the GPU, all of one type unless said otherwise; anything else raises.  Layouts are (batch, frame,
 head, width); a head must be contiguous, the other strides are free (views of one packed projection need no copy).
 Calls enqueue on the current stream of the tensors' device and return without synchronising; gradients are computed by
-kernels too, without atomics: the same call gives the same bits.
+kernels too, without atomics: the same call gives the same bits.  First derivatives in reverse mode only: a second derivative,
+a forward-mode tangent and a ``torch.jit`` trace raise.  Calls and their backward passes can be captured into a HIP graph; as with
+torch's own operations, no eager graph of the same leaves may be alive then.
 """
 import ctypes as C
 import functools
@@ -159,7 +161,12 @@ def bucket_attention(q, k, v, table=None, lengths=None, keep=None, offset=None, 
     of the buckets is for the keys behind the query.  Keys from ``lengths[b]`` on and keys with ``keep[b, j]`` false are left
     out, whatever they hold (infinities and NaN too); a query that no key is left for gets zeros, and passes no gradient.
     D at most 128, num_buckets at most 256, max_distance at most 1024.  Without gradients, calls with few queries
-    (one new frame against a cache, one utterance at a time) split the keys over the GPU."""
+    (one new frame against a cache, one utterance at a time) split the keys over the GPU.
+
+    Scores, statistics and sums are float32.  Between two products float32 keeps 24 bits of the probabilities and score
+    gradients, float16 16 or more; bfloat16 keeps 24 (16 with split keys) for the output, 16 for dq and 8 for dk, dv and for the
+    output of a call without gradients whose keys are not split: those errors are up to 1.4 of the last rounding, the others' 1.0.  With
+    ``causal``, what a later key of the same 128 queries holds reaches an earlier query only if it is infinite or NaN."""
     who = "bucket_attention"
     if not _like(q, 4, k, v):
         _tensor(who, "q", q, 4)

@@ -13,8 +13,9 @@
 // on both operands: slot (half, e) of a 16-step is row 16 c + 8 (e / 4) + 4 half + e % 4, which is how the transposing LDS
 // reads deliver the left operand).  Nothing is shuffled between the two products.
 //
-// Bound: with 16-bit tensors the vector units, not the matrix cores: a score costs a fused multiply-add, a maximum, a
-// subtraction, an exponential (a quarter-rate instruction), a sum and a conversion, ten times its matrix time at D = 64.  So:
+// Bound: with 16-bit tensors the vector units beside the matrix cores: 64 scores (a register of a wave) cost a fused
+// multiply-add, a maximum, a subtraction, an exponential (a quarter-rate instruction), a sum and half a conversion, 34 cycles, and
+// 16 matrix cycles at D = 64, 32 at D = 128; a training forward's three pieces of P make that 64 there, the larger side.  So:
 // base-2 exponentials with the scale and the bias folded into one multiply-add; the running maximum only moves (and rescales
 // the output) when a score exceeds it by 2^8; tiles that need no mask have none; beyond the last bucket edge the bias is one
 // number per tile; closer, it is one LDS read at a fixed offset from the lane's distance (a line of biases by distance per head).

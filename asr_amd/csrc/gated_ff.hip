@@ -991,7 +991,7 @@ static int gff_gate(GateParams &g, hipStream_t st) {
         if (g.fp % 128 == 0 && 1.85 * (double)wide <= (double)narrow) return gff_gate_go<typename G::Gate, OP, 256, 128, BWD>(g, st);
     }
     if (rows * (g.fp / 64) >= 256) return gff_gate_go<typename G::Mid, OP, 256, 64, BWD>(g, st);
-    // (1003 x 200 x 683 float16, 88 tiles of 128 x 64: 25 and 17.5 us, in tiles of 64 x 64 16.3 and 11.9)
+    // (1003 x 200 x 683 float16, 88 tiles of 128 x 64: 17.4 us with dh and 13.2 without, in tiles of 64 x 64 12.2 and 9.2)
     if ((int64_t)cdiv(g.Mp, 128) * (g.fp / 64) < 256) return gff_gate_go<typename G::Deep, OP, 64, 64, BWD>(g, st);
     return gff_gate_go<typename G::Small, OP, 128, 64, BWD>(g, st);
 }
